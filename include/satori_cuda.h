@@ -182,6 +182,83 @@ SATORI_API int satori_attn_append(satori_attn *a, int layer, int position, const
                                   const float *v, float *out);
 SATORI_API int satori_attn_destroy(satori_attn *a);
 
+/* ------------------------------------------------------------------ many requests: a paged cache */
+/* No counterpart in the reference, whose sessions keep one contiguous cache each
+ * (src/Satori.Core/Model/DenseSession.cs:80-84).  A paged cache holds the keys and values of many sequences
+ * in `pages` pages of `page_tokens` tokens, laid out [layer][page][K, V][kv_head][token][head_dim]; a
+ * sequence is a list of page numbers.  A page is shared only when it is full, so appending to a sequence
+ * never changes another's tokens.  The lowest free page is always taken first.  Calls that copy pages do so
+ * on the context's stream; calls change everything or, on an error, nothing. */
+typedef enum satori_type {
+    SATORI_F32 = 0,     /* the values are GGUF's type ids */
+    SATORI_F16 = 1,
+    SATORI_BF16 = 30
+} satori_type;
+typedef struct satori_pages satori_pages;
+/* page_tokens 16, 32, 64, 128 or 256; head_dim a multiple of 8, at most 256; type a satori_type.  `memory`:
+ * device memory of the caller's, 16-byte aligned, of layers * pages * 2 * kv_heads * page_tokens * head_dim
+ * elements, kept alive until the cache is destroyed; NULL: allocated here.  Its contents are not cleared:
+ * what lies behind a sequence's end is never read into a result.  ctx NULL (and memory NULL): the tables
+ * only, for a host that keeps the pages elsewhere; satori_pages_copies then says what to copy. */
+SATORI_API int satori_pages_create(satori_ctx *ctx, int layers, int pages, int page_tokens, int kv_heads, int head_dim,
+                                   int type, void *memory, satori_pages **out);
+/* Pages in use and free, 1 + the highest page in use, bytes of the cache, its device address. */
+SATORI_API int satori_pages_info(const satori_pages *p, int *used, int *free_pages, int *top, size_t *bytes,
+                                 void **memory);
+/* n new empty sequences. */
+SATORI_API int satori_pages_new(satori_pages *p, int n, int *seqs);
+/* Makes room for counts[i] more tokens at the end of each sequence (SATORI_ERR_CONTEXT_FULL when the pages do
+ * not suffice).  The tokens are unwritten until satori_batch_append_device or the host writes them. */
+SATORI_API int satori_pages_extend(satori_pages *p, int n, const int *seqs, const int *counts);
+/* children[i] = the first positions[i] tokens of parents[i] (positions NULL: all of them; a parent may come
+ * several times).  share != 0: full pages are shared, a partly filled last page is copied.  share == 0: every
+ * page is copied. */
+SATORI_API int satori_pages_fork(satori_pages *p, int n, const int *parents, const int *positions, int share,
+                                 int *children);
+/* Discards the tokens at and after positions[i] (satori_session_rewind for one sequence); a page that the
+ * new end cuts is copied first when other sequences share it. */
+SATORI_API int satori_pages_rewind(satori_pages *p, int n, const int *seqs, const int *positions);
+/* Removes the sequences; pages that no other sequence holds become free. */
+SATORI_API int satori_pages_free(satori_pages *p, int n, const int *seqs);
+/* Moves the live pages to the lowest numbers (those from the number of live pages up go to the free ones
+ * below, both in ascending order): afterwards top == used. */
+SATORI_API int satori_pages_compact(satori_pages *p, int *moved);
+/* The sequence's length and pages (up to `capacity` of them; *count = all). */
+SATORI_API int satori_pages_table(satori_pages *p, int seq, int *length, int *pages, int capacity, int *count);
+/* The (from, to) page pairs that the last fork, rewind or compact copied (up to `capacity` pairs). */
+SATORI_API int satori_pages_copies(satori_pages *p, int *pairs, int capacity, int *count);
+/* Batches that still refer to the cache report SATORI_ERR_DISPOSED from then on. */
+SATORI_API int satori_pages_destroy(satori_pages *p);
+
+/* A decode batch: the sequences of a paged cache that take a step together.  `rope_base` 0: no rotation;
+ * `rotary` 0: the whole head (otherwise a multiple of 8). */
+typedef struct satori_batch satori_batch;
+SATORI_API int satori_batch_create(satori_pages *p, int q_heads, double rope_base, int rotary, satori_batch **out);
+/* Extends each sequence by counts[i] tokens (1 for decoding, more for a prompt chunk, 0 for none) and plans
+ * the step: its query rows are the new tokens, sequence by sequence.  Sequences may not repeat.  The plan
+ * holds for all layers, until one of its sequences changes otherwise (then the calls below are refused).
+ * It is uploaded on the context's stream behind an address that stays the same while the plan fits
+ * (satori_batch_info's `reallocations`), so captured append and attention launches may be replayed after
+ * the next step when their row buffers are large enough for its rows; a step itself cannot be captured. */
+SATORI_API int satori_batch_step(satori_batch *b, int n, const int *seqs, const int *counts);
+/* The step's rows, the segments its keys fall into (a run of pages that sequences share is one), its work
+ * items, and how often the plan's address has changed. */
+SATORI_API int satori_batch_info(const satori_batch *b, int *rows, int *segments, int *items, int *reallocations);
+/* DenseForward.Step's RopeHalf and cache append (DenseForward.cs:135-141) for every row of the step: k is
+ * rotated at its row's position and stored with v in the layer's pages, q (NULL: none) is rotated into q_out
+ * [rows][q_heads * head_dim].  Device pointers on the context's stream; inputs are float32 or of the cache's
+ * type (in_type), rows ldq / ldk / ldv elements apart (0: packed); q_out has the cache's type.  The rotation
+ * is FP64 like RopeHalf's, rounded once. */
+SATORI_API int satori_batch_append_device(satori_batch *b, int layer, int in_type, const void *q, long long ldq,
+                                          const void *k, long long ldk, const void *v, long long ldv, void *q_out);
+/* TransformerOps.GroupedAttention (TransformerOps.cs:140-179) for every row of the step over its sequence's
+ * tokens up to its own position: q [rows][q_heads * head_dim] of the cache's type, rotated and ldq elements
+ * apart (0: packed) -> out of the cache's type or float32 (out_type), ldo apart.  Keys that several of the
+ * step's sequences share are read once for all their rows.  Scores, sums and accumulators are FP32. */
+SATORI_API int satori_batch_attention_device(satori_batch *b, int layer, const void *q, long long ldq, void *out,
+                                             long long ldo, int out_type);
+SATORI_API int satori_batch_destroy(satori_batch *b);
+
 /* ------------------------------------------------------------------ dense decode session */
 /* One tensor of the model description (names follow GGUF: token_embd.weight, blk.N.attn_q.weight ...). */
 typedef struct satori_tensor {

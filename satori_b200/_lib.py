@@ -25,6 +25,7 @@ ERR_OUT_OF_MEMORY = 8
 Q8_0, Q4_0, T2_64, T2_128, T2_256 = 0, 1, 64, 128, 256
 Q4_K, Q6_K = 12, 14
 TB_64, TB_128, TB_256 = 1064, 1128, 1256
+F32, F16, BF16 = 0, 1, 30
 ORDER_EXECUTE, ORDER_SCALAR, ORDER_BATCH, ORDER_TENSOR = 0, 1, 2, 3
 
 
@@ -145,6 +146,24 @@ _SIGS = {
     "satori_gguf_model_desc": (C.c_int, [_vp, C.POINTER(ModelDesc), _vp, C.c_int, _i32p]),
     "satori_session_create_from_gguf": (C.c_int, [_vp, _vp, C.c_int, C.POINTER(_vp)]),
     "satori_stq2_open": (C.c_int, [_vp, C.c_char_p, C.POINTER(_vp)]),
+    "satori_pages_create": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.POINTER(_vp)]),
+    "satori_pages_info": (C.c_int, [_vp, _i32p, _i32p, _i32p, C.POINTER(C.c_size_t), C.POINTER(_vp)]),
+    "satori_pages_new": (C.c_int, [_vp, C.c_int, _vp]),
+    "satori_pages_extend": (C.c_int, [_vp, C.c_int, _vp, _vp]),
+    "satori_pages_fork": (C.c_int, [_vp, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "satori_pages_rewind": (C.c_int, [_vp, C.c_int, _vp, _vp]),
+    "satori_pages_free": (C.c_int, [_vp, C.c_int, _vp]),
+    "satori_pages_compact": (C.c_int, [_vp, _i32p]),
+    "satori_pages_table": (C.c_int, [_vp, C.c_int, _i32p, _vp, C.c_int, _i32p]),
+    "satori_pages_copies": (C.c_int, [_vp, _vp, C.c_int, _i32p]),
+    "satori_pages_destroy": (C.c_int, [_vp]),
+    "satori_batch_create": (C.c_int, [_vp, C.c_int, C.c_double, C.c_int, C.POINTER(_vp)]),
+    "satori_batch_step": (C.c_int, [_vp, C.c_int, _vp, _vp]),
+    "satori_batch_info": (C.c_int, [_vp, _i32p, _i32p, _i32p, _i32p]),
+    "satori_batch_append_device": (C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_longlong, _vp, C.c_longlong, _vp,
+                                             C.c_longlong, _vp]),
+    "satori_batch_attention_device": (C.c_int, [_vp, C.c_int, _vp, C.c_longlong, _vp, C.c_longlong, C.c_int]),
+    "satori_batch_destroy": (C.c_int, [_vp]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -1,0 +1,620 @@
+// batch.cu -- a decode batch over a paged cache: its C ABI, the append of the new tokens, and the merge of
+// partial attention records.
+//
+// A step plans once on the host what every layer repeats: where each new token goes, and which keys are read
+// for which rows together.  The plan is uploaded behind one device pointer that never moves while it fits, so
+// the launches of a step's layers can be captured and replayed for the next steps.
+#include "batch.cuh"
+#include "common.cuh"
+#include "paged_internal.h"
+
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+
+using namespace satori;
+
+struct satori_batch {
+    satori_pages *pages = nullptr;
+    int q_heads = 0, rotary = 0;
+    double rope_base = 0;
+    PlanShape shape = {};
+    Plan plan;
+    struct Member {
+        int id;
+        unsigned version;
+    };
+    std::vector<Member> members;
+    bool planned = false;
+    int reallocations = 0;                     // times that the plan moved: earlier captures repeat an old step
+    // Device buffers; one that grows leaves the old one allocated, so that a graph captured before finds
+    // valid memory (of an old step) and no freed one.
+    int *d_plan = nullptr;
+    size_t plan_ints = 0;
+    uint8_t *d_partials = nullptr;             // [records][rows][dim] floats, then [records][rows] (max, sum)
+    size_t partials = 0;
+    double *d_rope = nullptr;                  // [row][rotary / 2] (cos, sin)
+    size_t rope_rows = 0;
+    std::vector<void *> outgrown;
+    // Upload staging: two pinned buffers in turn, each reused only after its last copy has run.
+    int *h_stage[2] = {nullptr, nullptr};
+    size_t stage_ints[2] = {0, 0};
+    cudaEvent_t staged[2] = {nullptr, nullptr};
+    int turn = 0;
+};
+
+namespace {
+
+template <typename V>
+int place(std::vector<V> const &v, size_t &at)
+{
+    at = (at + 3) / 4 * 4;                     // 16-byte aligned arrays
+    const int here = (int)at;
+    at += v.size() * sizeof(V) / 4;
+    return here;
+}
+
+template <typename V>
+void put(int *base, int at, std::vector<V> const &v)
+{
+    if (!v.empty()) memcpy(base + at, v.data(), v.size() * sizeof(V));
+}
+
+// ------------------------------------------------------------------------------------------- kernels
+
+// The step's RoPE factors: (cos, sin) of TransformerOps.RopeHalf's FP64 angle (TransformerOps.cs:99-118) for
+// every row and pair, the same for every head and layer.
+__global__ void rope_rows_kernel(const DevPlan *plan, double base, int rotary, double *table)
+{
+    const int half = rotary / 2, n = plan->head.rows * half;
+    const int *position = plan_array<int>(plan, plan->row_position);
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+        const int row = i / half, k = i % half;
+        const double angle = __ddiv_rn((double)position[row], pow(base, __ddiv_rn(2.0 * k, (double)rotary)));
+        double sn, cs;
+        sincos(angle, &sn, &cs);
+        table[2 * (size_t)i] = cs;
+        table[2 * (size_t)i + 1] = sn;
+    }
+}
+
+struct AppendArgs {
+    const DevPlan *plan;
+    const void *q, *k, *v;                     // rows ldq / ldk / ldv elements apart; q may be null
+    long long ldq, ldk, ldv;
+    void *q_out;                               // [rows][q_heads * head_dim]
+    uint8_t *pool;                             // the layer's pages
+    int q_heads, kv_heads, head_dim, rotary, page_tokens;
+};
+
+// Loads and stores of 4 values; `wide`: the rows are aligned for one access.
+template <int TYPE>
+__device__ __forceinline__ void load4(const typename Elem<TYPE>::type *p, bool wide, float *f)
+{
+    typedef typename Elem<TYPE>::type T;
+    union {
+        T t[4];
+        float4 f4;
+        uint2 u2;
+    } v;
+    if (wide) {
+        if (TYPE == SATORI_F32)
+            v.f4 = __ldg(reinterpret_cast<const float4 *>(p));
+        else
+            v.u2 = __ldg(reinterpret_cast<const uint2 *>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.t[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = Elem<TYPE>::to_float(v.t[i]);
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store4(typename Elem<TYPE>::type *p, bool wide, const typename Elem<TYPE>::type *t)
+{
+    if (!wide) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = t[i];
+    } else if (TYPE == SATORI_F32) {
+        *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(t);
+    } else {
+        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(t);
+    }
+}
+
+// One thread turns 8 values of one (row, head): two runs of 4, `rotary / 2` apart where they rotate
+// (RopeHalf pairs i and i + rotary / 2), together where they do not.  The products are FP64 like
+// RopeHalf's, rounded once to the output's type.  Bytes bound it: every value is read and written once.
+template <int IN, int TYPE>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, int wide_in, int wide_out)
+{
+    typedef typename Elem<IN>::type TI;
+    typedef typename Elem<TYPE>::type T;
+    const DevPlan *plan = a.plan;
+    const int chunks = a.head_dim / 8, heads = (a.q ? a.q_heads : 0) + 2 * a.kv_heads;
+    const long long n = (long long)plan->head.rows * heads * chunks;
+    const int *page = plan_array<int>(plan, plan->row_page), *slot = plan_array<int>(plan, plan->row_slot);
+    const long long kv_stride = (long long)a.kv_heads * a.page_tokens * a.head_dim;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        const int c = (int)(i % chunks);
+        const long long j = i / chunks;
+        int h = (int)(j % heads);
+        const int row = (int)(j / heads);
+        const TI *src;
+        T *dst;
+        bool rotates = true, wide = wide_out;
+        if (a.q && h < a.q_heads) {
+            src = (const TI *)a.q + row * a.ldq + (long long)h * a.head_dim;
+            dst = (T *)a.q_out + ((long long)row * a.q_heads + h) * a.head_dim;
+        } else {
+            if (a.q) h -= a.q_heads;
+            const bool value = h >= a.kv_heads;
+            if (value) h -= a.kv_heads;
+            src = value ? (const TI *)a.v + row * a.ldv + (long long)h * a.head_dim
+                        : (const TI *)a.k + row * a.ldk + (long long)h * a.head_dim;
+            dst = (T *)a.pool + (2ll * page[row] + value) * kv_stride + (long long)h * a.page_tokens * a.head_dim +
+                  (long long)slot[row] * a.head_dim;
+            rotates = !value;
+            wide = true;
+        }
+        const int half = a.rotary / 2;
+        rotates = rotates && c < a.rotary / 8;
+        const int at = rotates ? 4 * c : 8 * c, step = rotates ? half : 4;
+        float x[4], y[4];
+        load4<IN>(src + at, wide_in, x);
+        load4<IN>(src + at + step, wide_in, y);
+        alignas(16) T ox[4], oy[4];
+        if (rotates) {
+            const double2 *cs = reinterpret_cast<const double2 *>(plan->rope) + (long long)row * half + 4 * c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double2 f = __ldg(cs + e);
+                ox[e] = Elem<TYPE>::from_double(__dsub_rn(__dmul_rn(x[e], f.x), __dmul_rn(y[e], f.y)));
+                oy[e] = Elem<TYPE>::from_double(__dadd_rn(__dmul_rn(x[e], f.y), __dmul_rn(y[e], f.x)));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ox[e] = Elem<TYPE>::from_float(x[e]);
+                oy[e] = Elem<TYPE>::from_float(y[e]);
+            }
+        }
+        store4<TYPE>(dst + at, wide, ox);
+        store4<TYPE>(dst + at + step, wide, oy);
+    }
+}
+
+struct CombineShape {
+    int record_rows, tile_m, slots_per_item, solo_m;
+};
+
+// One warp per (row, query head): out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - max m), over the
+// records of all the row's segments in their order, so the result does not depend on scheduling.
+template <int TYPE>
+__global__ void __launch_bounds__(128) combine_kernel(const BatchAttn a, const CombineShape c)
+{
+    const DevPlan *plan = a.plan;
+    const int lane = threadIdx.x & 31, q_heads = a.kv_heads * a.group;
+    const int *chain_off = plan_array<int>(plan, plan->chain_off);
+    const PlanLink *chain = plan_array<PlanLink>(plan, plan->chain);
+    const PlanSegment *segments = plan_array<PlanSegment>(plan, plan->segments);
+    const PlanTile *tiles = plan_array<PlanTile>(plan, plan->tiles);
+    const PlanSlots *slots = plan_array<PlanSlots>(plan, plan->slots);
+    const long long n = (long long)plan->head.rows * q_heads;
+    for (long long w = blockIdx.x * 4ll + (threadIdx.x >> 5); w < n; w += gridDim.x * 4ll) {
+        const int row = (int)(w / q_heads), head = (int)(w % q_heads), kv_head = head / a.group, g = head % a.group;
+        const int c0 = chain_off[row], c1 = chain_off[row + 1];
+        // Record i of link k: base + i * step, for i < count, at row `at` of the record.
+        auto locate = [&](int k, int &count, int &step, long long &base) -> bool {
+            const PlanLink link = chain[k];
+            const int m = link.index * a.group + g, t = segments[link.segment].tile0 + m / c.tile_m, mt = m % c.tile_m;
+            const PlanSlots s = slots[t * a.kv_heads + kv_head];
+            if (s.first < 0) return false;
+            const bool solo = c.slots_per_item == 1 || tiles[t].m <= c.solo_m;
+            count = solo ? s.items * c.slots_per_item : s.items;
+            step = (solo ? 1 : c.slots_per_item) * c.record_rows;
+            base = (long long)s.first * c.record_rows + mt;    // a large tile's second record follows its first
+            return true;
+        };
+        int count, step;
+        long long base;
+        float top = -INFINITY;
+        bool merge = true;
+        for (int k = c0; k < c1 && merge; ++k) {
+            merge = locate(k, count, step, base);
+            if (!merge) break;                         // the item wrote the output itself
+            for (int i = lane; i < count; i += 32) top = fmaxf(top, plan->part_ml[base + (long long)i * step].x);
+        }
+        if (!merge) continue;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum = 0;
+        float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+        const int d0 = lane * 4, d1 = 128 + lane * 4;
+        for (int k = c0; k < c1; ++k) {
+            locate(k, count, step, base);
+#pragma unroll 4
+            for (int i = 0; i < count; ++i) {
+                const long long at = base + (long long)i * step;
+                const float2 ml = plan->part_ml[at];
+                const float weight = exp2f(ml.x - ref);
+                const float *o = plan->part_o + at * a.head_dim;
+                sum = fmaf(ml.y, weight, sum);
+                if (d0 < a.head_dim) {
+                    const float4 v = *reinterpret_cast<const float4 *>(o + d0);
+                    acc[0].x = fmaf(v.x, weight, acc[0].x);
+                    acc[0].y = fmaf(v.y, weight, acc[0].y);
+                    acc[0].z = fmaf(v.z, weight, acc[0].z);
+                    acc[0].w = fmaf(v.w, weight, acc[0].w);
+                }
+                if (d1 < a.head_dim) {
+                    const float4 v = *reinterpret_cast<const float4 *>(o + d1);
+                    acc[1].x = fmaf(v.x, weight, acc[1].x);
+                    acc[1].y = fmaf(v.y, weight, acc[1].y);
+                    acc[1].z = fmaf(v.z, weight, acc[1].z);
+                    acc[1].w = fmaf(v.w, weight, acc[1].w);
+                }
+            }
+        }
+        const float inverse = 1.0f / sum;
+        const long long to = (long long)row * a.ldo + (long long)head * a.head_dim;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const int d = part ? d1 : d0;
+            if (d >= a.head_dim) continue;
+            const float v[4] = {acc[part].x * inverse, acc[part].y * inverse, acc[part].z * inverse, acc[part].w * inverse};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (a.out_f32)
+                    reinterpret_cast<float *>(a.out)[to + d + e] = v[e];
+                else
+                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + d + e] = Elem<TYPE>::from_float(v[e]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- host side
+
+int check_batch(satori_batch *b)
+{
+    if (!b) return set_error(SATORI_ERR_DISPOSED, "batch is disposed");
+    if (b->pages->disposed) return set_error(SATORI_ERR_DISPOSED, "the batch's paged cache is disposed");
+    return SATORI_OK;
+}
+
+// The tables are still those that the step planned for.
+int check_planned(satori_batch *b)
+{
+    int rc = check_batch(b);
+    if (rc) return rc;
+    if (!b->planned) return set_error(SATORI_ERR_ARGUMENT, "the batch has no step yet");
+    for (const satori_batch::Member &m : b->members) {
+        const PageSequence *s = b->pages->tables.find(m.id);
+        if (!s || s->version != m.version)
+            return set_error(SATORI_ERR_ARGUMENT, "sequence %d changed after the batch's step", m.id);
+    }
+    if (!b->pages->ctx) return set_error(SATORI_ERR_NOT_SUPPORTED, "the cache has no device memory");
+    return SATORI_OK;
+}
+
+// A device buffer of at least `need` units of `unit` bytes; `have` is updated.
+template <typename P>
+cudaError_t grow(satori_batch *b, P *&buffer, size_t &have, size_t need, size_t unit, size_t least)
+{
+    if (need <= have) return cudaSuccess;
+    const size_t count = std::max(std::max(need, 2 * have), least);
+    void *fresh = nullptr;
+    if (buffer) b->outgrown.reserve(b->outgrown.size() + 1);
+    cudaError_t e = cudaMalloc(&fresh, count * unit);
+    if (e != cudaSuccess) return e;
+    if (buffer) {
+        b->outgrown.push_back(buffer);
+    }
+    buffer = static_cast<P *>(fresh);
+    have = count;
+    return cudaSuccess;
+}
+
+size_t record_rows(const satori_batch *) { return (size_t)generic_record_rows(); }
+
+int upload_plan(satori_batch *b)
+{
+    satori_ctx *ctx = b->pages->ctx;
+    DeviceScope scope(ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    const Plan &p = b->plan;
+    DevPlan head = {};
+    head.head = p.head;
+    size_t ints = sizeof(DevPlan) / 4;
+    head.row_position = place(p.row_position, ints);
+    head.row_page = place(p.row_page, ints);
+    head.row_slot = place(p.row_slot, ints);
+    head.chain_off = place(p.chain_off, ints);
+    head.chain = place(p.chain, ints);
+    head.seg_rows = place(p.seg_rows, ints);
+    head.pages = place(p.pages, ints);
+    head.cta_off = place(p.cta_off, ints);
+    head.segments = place(p.segments, ints);
+    head.tiles = place(p.tiles, ints);
+    head.slots = place(p.slots, ints);
+    head.items = place(p.items, ints);
+    if (ints > 0x7fffffff) return set_error(SATORI_ERR_NOT_SUPPORTED, "the step's plan exceeds Int32 limits");
+    const size_t rows = record_rows(b), record = rows * ((size_t)b->pages->head_dim + 2) * 4;
+    const int *old_plan = b->d_plan;
+    cudaError_t e = grow(b, b->d_plan, b->plan_ints, ints, 4, 1 << 16);
+    b->reallocations += old_plan && old_plan != b->d_plan;
+    if (e == cudaSuccess) e = grow(b, b->d_partials, b->partials, (size_t)p.partials, record, 1);
+    if (e == cudaSuccess && b->rotary)
+        e = grow(b, b->d_rope, b->rope_rows, (size_t)p.head.rows, (size_t)b->rotary * 8, 64);
+    if (e != cudaSuccess) return cuda_fail(e, "allocate batch buffers");
+    head.part_o = reinterpret_cast<float *>(b->d_partials);
+    head.part_ml = reinterpret_cast<float2 *>(head.part_o + b->partials * rows * b->pages->head_dim);
+    head.rope = b->d_rope;
+    // The staging buffer's previous copy has run before it is written again.
+    const int t = b->turn;
+    b->turn ^= 1;
+    if (!b->staged[t] && (e = cudaEventCreateWithFlags(&b->staged[t], cudaEventDisableTiming)) != cudaSuccess)
+        return cuda_fail(e, "create event");
+    if ((e = cudaEventSynchronize(b->staged[t])) != cudaSuccess) return cuda_fail(e, "wait for the plan's last upload");
+    if (ints > b->stage_ints[t]) {
+        cudaFreeHost(b->h_stage[t]);
+        b->h_stage[t] = nullptr;
+        b->stage_ints[t] = 0;
+        const size_t count = std::max<size_t>(2 * ints, 1 << 16);
+        e = cudaHostAlloc(reinterpret_cast<void **>(&b->h_stage[t]), count * 4, cudaHostAllocDefault);
+        if (e != cudaSuccess) return cuda_fail(e, "allocate plan staging");
+        b->stage_ints[t] = count;
+    }
+    int *stage = b->h_stage[t];
+    memcpy(stage, &head, sizeof head);
+    put(stage, head.row_position, p.row_position);
+    put(stage, head.row_page, p.row_page);
+    put(stage, head.row_slot, p.row_slot);
+    put(stage, head.chain_off, p.chain_off);
+    put(stage, head.chain, p.chain);
+    put(stage, head.seg_rows, p.seg_rows);
+    put(stage, head.pages, p.pages);
+    put(stage, head.cta_off, p.cta_off);
+    put(stage, head.segments, p.segments);
+    put(stage, head.tiles, p.tiles);
+    put(stage, head.slots, p.slots);
+    put(stage, head.items, p.items);
+    e = cudaMemcpyAsync(b->d_plan, stage, ints * 4, cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = cudaEventRecord(b->staged[t], ctx->stream);
+    if (e == cudaSuccess && b->rotary && p.head.rows) {
+        const long long pairs = (long long)p.head.rows * (b->rotary / 2);
+        const unsigned blocks = (unsigned)std::min<long long>((pairs + 127) / 128, 8ll * ctx->sm_count);
+        rope_rows_kernel<<<blocks, 128, 0, ctx->stream>>>(reinterpret_cast<const DevPlan *>(b->d_plan), b->rope_base,
+                                                         b->rotary, b->d_rope);
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "upload the step's plan");
+}
+
+template <int IN, int TYPE>
+cudaError_t launch_append(const AppendArgs &a, int rows, int wide_in, int wide_out, int sm_count, cudaStream_t stream)
+{
+    const long long n = (long long)rows * ((a.q ? a.q_heads : 0) + 2 * a.kv_heads) * (a.head_dim / 8);
+    const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>((n + 255) / 256, 32ll * sm_count));
+    append_kernel<IN, TYPE><<<blocks, 256, 0, stream>>>(a, wide_in, wide_out);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, int slots_per_item, int solo_m,
+                                   int sm_count, cudaStream_t stream)
+{
+    const CombineShape c = {record_rows, tile_m, slots_per_item, solo_m};
+    const int blocks = 8 * sm_count;
+    switch (a.type) {
+    case SATORI_F32: combine_kernel<SATORI_F32><<<blocks, 128, 0, stream>>>(a, c); break;
+    case SATORI_F16: combine_kernel<SATORI_F16><<<blocks, 128, 0, stream>>>(a, c); break;
+    default: combine_kernel<SATORI_BF16><<<blocks, 128, 0, stream>>>(a, c);
+    }
+    return cudaGetLastError();
+}
+
+extern "C" int satori_batch_create(satori_pages *pages, int q_heads, double rope_base, int rotary, satori_batch **out)
+{
+    return guarded([&]() -> int {
+        if (!out) return set_error(SATORI_ERR_ARGUMENT, "out is null");
+        if (!pages || pages->disposed) return set_error(SATORI_ERR_DISPOSED, "paged cache is disposed");
+        if (q_heads <= 0 || q_heads % pages->kv_heads)
+            return set_error(SATORI_ERR_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
+        if (rope_base != 0 && (!(rope_base > 0) || isinf(rope_base)))
+            return set_error(SATORI_ERR_ARGUMENT, "rope_base must be 0 (no rotation) or positive and finite");
+        if (rope_base != 0 && rotary == 0) rotary = pages->head_dim;
+        if (rotary < 0 || rotary > pages->head_dim || rotary % 8)
+            return set_error(SATORI_ERR_ARGUMENT, "rotary must be a multiple of 8, at most head_dim");
+        satori_batch *b = new satori_batch();
+        b->pages = pages;
+        b->q_heads = q_heads;
+        b->rope_base = rope_base;
+        b->rotary = rope_base != 0 ? rotary : 0;
+        b->shape.page_tokens = pages->tables.page_tokens();
+        b->shape.kv_heads = pages->kv_heads;
+        b->shape.group = q_heads / pages->kv_heads;
+        generic_plan_shape(pages->type, pages->head_dim, pages->ctx ? pages->ctx->sm_count : 148, b->shape);
+        ++pages->users;
+        *out = b;
+        return SATORI_OK;
+    });
+}
+
+extern "C" int satori_batch_step(satori_batch *b, int n, const int *seqs, const int *counts)
+{
+    return guarded([&]() -> int {
+        int rc = check_batch(b);
+        if (rc) return rc;
+        satori_pages *p = b->pages;
+        if (p->ctx) {
+            cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+            cudaError_t e = cudaStreamIsCapturing(p->ctx->stream, &status);
+            if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+            if (status != cudaStreamCaptureStatusNone)
+                return set_error(SATORI_ERR_NOT_SUPPORTED, "a step cannot be planned inside a stream capture");
+        }
+        if (n > 0 && !counts) return set_error(SATORI_ERR_ARGUMENT, "counts is null");
+        long long rows = 0;
+        for (int i = 0; i < n; ++i) rows += counts[i] > 0 ? counts[i] : 0;
+        if (rows * b->q_heads > 0x7fffffff) return set_error(SATORI_ERR_NOT_SUPPORTED, "the step has too many rows");
+        std::vector<PlanMember> members((size_t)std::max(n, 0));
+        std::vector<satori_batch::Member> ids;
+        ids.reserve(members.size());
+        rc = pages_extend(p, n, seqs, counts);
+        if (rc) return rc;                           // the last step's plan still stands
+        b->planned = false;
+        try {
+            for (int i = 0; i < n; ++i) {
+                const PageSequence &s = *p->tables.find(seqs[i]);
+                members[i] = {s.pages.data(), (int)s.pages.size(), s.length, counts[i]};
+                ids.push_back({seqs[i], s.version});
+            }
+            make_plan(b->shape, members, b->plan);
+            if (p->ctx) rc = upload_plan(b);
+        } catch (...) {
+            pages_shrink(p, n, seqs, counts);
+            throw;
+        }
+        if (rc) {
+            pages_shrink(p, n, seqs, counts);
+            return rc;
+        }
+        b->members.swap(ids);
+        b->planned = true;
+        return SATORI_OK;
+    });
+}
+
+extern "C" int satori_batch_info(const satori_batch *batch, int *rows, int *segments, int *items, int *reallocations)
+{
+    satori_batch *b = const_cast<satori_batch *>(batch);
+    int rc = check_batch(b);
+    if (rc) return rc;
+    if (rows) *rows = b->planned ? b->plan.head.rows : 0;
+    if (segments) *segments = b->planned ? b->plan.head.segments : 0;
+    if (items) *items = b->planned ? b->plan.head.items : 0;
+    if (reallocations) *reallocations = b->reallocations;
+    return SATORI_OK;
+}
+
+extern "C" int satori_batch_append_device(satori_batch *b, int layer, int in_type, const void *q, long long ldq,
+                                          const void *k, long long ldk, const void *v, long long ldv, void *q_out)
+{
+    int rc = check_planned(b);
+    if (rc) return rc;
+    satori_pages *p = b->pages;
+    if (layer < 0 || layer >= p->layers) return set_error(SATORI_ERR_ARGUMENT, "layer %d out of range", layer);
+    if (in_type != SATORI_F32 && in_type != p->type)
+        return set_error(SATORI_ERR_ARGUMENT, "inputs must be float32 or of the cache's type");
+    if (b->plan.head.rows == 0) return SATORI_OK;
+    if (!k || !v || (q && !q_out)) return set_error(SATORI_ERR_ARGUMENT, "null argument");
+    const long long qw = (long long)b->q_heads * p->head_dim, kvw = (long long)p->kv_heads * p->head_dim;
+    if (!ldq) ldq = qw;
+    if (!ldk) ldk = kvw;
+    if (!ldv) ldv = kvw;
+    if ((q && ldq < qw) || ldk < kvw || ldv < kvw) return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
+    const size_t es = type_size(in_type), os = type_size(p->type);
+    if ((uintptr_t)k % es || (uintptr_t)v % es || (uintptr_t)q % es || (uintptr_t)q_out % os)
+        return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
+    DeviceScope scope(p->ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    AppendArgs a = {};
+    a.plan = reinterpret_cast<const DevPlan *>(b->d_plan);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.q_out = q_out;
+    a.pool = p->memory + (size_t)layer * p->layer_bytes();
+    a.q_heads = b->q_heads;
+    a.kv_heads = p->kv_heads;
+    a.head_dim = p->head_dim;
+    a.rotary = b->rotary;
+    a.page_tokens = p->tables.page_tokens();
+    const uintptr_t in = (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)(ldk * es) | (uintptr_t)(ldv * es) |
+                         (uintptr_t)(q ? ldq * es : 0);
+    const int wide_in = in % (4 * es) == 0, wide_out = (uintptr_t)q_out % (4 * os) == 0;
+    const int rows = b->plan.head.rows, sms = p->ctx->sm_count;
+    cudaStream_t st = p->ctx->stream;
+    cudaError_t e;
+    if (p->type == SATORI_F32)
+        e = launch_append<SATORI_F32, SATORI_F32>(a, rows, wide_in, wide_out, sms, st);
+    else if (p->type == SATORI_F16)
+        e = in_type == SATORI_F32 ? launch_append<SATORI_F32, SATORI_F16>(a, rows, wide_in, wide_out, sms, st)
+                                  : launch_append<SATORI_F16, SATORI_F16>(a, rows, wide_in, wide_out, sms, st);
+    else
+        e = in_type == SATORI_F32 ? launch_append<SATORI_F32, SATORI_BF16>(a, rows, wide_in, wide_out, sms, st)
+                                  : launch_append<SATORI_BF16, SATORI_BF16>(a, rows, wide_in, wide_out, sms, st);
+    return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "append");
+}
+
+extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const void *q, long long ldq, void *out,
+                                             long long ldo, int out_type)
+{
+    int rc = check_planned(b);
+    if (rc) return rc;
+    satori_pages *p = b->pages;
+    if (layer < 0 || layer >= p->layers) return set_error(SATORI_ERR_ARGUMENT, "layer %d out of range", layer);
+    if (out_type != SATORI_F32 && out_type != p->type)
+        return set_error(SATORI_ERR_ARGUMENT, "outputs must be float32 or of the cache's type");
+    if (b->plan.head.rows == 0) return SATORI_OK;
+    if (!q || !out) return set_error(SATORI_ERR_ARGUMENT, "null argument");
+    const long long qw = (long long)b->q_heads * p->head_dim;
+    if (!ldq) ldq = qw;
+    if (!ldo) ldo = qw;
+    if (ldq < qw || ldo < qw) return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
+    if ((uintptr_t)q % type_size(p->type) || (uintptr_t)out % type_size(out_type))
+        return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
+    DeviceScope scope(p->ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    const size_t rows = record_rows(b);
+    BatchAttn a = {};
+    a.plan = reinterpret_cast<const DevPlan *>(b->d_plan);
+    a.pool = p->memory + (size_t)layer * p->layer_bytes();
+    a.page_tokens = p->tables.page_tokens();
+    a.kv_heads = p->kv_heads;
+    a.group = b->shape.group;
+    a.head_dim = p->head_dim;
+    a.type = p->type;
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.out_f32 = out_type == SATORI_F32;
+    a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
+    a.ctas = b->shape.ctas;
+    a.err = p->ctx->d_err;
+    cudaError_t e = launch_generic_attention(a, p->ctx->stream);
+    if (e == cudaSuccess)
+        e = launch_combine(a, (int)rows, b->shape.tile_m, b->shape.slots_per_item, b->shape.solo_m, p->ctx->sm_count,
+                           p->ctx->stream);
+    return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "batch attention");
+}
+
+extern "C" int satori_batch_destroy(satori_batch *b)
+{
+    if (!b) return SATORI_OK;
+    if (b->pages->ctx) {
+        DeviceScope scope(b->pages->ctx->device);
+        cudaStreamSynchronize(b->pages->ctx->stream);
+        cudaFree(b->d_plan);
+        cudaFree(b->d_partials);
+        cudaFree(b->d_rope);
+        for (void *old : b->outgrown) cudaFree(old);
+        for (int t = 0; t < 2; ++t) {
+            cudaFreeHost(b->h_stage[t]);
+            if (b->staged[t]) cudaEventDestroy(b->staged[t]);
+        }
+    }
+    pages_unref(b->pages);
+    delete b;
+    return SATORI_OK;
+}

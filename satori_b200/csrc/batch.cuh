@@ -1,0 +1,79 @@
+// batch.cuh -- device view of a decode batch's plan, and the launch interfaces of its kernels.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged.h"
+
+namespace satori {
+
+// The plan as the kernels read it: this header, then the arrays it gives the offsets of (in ints from the
+// header's start).  Everything that changes from step to step is behind the one pointer, the work buffers
+// included, so captured launches read the current step's plan and write the buffers that it was sized for.
+struct DevPlan {
+    float *part_o;                   // partial records: [record][record_rows][head_dim], not normalised
+    float2 *part_ml;                 // [record][record_rows]: running maximum (log2 units) and sum
+    const double *rope;              // [row][rotary / 2] (cos, sin)
+    PlanHeader head;
+    int row_position, row_page, row_slot, chain_off, chain, seg_rows, pages, cta_off, segments, tiles, slots, items;
+};
+
+template <typename T>
+__device__ __forceinline__ const T *plan_array(const DevPlan *plan, int offset)
+{
+    return reinterpret_cast<const T *>(reinterpret_cast<const int *>(plan) + offset);
+}
+
+struct BatchAttn {
+    const DevPlan *plan;
+    const uint8_t *pool;             // the layer's pages
+    int page_tokens, kv_heads, group, head_dim, type;
+    const void *q;                   // rows of q_heads * head_dim elements of the cache's type, ldq apart
+    long long ldq;
+    void *out;                       // the same, of the cache's type or float
+    long long ldo;
+    int out_f32;
+    float scale_log2;                // log2(e) / sqrt(head_dim)
+    int ctas;
+    unsigned *err;
+};
+
+// The kernels' share of PlanShape: tile and block sizes, costs and the CTAs a GPU holds at once.
+void generic_plan_shape(int type, int head_dim, int sm_count, PlanShape &shape);
+int generic_record_rows();
+cudaError_t launch_generic_attention(const BatchAttn &a, cudaStream_t stream);
+
+// Merges the partial records of every row that has more than one source and writes its outputs.
+cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, int slots_per_item, int solo_m, int sm_count,
+                           cudaStream_t stream);
+
+// --------------------------------------------------------------------------- element types
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<SATORI_F32> {
+    typedef float type;
+    static __device__ __forceinline__ float to_float(float v) { return v; }
+    static __device__ __forceinline__ float from_float(float v) { return v; }
+    static __device__ __forceinline__ float from_double(double v) { return (float)v; }
+};
+template <>
+struct Elem<SATORI_F16> {
+    typedef __half type;
+    static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ __half from_double(double v) { return __double2half(v); }
+};
+template <>
+struct Elem<SATORI_BF16> {
+    typedef __nv_bfloat16 type;
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_double(double v) { return __double2bfloat16(v); }
+};
+
+}  // namespace satori
