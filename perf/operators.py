@@ -271,7 +271,9 @@ def _prepare_batch(case, seed):
             seqs = cache.fork(root * len(counts))
         else:
             seqs = cache.create(len(counts))
-        cache.extend(seqs, [int(a) - cache.length(q) for a, q in zip(before, seqs)])
+        # Each sequence's pages follow one another: all of its tokens get room, then the step's go again.
+        cache.extend(seqs, [int(a) + n - cache.length(q) for a, n, q in zip(before, counts, seqs)])
+        cache.rewind(seqs, [int(a) for a in before])
         batch = sat.DecodeBatch(cache, case["heads"], rope_base=ROPE_BASE)
         batch.step(seqs, counts)
         s["cache"], s["batch"] = cache, batch
