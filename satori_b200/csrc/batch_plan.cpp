@@ -130,7 +130,8 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
 
     // Deal the blocks to the CTAs in order: segment, KV head, tile, so that tiles that read the same keys
     // run at about the same time.
-    const long long budget = std::max<long long>(1, (total + shape.ctas - 1) / shape.ctas);
+    // A CTA's border may cut a tile's keys into one more item, whose cost the budget has to hold.
+    const long long budget = (total + shape.ctas - 1) / shape.ctas + shape.item_cost;
     plan.cta_off.assign(1, 0);
     long long room = budget;
     for (const PlanSegment &seg : plan.segments) {
