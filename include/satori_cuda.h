@@ -259,6 +259,36 @@ SATORI_API int satori_batch_attention_device(satori_batch *b, int layer, const v
                                              long long ldo, int out_type);
 SATORI_API int satori_batch_destroy(satori_batch *b);
 
+/* ------------------------------------------------------------------ many requests: low-rank adapters */
+/* No counterpart in the reference.  The adapters of one projection: slot s holds A [rank][cols] and
+ * B [rows][rank] of a satori_type, and a scale; row p of a batch with slot s gets
+ * scale * B (A x[p]) added to its projection.  Ranks up to max_rank (at most 128) may differ from slot to
+ * slot; an empty slot (rank 0) adds nothing. */
+typedef struct satori_adapters satori_adapters;
+SATORI_API int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int slots, int max_rank, int type,
+                                      satori_adapters **out);
+/* Copies an adapter into a slot (host or device memory; rows lda / ldb elements apart, 0: packed).  rank 0
+ * empties the slot.  Synchronous: queued work that reads the slot runs first. */
+SATORI_API int satori_adapters_load(satori_adapters *s, int slot, int rank, const void *a, long long lda, const void *b,
+                                    long long ldb, float scale);
+SATORI_API int satori_adapters_destroy(satori_adapters *s);
+/* Which slot each row of a batch uses (-1: none), for all projections of a step.  Captured applications may
+ * be replayed after the next assignment when their row buffers are large enough for its rows. */
+typedef struct satori_adapter_rows satori_adapter_rows;
+SATORI_API int satori_adapter_rows_create(satori_ctx *ctx, satori_adapter_rows **out);
+SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const int *slots);
+SATORI_API int satori_adapter_rows_destroy(satori_adapter_rows *r);
+/* out[p] = base[p] + scale * B (A x[p]) for the assigned rows: device pointers on the context's stream, x
+ * rows of cols floats ldx apart, base and out rows of `rows` floats (0: packed).  out may be base itself and
+ * must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits, FP32 sums. */
+SATORI_API int satori_adapters_apply_device(satori_adapters *s, const satori_adapter_rows *r, const float *x,
+                                            long long ldx, const float *base, long long ldbase, float *out,
+                                            long long ldo);
+/* satori_matrix_execute_device for the assigned rows (dx [rows][cols] -> dy [rows][matrix rows]) with their
+ * adapters added: the shared projection beside each row's own. */
+SATORI_API int satori_matrix_execute_adapted_device(satori_matrix *m, satori_adapters *s, const satori_adapter_rows *r,
+                                                    const float *dx, float *dy, int order);
+
 /* ------------------------------------------------------------------ dense decode session */
 /* One tensor of the model description (names follow GGUF: token_embd.weight, blk.N.attn_q.weight ...). */
 typedef struct satori_tensor {

@@ -13,7 +13,7 @@ from .core import (AttentionCache, BlockQuantization, Context, CudaMatrixFactory
 from .gguf import GgufFile, GgufMetadata, GgufTensor, open_stq2, session_from_gguf
 from .model import (CudaDenseSession, ModelSpec, broadcast_nccl_id, nccl_unique_id, qwen2_1_5b, qwen2_7b,
                     shard_ranges, tiny)
-from .serving import DecodeBatch, PagedCache
+from .serving import AdapterRows, AdapterSet, DecodeBatch, PagedCache
 
 __all__ = [
     "ArgumentError", "ContextFullError", "DeviceError", "DisposedError", "InvalidDataError", "NotSupportedError",
@@ -24,6 +24,6 @@ __all__ = [
     "TernaryBitplaneMatVec", "TransformerOps",
     "default_context", "sharded_matrix_rows", "stq2_header", "stq2_read_header", "ternary2_byte_length", "CudaDenseSession", "ModelSpec",
     "qwen2_1_5b", "qwen2_7b", "tiny", "nccl_unique_id", "broadcast_nccl_id", "shard_ranges",
-    "PagedCache", "DecodeBatch",
+    "PagedCache", "DecodeBatch", "AdapterSet", "AdapterRows",
     "GgufFile", "GgufMetadata", "GgufTensor", "open_stq2", "session_from_gguf",
 ]

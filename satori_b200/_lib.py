@@ -164,6 +164,14 @@ _SIGS = {
                                              C.c_longlong, _vp]),
     "satori_batch_attention_device": (C.c_int, [_vp, C.c_int, _vp, C.c_longlong, _vp, C.c_longlong, C.c_int]),
     "satori_batch_destroy": (C.c_int, [_vp]),
+    "satori_adapters_create": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
+    "satori_adapters_load": (C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_longlong, _vp, C.c_longlong, C.c_float]),
+    "satori_adapters_destroy": (C.c_int, [_vp]),
+    "satori_adapter_rows_create": (C.c_int, [_vp, C.POINTER(_vp)]),
+    "satori_adapter_rows_assign": (C.c_int, [_vp, C.c_int, _vp]),
+    "satori_adapter_rows_destroy": (C.c_int, [_vp]),
+    "satori_adapters_apply_device": (C.c_int, [_vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong]),
+    "satori_matrix_execute_adapted_device": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int]),
 }
 
 EXPORTED = tuple(_SIGS)

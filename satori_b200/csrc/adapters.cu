@@ -1,0 +1,644 @@
+// adapters.cu -- low-rank adapters of many requests beside a shared projection:
+// out[p] = base[p] + scale_s * B_s (A_s x[p]), s the adapter slot of row p.
+//
+// The reference has no adapters; a host that serves fine-tuned variants of one model decodes their rows in one
+// batch, the quantized projection once for all rows (satori_matrix_execute_device) and each row's own
+// low-rank term beside it.
+//
+// One launch.  The rows are grouped by slot into items of at most 16 or 32 rows; a thread-block cluster takes
+// an item: its warps split the columns for t = A x, the partial t meet in shared memory and, across the
+// cluster's CTAs, in distributed shared memory, and the warps split the output rows for B t.  So t never
+// leaves the SMs, x is read once, base and out are touched once, and nothing is added by atomics: the order
+// of every sum is fixed by the shapes.
+//
+// Both products run on the tensor cores at FP32 accuracy: x and t are cut into three bf16 parts each (24
+// bits), a weight into as many as it needs to be exact (bf16 1, fp16 2, fp32 3), and the products of parts
+// above 2^-24 of the whole are added in FP32 (3, 5 and 6 MMAs per step).  Bytes bound it: the weights of the
+// slots in use, x, base and out.
+#include "batch.cuh"
+#include "common.cuh"
+#include "paged_internal.h"
+#include "staging.h"
+
+#include <cooperative_groups.h>
+#include <string.h>
+
+#include <algorithm>
+
+using namespace satori;
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = 8;
+constexpr int kMaxRank = 128, kMaxCluster = 8;
+
+struct SlotDesc {
+    const uint8_t *a, *b;                      // A [rank16][cols32] and B [rows][rank16], zero padded
+    int rank16;                                // rank rounded up to 16; 0: no adapter
+    float scale;
+};
+
+struct RowItem {
+    int slot, row_off, rows;
+};
+
+// Header of a row plan in device memory; the items for 16- and 32-row tiles and the row list follow.
+struct DevRows {
+    int items[2], item_off[2], rows_off, pad[3];
+};
+
+struct AdapterArgs {
+    const DevRows *plan;
+    const SlotDesc *slots;
+    const float *x, *base;
+    float *out;
+    long long ldx, ldbase, ldo;
+    int rows, cols, cols32;                    // output rows, columns, columns rounded up to 32
+    int wide_x, wide_out;                      // 16-byte accesses are possible
+};
+
+// ------------------------------------------------------------------------------------------- bf16 parts
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y)
+{
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&b);
+}
+
+// (x, y) cut into N packed bf16 parts; each residual is exact in FP32.
+template <int N>
+__device__ __forceinline__ void split(float x, float y, uint32_t *part)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        part[i] = pack_bf16(x, y);
+        x = __fsub_rn(x, __uint_as_float(part[i] << 16));
+        y = __fsub_rn(y, __uint_as_float(part[i] & 0xFFFF0000u));
+    }
+}
+
+template <int TYPE>
+struct Weights;
+template <>
+struct Weights<SATORI_BF16> {
+    static constexpr int kParts = 1, kBytes = 2;
+};
+template <>
+struct Weights<SATORI_F16> {
+    static constexpr int kParts = 2, kBytes = 2;
+};
+template <>
+struct Weights<SATORI_F32> {
+    static constexpr int kParts = 3, kBytes = 4;
+};
+
+// 4 consecutive weights as the B fragment of one MMA step: part[i][0] the first two, part[i][1] the others.
+template <int TYPE>
+__device__ __forceinline__ void weight_parts(const uint32_t *raw, uint32_t (*part)[2])
+{
+    if (TYPE == SATORI_BF16) {
+        part[0][0] = raw[0];
+        part[0][1] = raw[1];
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float2 f;
+            if (TYPE == SATORI_F16)
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&raw[h]));
+            else
+                f = make_float2(__uint_as_float(raw[2 * h]), __uint_as_float(raw[2 * h + 1]));
+            uint32_t p[Weights<TYPE>::kParts];
+            split<Weights<TYPE>::kParts>(f.x, f.y, p);
+#pragma unroll
+            for (int i = 0; i < Weights<TYPE>::kParts; ++i) part[i][h] = p[i];
+        }
+    }
+}
+
+__device__ __forceinline__ void mma_bf16(float *d, const uint32_t *a, const uint32_t *b)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// All products of parts i (of a, three) and j (of b) with i + j <= 2, small ones first.
+template <int NB>
+__device__ __forceinline__ void mma_parts(float *d, const uint32_t (*a)[4], const uint32_t (*b)[2])
+{
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (j <= s) mma_bf16(d, a[s - j], b[j]);
+}
+
+// ------------------------------------------------------------------------------------------- the kernel
+// RM: ranks at most, MT: 16-row tiles of an item.
+template <int RM, int MT>
+struct AdapterSmem {
+    static constexpr int TP = 16 * MT;
+    union {
+        float red[kWarps][TP][RM + 4];         // the warps' partial t
+        uint32_t parts[3][TP][RM / 2 + 4];     // t in bf16 parts, pairs of ranks
+    };
+    float t[TP][RM + 4];                       // the CTA's partial t, read by the whole cluster
+    int row[TP];
+};
+
+template <int TYPE, int RM, int MT>
+__global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterArgs a)
+{
+    typedef Weights<TYPE> W;
+    typedef AdapterSmem<RM, MT> Smem;
+    constexpr int TP = Smem::TP, NT = RM / 8;
+    constexpr int RAW = W::kBytes * 8 / 4;     // words of 8 weights
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int *plan = reinterpret_cast<const int *>(a.plan);
+    const int variant = MT - 1, items = a.plan->items[variant];
+    const RowItem *list = reinterpret_cast<const RowItem *>(plan + a.plan->item_off[variant]);
+    const int *rows = plan + a.plan->rows_off;
+
+    for (int it = blockIdx.x / ctas; it < items; it += gridDim.x / ctas) {
+        const RowItem item = list[it];
+        SlotDesc slot = {};
+        if (item.slot >= 0) slot = a.slots[item.slot];
+        const int nt = slot.rank16 / 8;
+        if (tid < TP) sm.row[tid] = tid < item.rows ? rows[item.row_off + tid] : -1;
+        __syncthreads();
+        if (nt > 0) {
+            // t = A x.  Each warp takes every (8 * ctas)-th run of 32 columns.  A lane holds 8 consecutive columns
+            // of a row: the MMA's k index is a permutation of the run's columns, the same for x and A.
+            float acc[MT][NT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
+            for (int k0 = (cta * kWarps + warp) * 32; k0 < a.cols32; k0 += ctas * kWarps * 32) {
+                const int k = k0 + q * 8;
+                float x[MT][2][8];
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int row = sm.row[i * 16 + h * 8 + g];
+                        const float *src = a.x + row * a.ldx + k;
+                        if (row >= 0 && a.wide_x && k + 8 <= a.cols) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 4) {
+                                const float4 v = __ldg(reinterpret_cast<const float4 *>(src + e));
+                                x[i][h][e] = v.x;
+                                x[i][h][e + 1] = v.y;
+                                x[i][h][e + 2] = v.z;
+                                x[i][h][e + 3] = v.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[i][h][e] = row >= 0 && k + e < a.cols ? __ldg(src + e) : 0.0f;
+                        }
+                    }
+                uint32_t raw[NT][RAW];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (j < nt) {
+                        const uint4 *src = reinterpret_cast<const uint4 *>(
+                            slot.a + ((long long)(j * 8 + g) * a.cols32 + k) * W::kBytes);
+#pragma unroll
+                        for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[j][4 * e]) = __ldg(src + e);
+                    }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    uint32_t xa[MT][3][4];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t p[3];
+                                split<3>(x[i][h][4 * s + 2 * e], x[i][h][4 * s + 2 * e + 1], p);
+#pragma unroll
+                                for (int c = 0; c < 3; ++c) xa[i][c][2 * e + h] = p[c];
+                            }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        if (j < nt) {
+                            uint32_t wb[W::kParts][2];
+                            weight_parts<TYPE>(&raw[j][s * RAW / 2], wb);
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) mma_parts<W::kParts>(acc[i][j], xa[i], wb);
+                        }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (j < nt) {
+                        float *d = &sm.red[warp][i * 16 + g][j * 8 + 2 * q];
+                        *reinterpret_cast<float2 *>(d) = make_float2(acc[i][j][0], acc[i][j][1]);
+                        *reinterpret_cast<float2 *>(d + 8 * (RM + 4)) = make_float2(acc[i][j][2], acc[i][j][3]);
+                    }
+            __syncthreads();
+            const int rank = nt * 8;
+            for (int i = tid; i < TP * rank; i += kThreads) {
+                const int p = i / rank, r = i % rank;
+                float sum = 0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) sum += sm.red[w][p][r];
+                sm.t[p][r] = sum;
+            }
+            cluster.sync();
+            // The whole t, scaled, in bf16 parts.
+            for (int i = tid; i < TP * rank / 2; i += kThreads) {
+                const int p = i / (rank / 2), r = 2 * (i % (rank / 2));
+                float2 sum = make_float2(0, 0);
+                for (int c = 0; c < ctas; ++c) {
+                    const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&sm.t[p][r], c));
+                    sum.x += v.x;
+                    sum.y += v.y;
+                }
+                uint32_t part[3];
+                split<3>(sum.x * slot.scale, sum.y * slot.scale, part);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) sm.parts[c][p][r / 2] = part[c];
+            }
+            __syncthreads();
+        }
+        // out = base + B t: each warp takes runs of 32 output rows.  Lane (g, q) ends up with 8 consecutive
+        // outputs, 8 q .. 8 q + 7, of tile rows g and g + 8: column 2 q + e of the MMA's n-tile j stands for
+        // output 8 q + 2 j + e.
+        for (int o0 = (cta * kWarps + warp) * 32; o0 < a.rows; o0 += ctas * kWarps * 32) {
+            float acc[MT][4][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
+            for (int s = 0; s < nt / 2; ++s) {             // 16 ranks: lane q holds 4 consecutive ones
+                uint32_t ta[MT][3][4];
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int c = 0; c < 3; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(&sm.parts[c][i * 16 + h * 8 + g][s * 8 + q * 2]);
+                            ta[i][c][h] = v.x;
+                            ta[i][c][2 + h] = v.y;
+                        }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int o = min(o0 + 8 * (g >> 1) + 2 * j + (g & 1), a.rows - 1);
+                    const uint8_t *src = slot.b + ((long long)o * slot.rank16 + s * 16 + q * 4) * W::kBytes;
+                    uint32_t raw[RAW / 2];
+#pragma unroll
+                    for (int e = 0; e < RAW / 2; e += 2)
+                        *reinterpret_cast<uint2 *>(&raw[e]) = __ldg(reinterpret_cast<const uint2 *>(src) + e / 2);
+                    uint32_t wb[W::kParts][2];
+                    weight_parts<TYPE>(raw, wb);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) mma_parts<W::kParts>(acc[i][j], ta[i], wb);
+                }
+            }
+            const int o = o0 + 8 * q;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = sm.row[i * 16 + h * 8 + g];
+                    if (row < 0) continue;
+                    const float *base = a.base + row * a.ldbase + o;
+                    float *out = a.out + row * a.ldo + o;
+                    if (a.wide_out && o + 8 <= a.rows) {
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2) {
+                            const float4 b = *reinterpret_cast<const float4 *>(base + 2 * j);
+                            *reinterpret_cast<float4 *>(out + 2 * j) =
+                                make_float4(b.x + acc[i][j][2 * h], b.y + acc[i][j][2 * h + 1],
+                                            b.z + acc[i][j + 1][2 * h], b.w + acc[i][j + 1][2 * h + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (o + e < a.rows) out[e] = base[e] + acc[i][e / 2][2 * h + (e & 1)];
+                    }
+                }
+        }
+        cluster.sync();                        // nobody still reads this CTA's t
+    }
+}
+
+}  // namespace
+
+struct satori_adapters {
+    satori_ctx *ctx = nullptr;
+    int rows = 0, cols = 0, slots = 0, max_rank = 0, max_rank16 = 0, type = 0;
+    uint8_t *d_weights = nullptr;
+    SlotDesc *d_slots = nullptr;
+    size_t a_bytes() const { return (size_t)max_rank16 * cols32() * type_size(type); }
+    size_t b_bytes() const { return ((size_t)rows * max_rank16 * type_size(type) + 255) / 256 * 256; }
+    int cols32() const { return (cols + 31) / 32 * 32; }
+};
+
+struct satori_adapter_rows {
+    satori_ctx *ctx = nullptr;
+    int rows = -1, top_slot = -1;              // rows assigned, highest slot used
+    int items[2] = {0, 0};
+    int *d_plan = nullptr;
+    size_t plan_ints = 0;
+    std::vector<void *> outgrown;              // kept for graphs captured before the plan moved
+    Staging staging;
+};
+
+namespace {
+
+template <int TYPE, int RM, int MT>
+cudaError_t launch_variant(const AdapterArgs &a, int items, int sm_count, cudaStream_t stream)
+{
+    auto kernel = adapter_kernel<TYPE, RM, MT>;
+    const size_t smem = sizeof(AdapterSmem<RM, MT>);
+    cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    // The smallest cluster that gives the SMs two CTAs each: few items are spread over many SMs, many items
+    // exchange less.
+    int cluster = 1;
+    while (cluster < kMaxCluster && items * cluster < 2 * sm_count) cluster *= 2;
+    const int clusters = std::max(1, std::min(items, 8 * sm_count / cluster));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int TYPE>
+cudaError_t launch_adapters(const AdapterArgs &a, int rank, const int *items, int sm_count, cudaStream_t stream)
+{
+    if (rank <= 16) return launch_variant<TYPE, 16, 2>(a, items[1], sm_count, stream);
+    if (rank <= 32) return launch_variant<TYPE, 32, 2>(a, items[1], sm_count, stream);
+    if (rank <= 64) return launch_variant<TYPE, 64, 2>(a, items[1], sm_count, stream);
+    return launch_variant<TYPE, 128, 1>(a, items[0], sm_count, stream);
+}
+
+bool overlap(const void *a, size_t na, const void *b, size_t nb)
+{
+    const char *x = (const char *)a, *y = (const char *)b;
+    return x < y + nb && y < x + na;
+}
+
+size_t span(long long rows, long long ld, long long width) { return (size_t)((rows - 1) * ld + width) * 4; }
+
+}  // namespace
+
+extern "C" int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int slots, int max_rank, int type,
+                                      satori_adapters **out)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !out) return set_error(SATORI_ERR_ARGUMENT, "ctx/out is null");
+        if (rows <= 0 || cols <= 0 || slots <= 0 || max_rank <= 0)
+            return set_error(SATORI_ERR_ARGUMENT, "rows/cols/slots/max_rank must be positive");
+        if (rows > (1 << 24) || cols > (1 << 24)) return set_error(SATORI_ERR_NOT_SUPPORTED, "more than 2^24 rows or columns");
+        if (max_rank > kMaxRank) return set_error(SATORI_ERR_NOT_SUPPORTED, "ranks above %d are not supported", kMaxRank);
+        if (!type_size(type)) return set_error(SATORI_ERR_ARGUMENT, "unsupported type %d", type);
+        DeviceScope scope(ctx->device);
+        if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+        satori_adapters *s = new satori_adapters();
+        s->ctx = ctx;
+        s->rows = rows;
+        s->cols = cols;
+        s->slots = slots;
+        s->max_rank = max_rank;
+        s->max_rank16 = (max_rank + 15) / 16 * 16;
+        s->type = type;
+        cudaError_t e = cudaMalloc(&s->d_weights, (s->a_bytes() + s->b_bytes()) * (size_t)slots);
+        if (e == cudaSuccess) e = cudaMalloc(&s->d_slots, sizeof(SlotDesc) * (size_t)slots);
+        if (e == cudaSuccess) e = cudaMemsetAsync(s->d_slots, 0, sizeof(SlotDesc) * (size_t)slots, ctx->stream);
+        if (e != cudaSuccess) {
+            int rc = cuda_fail(e, "allocate adapters");
+            satori_adapters_destroy(s);
+            return rc;
+        }
+        *out = s;
+        return SATORI_OK;
+    });
+}
+
+extern "C" int satori_adapters_load(satori_adapters *s, int slot, int rank, const void *a, long long lda, const void *b,
+                                    long long ldb, float scale)
+{
+    if (!s) return set_error(SATORI_ERR_DISPOSED, "adapters are disposed");
+    if (slot < 0 || slot >= s->slots) return set_error(SATORI_ERR_ARGUMENT, "slot %d out of range", slot);
+    if (rank < 0 || rank > s->max_rank)
+        return set_error(SATORI_ERR_ARGUMENT, "rank %d is outside 0..%d", rank, s->max_rank);
+    if (rank > 0 && (!a || !b)) return set_error(SATORI_ERR_ARGUMENT, "null argument");
+    if (!lda) lda = s->cols;
+    if (!ldb) ldb = rank;
+    if (rank > 0 && (lda < s->cols || ldb < rank)) return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
+    if (!(scale - scale == 0)) return set_error(SATORI_ERR_ARGUMENT, "scale must be finite");
+    satori_ctx *ctx = s->ctx;
+    DeviceScope scope(ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    const size_t es = type_size(s->type), ka = (size_t)s->cols32() * es;
+    const int rank16 = (rank + 15) / 16 * 16;
+    uint8_t *da = s->d_weights + (size_t)slot * s->a_bytes();
+    uint8_t *db = s->d_weights + (size_t)s->slots * s->a_bytes() + (size_t)slot * s->b_bytes();
+    SlotDesc d = {da, db, rank16, scale};
+    cudaError_t e = cudaSuccess;
+    if (rank > 0) {
+        // Padding columns and ranks are zero, so whole tiles may be multiplied.
+        e = cudaMemsetAsync(da, 0, s->a_bytes(), ctx->stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(db, 0, s->b_bytes(), ctx->stream);
+        if (e == cudaSuccess)
+            e = cudaMemcpy2DAsync(da, ka, a, (size_t)lda * es, (size_t)s->cols * es, (size_t)rank, cudaMemcpyDefault, ctx->stream);
+        if (e == cudaSuccess)
+            e = cudaMemcpy2DAsync(db, (size_t)rank16 * es, b, (size_t)ldb * es, (size_t)rank * es, (size_t)s->rows,
+                                  cudaMemcpyDefault, ctx->stream);
+    }
+    if (e == cudaSuccess) e = cudaMemcpyAsync(s->d_slots + slot, &d, sizeof d, cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);      // the caller may reuse its memory
+    return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "load adapter");
+}
+
+extern "C" int satori_adapters_destroy(satori_adapters *s)
+{
+    if (!s) return SATORI_OK;
+    DeviceScope scope(s->ctx->device);
+    cudaStreamSynchronize(s->ctx->stream);
+    cudaFree(s->d_weights);
+    cudaFree(s->d_slots);
+    delete s;
+    return SATORI_OK;
+}
+
+extern "C" int satori_adapter_rows_create(satori_ctx *ctx, satori_adapter_rows **out)
+{
+    return guarded([&]() -> int {
+        if (!ctx || !out) return set_error(SATORI_ERR_ARGUMENT, "ctx/out is null");
+        satori_adapter_rows *r = new satori_adapter_rows();
+        r->ctx = ctx;
+        *out = r;
+        return SATORI_OK;
+    });
+}
+
+extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const int *slots)
+{
+    return guarded([&]() -> int {
+        if (!r) return set_error(SATORI_ERR_DISPOSED, "adapter rows are disposed");
+        if (n < 0 || (n > 0 && !slots)) return set_error(SATORI_ERR_ARGUMENT, "bad slot list");
+        int top = -1;
+        for (int i = 0; i < n; ++i) {
+            if (slots[i] < -1) return set_error(SATORI_ERR_ARGUMENT, "slot %d is negative", slots[i]);
+            top = std::max(top, slots[i]);
+        }
+        satori_ctx *ctx = r->ctx;
+        DeviceScope scope(ctx->device);
+        if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        cudaError_t e = cudaStreamIsCapturing(ctx->stream, &status);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+        if (status != cudaStreamCaptureStatusNone)
+            return set_error(SATORI_ERR_NOT_SUPPORTED, "rows cannot be assigned inside a stream capture");
+        std::vector<int> order((size_t)n);
+        for (int i = 0; i < n; ++i) order[i] = i;
+        std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return slots[x] < slots[y]; });
+        std::vector<RowItem> items[2];
+        for (int i = 0; i < n;) {
+            int end = i;
+            while (end < n && slots[order[end]] == slots[order[i]]) ++end;
+            for (int v = 0; v < 2; ++v)
+                for (int at = i; at < end; at += 16 * (v + 1))
+                    items[v].push_back({slots[order[i]], at, std::min(16 * (v + 1), end - at)});
+            i = end;
+        }
+        DevRows head = {};
+        size_t ints = sizeof(DevRows) / 4;
+        for (int v = 0; v < 2; ++v) {
+            head.items[v] = (int)items[v].size();
+            head.item_off[v] = (int)ints;
+            ints += items[v].size() * sizeof(RowItem) / 4;
+        }
+        head.rows_off = (int)ints;
+        ints += (size_t)n;
+        if (ints > r->plan_ints) {
+            const size_t count = std::max<size_t>(std::max(ints, 2 * r->plan_ints), 1 << 14);
+            int *fresh = nullptr;
+            r->outgrown.reserve(r->outgrown.size() + 1);
+            if ((e = cudaMalloc(&fresh, count * 4)) != cudaSuccess) return cuda_fail(e, "allocate adapter rows");
+            if (r->d_plan) r->outgrown.push_back(r->d_plan);
+            r->d_plan = fresh;
+            r->plan_ints = count;
+            r->rows = -1;                      // nothing there until the upload
+        }
+        void *buffer = nullptr;
+        if ((e = r->staging.take(ints * 4, &buffer)) != cudaSuccess) return cuda_fail(e, "stage adapter rows");
+        int *stage = static_cast<int *>(buffer);
+        memcpy(stage, &head, sizeof head);
+        for (int v = 0; v < 2; ++v)
+            if (n) memcpy(stage + head.item_off[v], items[v].data(), items[v].size() * sizeof(RowItem));
+        if (n) memcpy(stage + head.rows_off, order.data(), (size_t)n * 4);
+        r->rows = -1;
+        if ((e = r->staging.send(r->d_plan, ints * 4, ctx->stream)) != cudaSuccess) return cuda_fail(e, "upload adapter rows");
+        r->rows = n;
+        r->top_slot = top;
+        r->items[0] = head.items[0];
+        r->items[1] = head.items[1];
+        return SATORI_OK;
+    });
+}
+
+extern "C" int satori_adapter_rows_destroy(satori_adapter_rows *r)
+{
+    if (!r) return SATORI_OK;
+    DeviceScope scope(r->ctx->device);
+    cudaStreamSynchronize(r->ctx->stream);
+    cudaFree(r->d_plan);
+    for (void *old : r->outgrown) cudaFree(old);
+    r->staging.release();
+    delete r;
+    return SATORI_OK;
+}
+
+extern "C" int satori_adapters_apply_device(satori_adapters *s, const satori_adapter_rows *r, const float *x, long long ldx,
+                                            const float *base, long long ldbase, float *out, long long ldo)
+{
+    if (!s) return set_error(SATORI_ERR_DISPOSED, "adapters are disposed");
+    if (!r) return set_error(SATORI_ERR_DISPOSED, "adapter rows are disposed");
+    if (r->ctx->device != s->ctx->device) return set_error(SATORI_ERR_ARGUMENT, "adapters and rows are on different devices");
+    if (r->rows < 0) return set_error(SATORI_ERR_ARGUMENT, "no rows are assigned yet");
+    if (r->top_slot >= s->slots)
+        return set_error(SATORI_ERR_ARGUMENT, "slot %d is assigned; these adapters have %d", r->top_slot, s->slots);
+    if (r->rows == 0) return SATORI_OK;
+    if (!x || !base || !out) return set_error(SATORI_ERR_ARGUMENT, "null argument");
+    if (!ldx) ldx = s->cols;
+    if (!ldbase) ldbase = s->rows;
+    if (!ldo) ldo = s->rows;
+    if (ldx < s->cols || ldbase < s->rows || ldo < s->rows)
+        return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
+    if (((uintptr_t)x | (uintptr_t)base | (uintptr_t)out) % 4) return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
+    const size_t nx = span(r->rows, ldx, s->cols), nb = span(r->rows, ldbase, s->rows), no = span(r->rows, ldo, s->rows);
+    if (overlap(out, no, x, nx) || (overlap(out, no, base, nb) && !(out == base && ldo == ldbase)))
+        return set_error(SATORI_ERR_ARGUMENT, "output must not overlap input (or be base itself)");
+    DeviceScope scope(s->ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    AdapterArgs a = {};
+    a.plan = reinterpret_cast<const DevRows *>(r->d_plan);
+    a.slots = s->d_slots;
+    a.x = x;
+    a.base = base;
+    a.out = out;
+    a.ldx = ldx;
+    a.ldbase = ldbase;
+    a.ldo = ldo;
+    a.rows = s->rows;
+    a.cols = s->cols;
+    a.cols32 = s->cols32();
+    a.wide_x = (uintptr_t)x % 16 == 0 && ldx % 4 == 0;
+    a.wide_out = ((uintptr_t)base | (uintptr_t)out) % 16 == 0 && ldbase % 4 == 0 && ldo % 4 == 0;
+    const int sms = s->ctx->sm_count;
+    cudaError_t e;
+    switch (s->type) {
+    case SATORI_F32: e = launch_adapters<SATORI_F32>(a, s->max_rank16, r->items, sms, s->ctx->stream); break;
+    case SATORI_F16: e = launch_adapters<SATORI_F16>(a, s->max_rank16, r->items, sms, s->ctx->stream); break;
+    default: e = launch_adapters<SATORI_BF16>(a, s->max_rank16, r->items, sms, s->ctx->stream);
+    }
+    return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "apply adapters");
+}
+
+extern "C" int satori_matrix_execute_adapted_device(satori_matrix *m, satori_adapters *s, const satori_adapter_rows *r,
+                                                    const float *dx, float *dy, int order)
+{
+    if (!m) return set_error(SATORI_ERR_DISPOSED, "matrix is disposed");
+    if (!s) return set_error(SATORI_ERR_DISPOSED, "adapters are disposed");
+    if (!r) return set_error(SATORI_ERR_DISPOSED, "adapter rows are disposed");
+    if (s->rows != m->rows || s->cols != m->cols)
+        return set_error(SATORI_ERR_ARGUMENT, "adapters of %d x %d beside a %d x %d matrix", s->rows, s->cols, m->rows, m->cols);
+    if (s->ctx != m->ctx) return set_error(SATORI_ERR_ARGUMENT, "adapters and matrix belong to different contexts");
+    if (r->rows < 0) return set_error(SATORI_ERR_ARGUMENT, "no rows are assigned yet");
+    if (r->top_slot >= s->slots)
+        return set_error(SATORI_ERR_ARGUMENT, "slot %d is assigned; these adapters have %d", r->top_slot, s->slots);
+    if (r->rows == 0) return SATORI_OK;
+    if (dx && dy && overlap(dy, span(r->rows, m->rows, m->rows), dx, span(r->rows, m->cols, m->cols)))
+        return set_error(SATORI_ERR_ARGUMENT, "output must not overlap input");
+    DeviceScope scope(m->ctx->device);
+    if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    int rc = satori_matrix_execute_device(m, dx, dy, r->rows, order);
+    return rc ? rc : satori_adapters_apply_device(s, r, dx, 0, dy, 0, dy, 0);
+}

@@ -7,6 +7,7 @@
 #include "batch.cuh"
 #include "common.cuh"
 #include "paged_internal.h"
+#include "staging.h"
 
 #include <math.h>
 #include <string.h>
@@ -37,11 +38,7 @@ struct satori_batch {
     double *d_rope = nullptr;                  // [row][rotary / 2] (cos, sin)
     size_t rope_rows = 0;
     std::vector<void *> outgrown;
-    // Upload staging: two pinned buffers in turn, each reused only after its last copy has run.
-    int *h_stage[2] = {nullptr, nullptr};
-    size_t stage_ints[2] = {0, 0};
-    cudaEvent_t staged[2] = {nullptr, nullptr};
-    int turn = 0;
+    Staging staging;
 };
 
 namespace {
@@ -354,22 +351,9 @@ int upload_plan(satori_batch *b)
     head.part_o = reinterpret_cast<float *>(b->d_partials);
     head.part_ml = reinterpret_cast<float2 *>(head.part_o + b->partials * rows * b->pages->head_dim);
     head.rope = b->d_rope;
-    // The staging buffer's previous copy has run before it is written again.
-    const int t = b->turn;
-    b->turn ^= 1;
-    if (!b->staged[t] && (e = cudaEventCreateWithFlags(&b->staged[t], cudaEventDisableTiming)) != cudaSuccess)
-        return cuda_fail(e, "create event");
-    if ((e = cudaEventSynchronize(b->staged[t])) != cudaSuccess) return cuda_fail(e, "wait for the plan's last upload");
-    if (ints > b->stage_ints[t]) {
-        cudaFreeHost(b->h_stage[t]);
-        b->h_stage[t] = nullptr;
-        b->stage_ints[t] = 0;
-        const size_t count = std::max<size_t>(2 * ints, 1 << 16);
-        e = cudaHostAlloc(reinterpret_cast<void **>(&b->h_stage[t]), count * 4, cudaHostAllocDefault);
-        if (e != cudaSuccess) return cuda_fail(e, "allocate plan staging");
-        b->stage_ints[t] = count;
-    }
-    int *stage = b->h_stage[t];
+    void *buffer = nullptr;
+    if ((e = b->staging.take(ints * 4, &buffer)) != cudaSuccess) return cuda_fail(e, "stage the step's plan");
+    int *stage = static_cast<int *>(buffer);
     memcpy(stage, &head, sizeof head);
     put(stage, head.row_position, p.row_position);
     put(stage, head.row_page, p.row_page);
@@ -383,8 +367,7 @@ int upload_plan(satori_batch *b)
     put(stage, head.tiles, p.tiles);
     put(stage, head.slots, p.slots);
     put(stage, head.items, p.items);
-    e = cudaMemcpyAsync(b->d_plan, stage, ints * 4, cudaMemcpyHostToDevice, ctx->stream);
-    if (e == cudaSuccess) e = cudaEventRecord(b->staged[t], ctx->stream);
+    e = b->staging.send(b->d_plan, ints * 4, ctx->stream);
     if (e == cudaSuccess && b->rotary && p.head.rows) {
         const long long pairs = (long long)p.head.rows * (b->rotary / 2);
         const unsigned blocks = (unsigned)std::min<long long>((pairs + 127) / 128, 8ll * ctx->sm_count);
@@ -609,10 +592,7 @@ extern "C" int satori_batch_destroy(satori_batch *b)
         cudaFree(b->d_partials);
         cudaFree(b->d_rope);
         for (void *old : b->outgrown) cudaFree(old);
-        for (int t = 0; t < 2; ++t) {
-            cudaFreeHost(b->h_stage[t]);
-            if (b->staged[t]) cudaEventDestroy(b->staged[t]);
-        }
+        b->staging.release();
     }
     pages_unref(b->pages);
     delete b;

@@ -3,7 +3,8 @@
 The reference decodes one sequence per session (``DenseSession``); this module mirrors the part of the C ABI
 that a host needs to serve many: ``PagedCache`` (sequences as lists of pages, forked without copying their
 full pages), ``DecodeBatch`` (append and grouped attention for the new tokens of several sequences; keys that
-sequences share are read once).  Device vectors are torch CUDA tensors, or any object with ``data_ptr``,
+sequences share are read once), ``AdapterSet`` and ``AdapterRows`` (the low-rank adapters of each row's
+request beside a shared projection).  Device vectors are torch CUDA tensors, or any object with ``data_ptr``,
 ``dtype``, ``shape`` and ``stride``; the work is queued on the context's stream.
 """
 from __future__ import annotations
@@ -14,7 +15,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import ArgumentError, DisposedError, check
-from .core import Context, default_context
+from .core import Context, CudaQuantizedMatrix, default_context
 
 _vp = C.c_void_p
 
@@ -267,6 +268,134 @@ class DecodeBatch:
     def dispose(self) -> None:
         if self._h:
             _lib.lib().satori_batch_destroy(self._h)
+            self._h = _vp()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.dispose()
+
+    def __del__(self):
+        try:
+            self.dispose()
+        except Exception:
+            pass
+
+
+class AdapterRows:
+    """Which adapter slot each row of a batch uses (-1: none), for all projections of a step."""
+
+    def __init__(self, ctx: Context | None = None):
+        self._h = _vp()
+        self.ctx = ctx or default_context()
+        h = _vp()
+        check(_lib.lib().satori_adapter_rows_create(self.ctx.handle, C.byref(h)), "adapter_rows_create")
+        self._h = h
+        self.rows = 0
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise DisposedError(_lib.ERR_DISPOSED, "adapter rows are disposed")
+        return self._h
+
+    def assign(self, slots) -> None:
+        s = _ints(slots, "slots")
+        check(_lib.lib().satori_adapter_rows_assign(self.handle, s.size, s.ctypes.data), "adapter_rows_assign")
+        self.rows = s.size
+
+    def dispose(self) -> None:
+        if self._h:
+            _lib.lib().satori_adapter_rows_destroy(self._h)
+            self._h = _vp()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.dispose()
+
+    def __del__(self):
+        try:
+            self.dispose()
+        except Exception:
+            pass
+
+
+class AdapterSet:
+    """The low-rank adapters of one projection of `rows` x `columns`: slot s adds
+    scale * B (A x) with A [rank, columns] and B [rows, rank]."""
+
+    def __init__(self, rows: int, columns: int, slots: int, max_rank: int, dtype="bf16", ctx: Context | None = None):
+        self._h = _vp()
+        self.ctx = ctx or default_context()
+        self.type = _type(dtype)
+        h = _vp()
+        check(_lib.lib().satori_adapters_create(self.ctx.handle, rows, columns, slots, max_rank, self.type, C.byref(h)),
+              "adapters_create")
+        self._h = h
+        self.rows, self.columns, self.slots = rows, columns, slots
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise DisposedError(_lib.ERR_DISPOSED, "adapters are disposed")
+        return self._h
+
+    def load(self, slot: int, a, b, scale: float = 1.0) -> None:
+        """A [rank, columns] and B [rows, rank]: CUDA tensors or host arrays / CPU tensors of the set's type;
+        rows may be strided."""
+        rank = int(a.shape[0])
+        if tuple(a.shape) != (rank, self.columns) or tuple(b.shape) != (self.rows, rank) or rank < 1:
+            raise _bad(f"A {tuple(a.shape)} and B {tuple(b.shape)} do not fit {self.rows} x {self.columns}")
+        (ap, lda, keep_a), (bp, ldb, keep_b) = self._weights(a, "A"), self._weights(b, "B")
+        check(_lib.lib().satori_adapters_load(self.handle, slot, rank, ap, lda, bp, ldb, scale), "adapters_load")
+        del keep_a, keep_b
+
+    def unload(self, slot: int) -> None:
+        """Empties a slot: its rows get their projection alone."""
+        check(_lib.lib().satori_adapters_load(self.handle, slot, 0, None, 0, None, 0, 0.0), "adapters_unload")
+
+    def _weights(self, w, name: str) -> tuple:
+        """(address, row stride in elements, what to keep alive)."""
+        if not hasattr(w, "data_ptr"):
+            w = np.asarray(w)
+            kinds = {"float32": _lib.F32, "float16": _lib.F16}
+            if kinds.get(str(w.dtype)) != self.type:
+                raise _bad(f"{name} has type {w.dtype}")
+            w = np.ascontiguousarray(w)
+            return w.ctypes.data, w.shape[1], w
+        if _TORCH_TYPES.get(str(w.dtype)) != self.type:
+            raise _bad(f"{name} has type {w.dtype}")
+        if w.is_cuda and w.device.index != self.ctx.device:
+            raise _bad(f"{name} is not on device {self.ctx.device}")
+        if (w.shape[1] > 1 and w.stride(1) != 1) or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
+            w = w.contiguous()
+        return w.data_ptr(), (w.stride(0) if w.shape[0] > 1 else w.shape[1]), w
+
+    def apply_device(self, rows: AdapterRows, x, base, out) -> None:
+        """out[p] = base[p] + scale * B (A x[p]) for the assigned rows (float32 device rows; out may be base)."""
+        device = self.ctx.device
+        xp, ldx, _ = _rows(x, rows.rows, self.columns, "x", device, (_lib.F32,))
+        bp, ldb, _ = _rows(base, rows.rows, self.rows, "base", device, (_lib.F32,))
+        op, ldo, _ = _rows(out, rows.rows, self.rows, "out", device, (_lib.F32,))
+        check(_lib.lib().satori_adapters_apply_device(self.handle, rows.handle, xp, ldx, bp, ldb, op, ldo),
+              "adapters_apply")
+
+    def execute_device(self, matrix: CudaQuantizedMatrix, rows: AdapterRows, x, out, order: int = _lib.ORDER_BATCH) -> None:
+        """The quantized projection of the assigned rows with their adapters added (packed float32 rows)."""
+        device = self.ctx.device
+        xp, ldx, _ = _rows(x, rows.rows, self.columns, "x", device, (_lib.F32,))
+        op, ldo, _ = _rows(out, rows.rows, self.rows, "out", device, (_lib.F32,))
+        if ldx != self.columns or ldo != self.rows:
+            raise _bad("x and out must be packed")
+        check(_lib.lib().satori_matrix_execute_adapted_device(matrix.handle, self.handle, rows.handle, xp, op, order),
+              "execute_adapted")
+
+    def dispose(self) -> None:
+        if self._h:
+            _lib.lib().satori_adapters_destroy(self._h)
             self._h = _vp()
 
     def __enter__(self):
