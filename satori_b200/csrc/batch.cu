@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const BatchAttn a, const C
             for (int i = 0; i < count; ++i) {
                 const long long at = base + (long long)i * step;
                 const float2 ml = plan->part_ml[at];
+                if (ml.x == -INFINITY) continue;       // no key: the record may hold no accumulator
                 const float weight = exp2f(ml.x - ref);
                 const float *o = plan->part_o + at * a.head_dim;
                 sum = fmaf(ml.y, weight, sum);
@@ -316,7 +317,12 @@ cudaError_t grow(satori_batch *b, P *&buffer, size_t &have, size_t need, size_t 
     return cudaSuccess;
 }
 
-size_t record_rows(const satori_batch *) { return (size_t)generic_record_rows(); }
+bool on_tensor_cores(const satori_batch *b) { return tensor_attention_takes(b->pages->type, b->pages->head_dim); }
+
+size_t record_rows(const satori_batch *b)
+{
+    return (size_t)(on_tensor_cores(b) ? tensor_record_rows() : generic_record_rows());
+}
 
 int upload_plan(satori_batch *b)
 {
@@ -422,7 +428,11 @@ extern "C" int satori_batch_create(satori_pages *pages, int q_heads, double rope
         b->shape.page_tokens = pages->tables.page_tokens();
         b->shape.kv_heads = pages->kv_heads;
         b->shape.group = q_heads / pages->kv_heads;
-        generic_plan_shape(pages->type, pages->head_dim, pages->ctx ? pages->ctx->sm_count : 148, b->shape);
+        const int sms = pages->ctx ? pages->ctx->sm_count : 148;
+        if (on_tensor_cores(b))
+            tensor_plan_shape(sms, b->shape);
+        else
+            generic_plan_shape(pages->type, pages->head_dim, sms, b->shape);
         ++pages->users;
         *out = b;
         return SATORI_OK;
@@ -575,7 +585,9 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
     a.ctas = b->shape.ctas;
     a.err = p->ctx->d_err;
-    cudaError_t e = launch_generic_attention(a, p->ctx->stream);
+    cudaError_t e = on_tensor_cores(b)
+                        ? launch_tensor_attention(a, p->map, layer * p->tables.pages() * 2 * p->kv_heads, p->ctx->stream)
+                        : launch_generic_attention(a, p->ctx->stream);
     if (e == cudaSuccess)
         e = launch_combine(a, (int)rows, b->shape.tile_m, b->shape.slots_per_item, b->shape.solo_m, p->ctx->sm_count,
                            p->ctx->stream);

@@ -47,6 +47,14 @@ void generic_plan_shape(int type, int head_dim, int sm_count, PlanShape &shape);
 int generic_record_rows();
 cudaError_t launch_generic_attention(const BatchAttn &a, cudaStream_t stream);
 
+// The tensor-core kernel of 16-bit caches with heads of 64 or 128.
+bool tensor_attention_takes(int type, int head_dim);
+void tensor_plan_shape(int sm_count, PlanShape &shape);
+int tensor_record_rows();
+// The cache as a 3-D tensor [block][token][dim] of (layer, page, K or V, head) blocks.
+cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim, int page_tokens, unsigned long long blocks);
+cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
+
 // Merges the partial records of every row that has more than one source and writes its outputs.
 cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, int slots_per_item, int solo_m, int sm_count,
                            cudaStream_t stream);

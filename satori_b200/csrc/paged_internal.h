@@ -19,6 +19,7 @@ struct satori_pages {
     bool owned = false;                        // allocated here
     bool disposed = false;
     int users = 0;                             // decode batches that point here
+    alignas(64) CUtensorMap map = {};          // the memory as the tensor-core attention loads it
     std::vector<int> copies;                   // (from, to) page pairs of the last fork / rewind / compact
 
     satori_pages(int pages, int page_tokens) : tables(pages, page_tokens) {}

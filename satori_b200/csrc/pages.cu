@@ -7,6 +7,7 @@
 //
 // Page copies (a fork's or rewind's partly filled page, a compaction's moves) are one launch for all pairs
 // and all layers.  A copy reads and writes every byte once, so HBM bounds it.
+#include "batch.cuh"
 #include "common.cuh"
 #include "paged_internal.h"
 
@@ -225,6 +226,15 @@ extern "C" int satori_pages_create(satori_ctx *ctx, int layers, int pages, int p
                 return cuda_fail(e, "allocate paged cache");
             }
             p->owned = true;
+        }
+        if (ctx && tensor_attention_takes(type, head_dim)) {
+            DeviceScope scope(ctx->device);
+            cudaError_t e = make_page_map(&p->map, p->memory, type, head_dim, page_tokens,
+                                          (unsigned long long)layers * pages * 2 * kv_heads);
+            if (e != cudaSuccess) {
+                satori_pages_destroy(p);
+                return cuda_fail(e, "describe the cache for TMA");
+            }
         }
         *out = p;
         return SATORI_OK;
