@@ -184,94 +184,117 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, int wid
 }
 
 struct CombineShape {
-    int record_rows, tile_m, slots_per_item, solo_m;
+    int record_rows, tile_m, by_column, octets;
 };
 
-// One warp per (row, query head): out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - max m), over the
-// records of all the row's segments in their order, so the result does not depend on scheduling.
+// out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - max m), over the records of all the row's segments
+// in their order, so the result does not depend on scheduling.  A block takes one row and up to 8 query
+// heads of a KV head: their values lie side by side in the records.  16 threads find a head's records and
+// weights; then all threads add the accumulators, 4 values each.
 template <int TYPE>
 __global__ void __launch_bounds__(128) combine_kernel(const BatchAttn a, const CombineShape c)
 {
+    constexpr int kHeads = 8, kChunk = 64;
+    __shared__ long long base[kHeads][kChunk];
+    __shared__ float weight[kHeads][kChunk], total[kHeads];
+    __shared__ int count[kHeads];
+    pdl_wait();      // and no early start for the next launch: its blocks would take the SMs from this one's
     const DevPlan *plan = a.plan;
-    const int lane = threadIdx.x & 31, q_heads = a.kv_heads * a.group;
+    const int tid = threadIdx.x, mine = tid >> 4, lane16 = tid & 15;
+    const int quads = a.head_dim / 4;
     const int *chain_off = plan_array<int>(plan, plan->chain_off);
     const PlanLink *chain = plan_array<PlanLink>(plan, plan->chain);
-    const PlanSegment *segments = plan_array<PlanSegment>(plan, plan->segments);
-    const PlanTile *tiles = plan_array<PlanTile>(plan, plan->tiles);
     const PlanSlots *slots = plan_array<PlanSlots>(plan, plan->slots);
-    const long long n = (long long)plan->head.rows * q_heads;
-    for (long long w = blockIdx.x * 4ll + (threadIdx.x >> 5); w < n; w += gridDim.x * 4ll) {
-        const int row = (int)(w / q_heads), head = (int)(w % q_heads), kv_head = head / a.group, g = head % a.group;
+    const long long units = (long long)plan->head.rows * a.kv_heads * c.octets;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+        const int g0 = (int)(u % c.octets) * kHeads, heads = min(kHeads, a.group - g0);
+        const int kv_head = (int)(u / c.octets % a.kv_heads), row = (int)(u / c.octets / a.kv_heads);
         const int c0 = chain_off[row], c1 = chain_off[row + 1];
-        // Record i of link k: base + i * step, for i < count, at row `at` of the record.
-        auto locate = [&](int k, int &count, int &step, long long &base) -> bool {
-            const PlanLink link = chain[k];
-            const int m = link.index * a.group + g, t = segments[link.segment].tile0 + m / c.tile_m, mt = m % c.tile_m;
-            const PlanSlots s = slots[t * a.kv_heads + kv_head];
-            if (s.first < 0) return false;
-            const bool solo = c.slots_per_item == 1 || tiles[t].m <= c.solo_m;
-            count = solo ? s.items * c.slots_per_item : s.items;
-            step = (solo ? 1 : c.slots_per_item) * c.record_rows;
-            base = (long long)s.first * c.record_rows + mt;    // a large tile's second record follows its first
-            return true;
+        // Calls f(place, row in the record, record) for this thread's records of its head, in order; the number
+        // of the head's records, or -1 where its item wrote the output itself.
+        auto walk = [&](auto f) -> int {
+            int at = 0;
+            for (int k = c0; k < c1; ++k) {
+                const PlanLink link = chain[k];
+                const int m = link.index * a.group + g0 + mine, mt = m % c.tile_m;
+                const PlanSlots s = slots[(link.tile0 + m / c.tile_m) * a.kv_heads + kv_head];
+                if (s.first < 0) return -1;
+                const int first = s.first + mt / c.record_rows;    // a large tile's second record follows its first
+                const int n = s.records / s.step;
+                for (int i = lane16; i < n; i += 16) f(at + i, mt % c.record_rows, first + i * s.step);
+                at += n;
+            }
+            return at;
         };
-        int count, step;
-        long long base;
+        const bool active = mine < heads;
         float top = -INFINITY;
-        bool merge = true;
-        for (int k = c0; k < c1 && merge; ++k) {
-            merge = locate(k, count, step, base);
-            if (!merge) break;                         // the item wrote the output itself
-            for (int i = lane; i < count; i += 32) top = fmaxf(top, plan->part_ml[base + (long long)i * step].x);
-        }
-        if (!merge) continue;
+        int n = -1;
+        if (active)
+            n = walk([&](int, int r, int record) { top = fmaxf(top, plan->part_ml[(long long)record * c.record_rows + r].x); });
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         const float ref = top == -INFINITY ? 0.0f : top;
         float sum = 0;
-        float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-        const int d0 = lane * 4, d1 = 128 + lane * 4;
-        for (int k = c0; k < c1; ++k) {
-            locate(k, count, step, base);
+        float4 acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = make_float4(0, 0, 0, 0);
+        if (lane16 == 0) count[mine] = n;
+        __syncthreads();
+        int most = 0;
+        for (int g = 0; g < heads; ++g) most = max(most, count[g]);
+        for (int chunk = 0; chunk < most; chunk += kChunk) {
+            if (n > chunk)
+                walk([&](int at, int r, int record) {
+                    if (at < chunk || at >= chunk + kChunk) return;
+                    const float2 ml = plan->part_ml[(long long)record * c.record_rows + r];
+                    const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - ref);  // no key: nothing was stored
+                    sum += w == 0 ? 0.0f : w * ml.y;
+                    weight[mine][at - chunk] = w;
+                    base[mine][at - chunk] = (long long)record * c.record_rows * quads + (c.by_column ? r : r * quads);
+                });
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = tid + j * 128;
+                if (i >= heads * quads) continue;
+                const int g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
+                const long long off = c.by_column ? (long long)quad * c.record_rows : quad;
+                const int end = min(kChunk, count[g] - chunk);
 #pragma unroll 4
-            for (int i = 0; i < count; ++i) {
-                const long long at = base + (long long)i * step;
-                const float2 ml = plan->part_ml[at];
-                if (ml.x == -INFINITY) continue;       // no key: the record may hold no accumulator
-                const float weight = exp2f(ml.x - ref);
-                const float *o = plan->part_o + at * a.head_dim;
-                sum = fmaf(ml.y, weight, sum);
-                if (d0 < a.head_dim) {
-                    const float4 v = *reinterpret_cast<const float4 *>(o + d0);
-                    acc[0].x = fmaf(v.x, weight, acc[0].x);
-                    acc[0].y = fmaf(v.y, weight, acc[0].y);
-                    acc[0].z = fmaf(v.z, weight, acc[0].z);
-                    acc[0].w = fmaf(v.w, weight, acc[0].w);
-                }
-                if (d1 < a.head_dim) {
-                    const float4 v = *reinterpret_cast<const float4 *>(o + d1);
-                    acc[1].x = fmaf(v.x, weight, acc[1].x);
-                    acc[1].y = fmaf(v.y, weight, acc[1].y);
-                    acc[1].z = fmaf(v.z, weight, acc[1].z);
-                    acc[1].w = fmaf(v.w, weight, acc[1].w);
+                for (int f = 0; f < end; ++f) {
+                    const float w = weight[g][f];
+                    const float4 v = *(reinterpret_cast<const float4 *>(plan->part_o) + base[g][f] + off);
+                    if (w == 0) continue;
+                    acc[j].x = fmaf(v.x, w, acc[j].x);
+                    acc[j].y = fmaf(v.y, w, acc[j].y);
+                    acc[j].z = fmaf(v.z, w, acc[j].z);
+                    acc[j].w = fmaf(v.w, w, acc[j].w);
                 }
             }
+            __syncthreads();
         }
-        const float inverse = 1.0f / sum;
-        const long long to = (long long)row * a.ldo + (long long)head * a.head_dim;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-            const int d = part ? d1 : d0;
-            if (d >= a.head_dim) continue;
-            const float v[4] = {acc[part].x * inverse, acc[part].y * inverse, acc[part].z * inverse, acc[part].w * inverse};
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane16 == 0) total[mine] = sum;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = tid + j * 128;
+            if (i >= heads * quads) continue;
+            const int g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
+            if (count[g] < 0) continue;
+            const float inverse = 1.0f / total[g];
+            const float v[4] = {acc[j].x * inverse, acc[j].y * inverse, acc[j].z * inverse, acc[j].w * inverse};
+            const long long to = (long long)row * a.ldo + (long long)(kv_head * a.group + g0 + g) * a.head_dim + quad * 4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (a.out_f32)
-                    reinterpret_cast<float *>(a.out)[to + d + e] = v[e];
+                    reinterpret_cast<float *>(a.out)[to + e] = v[e];
                 else
-                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + d + e] = Elem<TYPE>::from_float(v[e]);
+                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + e] = Elem<TYPE>::from_float(v[e]);
             }
         }
+        __syncthreads();
     }
 }
 
@@ -341,8 +364,6 @@ int upload_plan(satori_batch *b)
     head.seg_rows = place(p.seg_rows, ints);
     head.pages = place(p.pages, ints);
     head.cta_off = place(p.cta_off, ints);
-    head.segments = place(p.segments, ints);
-    head.tiles = place(p.tiles, ints);
     head.slots = place(p.slots, ints);
     head.items = place(p.items, ints);
     if (ints > 0x7fffffff) return set_error(SATORI_ERR_NOT_SUPPORTED, "the step's plan exceeds Int32 limits");
@@ -369,8 +390,6 @@ int upload_plan(satori_batch *b)
     put(stage, head.seg_rows, p.seg_rows);
     put(stage, head.pages, p.pages);
     put(stage, head.cta_off, p.cta_off);
-    put(stage, head.segments, p.segments);
-    put(stage, head.tiles, p.tiles);
     put(stage, head.slots, p.slots);
     put(stage, head.items, p.items);
     e = b->staging.send(b->d_plan, ints * 4, ctx->stream);
@@ -395,17 +414,16 @@ cudaError_t launch_append(const AppendArgs &a, int rows, int wide_in, int wide_o
 
 }  // namespace
 
-cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, int slots_per_item, int solo_m,
-                                   int sm_count, cudaStream_t stream)
+cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int sm_count,
+                                   cudaStream_t stream)
 {
-    const CombineShape c = {record_rows, tile_m, slots_per_item, solo_m};
-    const int blocks = 8 * sm_count;
+    const CombineShape c = {record_rows, tile_m, by_column, (a.group + 7) / 8};
+    const dim3 grid((unsigned)(16 * sm_count));
     switch (a.type) {
-    case SATORI_F32: combine_kernel<SATORI_F32><<<blocks, 128, 0, stream>>>(a, c); break;
-    case SATORI_F16: combine_kernel<SATORI_F16><<<blocks, 128, 0, stream>>>(a, c); break;
-    default: combine_kernel<SATORI_BF16><<<blocks, 128, 0, stream>>>(a, c);
+    case SATORI_F32: return launch_overlapped(combine_kernel<SATORI_F32>, grid, 128, 0, stream, a, c);
+    case SATORI_F16: return launch_overlapped(combine_kernel<SATORI_F16>, grid, 128, 0, stream, a, c);
+    default: return launch_overlapped(combine_kernel<SATORI_BF16>, grid, 128, 0, stream, a, c);
     }
-    return cudaGetLastError();
 }
 
 extern "C" int satori_batch_create(satori_pages *pages, int q_heads, double rope_base, int rotary, satori_batch **out)
@@ -589,8 +607,7 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
                         ? launch_tensor_attention(a, p->map, layer * p->tables.pages() * 2 * p->kv_heads, p->ctx->stream)
                         : launch_generic_attention(a, p->ctx->stream);
     if (e == cudaSuccess)
-        e = launch_combine(a, (int)rows, b->shape.tile_m, b->shape.slots_per_item, b->shape.solo_m, p->ctx->sm_count,
-                           p->ctx->stream);
+        e = launch_combine(a, (int)rows, b->shape.tile_m, on_tensor_cores(b), p->ctx->sm_count, p->ctx->stream);
     return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "batch attention");
 }
 

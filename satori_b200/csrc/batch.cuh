@@ -15,11 +15,11 @@ namespace satori {
 // header's start).  Everything that changes from step to step is behind the one pointer, the work buffers
 // included, so captured launches read the current step's plan and write the buffers that it was sized for.
 struct DevPlan {
-    float *part_o;                   // partial records: [record][record_rows][head_dim], not normalised
+    float *part_o;                   // partial records of record_rows x head_dim, not normalised
     float2 *part_ml;                 // [record][record_rows]: running maximum (log2 units) and sum
     const double *rope;              // [row][rotary / 2] (cos, sin)
     PlanHeader head;
-    int row_position, row_page, row_slot, chain_off, chain, seg_rows, pages, cta_off, segments, tiles, slots, items;
+    int row_position, row_page, row_slot, chain_off, chain, seg_rows, pages, cta_off, slots, items;
 };
 
 template <typename T>
@@ -56,8 +56,27 @@ cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim
 cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
 
 // Merges the partial records of every row that has more than one source and writes its outputs.
-cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, int slots_per_item, int solo_m, int sm_count,
+// A record holds record_rows rows; by_column: as [head_dim / 4][row] groups of 4 values, otherwise [row][head_dim].
+cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int sm_count,
                            cudaStream_t stream);
+
+// A launch that may start while the kernel before it on the stream still runs; it waits for that kernel's
+// results itself (pdl_wait).
+template <typename K, typename... Args>
+cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args &...args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // --------------------------------------------------------------------------- element types
 template <int TYPE>

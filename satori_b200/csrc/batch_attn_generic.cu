@@ -65,26 +65,25 @@ struct Smem {
 
 // The item's rows: query values scaled by log2(e) / sqrt(d) are not rounded again (FP32), limits, indices.
 template <int TYPE, int HD>
-__device__ void load_rows(const BatchAttn &a, const DevPlan *plan, const PlanSegment &seg, const PlanTile &tile,
-                          int kv_head, Smem<TYPE, HD> &sm, int rows)
+__device__ void load_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
+                          Smem<TYPE, HD> &sm, int rows)
 {
     typedef typename Elem<TYPE>::type T;
-    const int *seg_rows = plan_array<int>(plan, plan->seg_rows) + seg.row_off;
-    const int *position = plan_array<int>(plan, plan->row_position);
+    const PlanRow *seg_rows = plan_array<PlanRow>(plan, plan->seg_rows) + item.row_off;
     for (int r = threadIdx.x; r < rows; r += kThreads) {
-        const int m = tile.m0 + r;
-        const bool live = r < tile.m;
-        const int row = live ? seg_rows[m / a.group] : 0;
-        sm.row[r] = row;
-        sm.head[r] = kv_head * a.group + m % a.group;
-        sm.limit[r] = !live ? 0 : seg.causal ? position[row] + 1 - seg.start : seg.keys;
+        const int m = item.m0 + r;
+        const bool live = r < item.m;
+        const PlanRow row = live ? seg_rows[m / a.group] : PlanRow{0, 0};
+        sm.row[r] = row.row;
+        sm.head[r] = item.kv_head * a.group + m % a.group;
+        sm.limit[r] = !live ? 0 : item.start >= 0 ? row.position + 1 - item.start : item.keys;
     }
     __syncthreads();
     const int chunks = a.head_dim / 8;
     for (int i = threadIdx.x; i < rows * (HD / 8); i += kThreads) {
         const int r = i / (HD / 8), c = i % (HD / 8);
         float f[8] = {};
-        if (r < tile.m && c < chunks) {
+        if (r < item.m && c < chunks) {
             const T *src = reinterpret_cast<const T *>(a.q) + (long long)sm.row[r] * a.ldq +
                            (long long)sm.head[r] * a.head_dim + c * 8;
 #pragma unroll
@@ -122,22 +121,22 @@ __device__ __forceinline__ void store_out(const BatchAttn &a, int row, int head,
 
 // ---- few rows: one warp, 8 keys at a time
 template <int TYPE, int HD>
-__device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item, const PlanTile &tile,
-                         const PlanSegment &seg, const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
+__device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
+                         const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
 {
     typedef typename Elem<TYPE>::type T;
     constexpr int EV = 16 / sizeof(T);                 // elements of a 16-byte chunk
     constexpr int CH = HD / EV / 4;                    // chunks of a K row per lane (4 lanes share a key)
     constexpr int VW = HD / 32;                        // V elements per lane
-    load_rows<TYPE, HD>(a, plan, seg, tile, item.kv_head, sm, kFewRows);
+    load_rows<TYPE, HD>(a, plan, item, sm, kFewRows);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = lane & 3;
-    const int key0 = item.block0 * kBlock, key1 = min(key0 + item.blocks * kBlock, tile.keys);
+    const int key0 = item.block0 * kBlock, key1 = min(key0 + item.blocks * kBlock, item.keys);
     const int chunks = a.head_dim / EV;
     int limit[kFewRows], least = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < kFewRows; ++r) {
         limit[r] = sm.limit[r];
-        if (r < tile.m) least = min(least, limit[r]);
+        if (r < item.m) least = min(least, limit[r]);
     }
     float m[kFewRows], l[kFewRows], acc[kFewRows][VW];
 #pragma unroll
@@ -249,7 +248,7 @@ __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem
     }
     __syncthreads();
     const int r = warp;                                // warp r merges row r
-    if (r < tile.m) {
+    if (r < item.m) {
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.few_m[w][r]);
@@ -276,13 +275,13 @@ __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem
 
 // ---- many rows: 64 x 64 tiles
 template <int TYPE, int HD>
-__device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item, const PlanTile &tile,
-                          const PlanSegment &seg, const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
+__device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
+                          const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
 {
     typedef typename Elem<TYPE>::type T;
     constexpr int EV = 16 / sizeof(T);
     constexpr int OC = HD / 64;                        // float4 groups of output columns per thread
-    load_rows<TYPE, HD>(a, plan, seg, tile, item.kv_head, sm, kTileM);
+    load_rows<TYPE, HD>(a, plan, item, sm, kTileM);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int chunks = a.head_dim / EV;
     float m[4], l[4], acc[4][OC * 4];
@@ -295,10 +294,9 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
 #pragma unroll
         for (int j = 0; j < OC * 4; ++j) acc[i][j] = 0;
     }
-    int least = seg.keys;                              // keys that every row of the tile sees
-    if (seg.causal) least = sm.limit[0];
+    const int least = sm.limit[0];                     // keys that every row of the tile sees
     for (int block = item.block0; block < item.block0 + item.blocks; ++block) {
-        const int t0 = block * kBlock, have = min(kBlock, tile.keys - t0);
+        const int t0 = block * kBlock, have = min(kBlock, item.keys - t0);
         for (int i = threadIdx.x; i < kBlock * (HD / EV); i += kThreads) {
             const int t = i / (HD / EV), c = i % (HD / EV);
             float fk[EV], fv[EV];
@@ -393,7 +391,7 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], o);
         const int r = ty * 4 + i;
-        if (r < tile.m) {
+        if (r < item.m) {
             const float inverse = 1.0f / l[i];
 #pragma unroll
             for (int c = 0; c < OC; ++c)
@@ -419,6 +417,8 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) generic_attention
     typedef typename Elem<TYPE>::type T;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Smem<TYPE, HD> &sm = *reinterpret_cast<Smem<TYPE, HD> *>(smem_raw);
+    pdl_launch_dependents();
+    pdl_wait();
     const DevPlan *plan = a.plan;
     const int *cta_off = plan_array<int>(plan, plan->cta_off);
     KeyRows<T> rows;
@@ -430,14 +430,12 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) generic_attention
     rows.page_elems = 2 * rows.kv_stride;
     for (int i = cta_off[blockIdx.x]; i < cta_off[blockIdx.x + 1]; ++i) {
         const PlanItem item = plan_array<PlanItem>(plan, plan->items)[i];
-        const PlanTile tile = plan_array<PlanTile>(plan, plan->tiles)[item.tile];
-        const PlanSegment seg = plan_array<PlanSegment>(plan, plan->segments)[tile.segment];
-        rows.pages = plan_array<int>(plan, plan->pages) + seg.page_off;
+        rows.pages = plan_array<int>(plan, plan->pages) + item.page_off;
         rows.head_off = (long long)item.kv_head * a.page_tokens * a.head_dim;
-        if (tile.m <= kFewRows)
-            few_rows<TYPE, HD>(a, plan, item, tile, seg, rows, sm);
+        if (item.m <= kFewRows)
+            few_rows<TYPE, HD>(a, plan, item, rows, sm);
         else
-            many_rows<TYPE, HD>(a, plan, item, tile, seg, rows, sm);
+            many_rows<TYPE, HD>(a, plan, item, rows, sm);
     }
 }
 
@@ -446,8 +444,7 @@ cudaError_t launch(const BatchAttn &a, cudaStream_t stream)
 {
     cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(&generic_attention_kernel<TYPE, HD>), sizeof(Smem<TYPE, HD>));
     if (e != cudaSuccess) return e;
-    generic_attention_kernel<TYPE, HD><<<a.ctas, kThreads, sizeof(Smem<TYPE, HD>), stream>>>(a);
-    return cudaGetLastError();
+    return launch_overlapped(generic_attention_kernel<TYPE, HD>, dim3(a.ctas), kThreads, sizeof(Smem<TYPE, HD>), stream, a);
 }
 
 template <int TYPE>

@@ -17,7 +17,10 @@ struct Builder {
     const std::vector<PlanMember> &members;
     Plan &plan;
     std::vector<int> order, row0;                      // members by table; first row of a member
-    std::vector<std::vector<PlanLink>> links;          // per member: (segment, index of its first row)
+    struct Place {
+        int segment, index;
+    };
+    std::vector<std::vector<Place>> places;            // per member: its segments, and its first row's place in each
 
     void segment(int lo, int hi, int page0, int page1, int keys, bool causal)
     {
@@ -31,8 +34,8 @@ struct Builder {
         plan.pages.insert(plan.pages.end(), first.pages + page0, first.pages + page1);
         for (int i = lo; i < hi; ++i) {
             const int b = order[i];
-            links[b].push_back({(int)plan.segments.size(), s.rows});
-            for (int r = 0; r < members[b].rows; ++r) plan.seg_rows.push_back(row0[b] + r);
+            places[b].push_back({(int)plan.segments.size(), s.rows});
+            for (int r = 0; r < members[b].rows; ++r) plan.seg_rows.push_back({row0[b] + r, plan.row_position[row0[b] + r]});
             s.rows += members[b].rows;
         }
         plan.segments.push_back(s);
@@ -84,7 +87,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
     plan.items.clear();
     plan.partials = 0;
 
-    Builder b{shape, members, plan, {}, std::vector<int>((size_t)n), std::vector<std::vector<PlanLink>>((size_t)n)};
+    Builder b{shape, members, plan, {}, std::vector<int>((size_t)n), std::vector<std::vector<Builder::Place>>((size_t)n)};
     for (int i = 0; i < n; ++i) {
         b.row0[i] = (int)plan.row_position.size();
         const PlanMember &m = members[i];
@@ -102,12 +105,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
     });
     b.walk(0, (int)b.order.size(), 0, 0);
     for (int i = 0; i < n; ++i)
-        for (int r = 0; r < members[i].rows; ++r) {
-            for (const PlanLink &l : b.links[i]) plan.chain.push_back({l.segment, l.index + r});
-            plan.chain_off.push_back((int)plan.chain.size());
-        }
-    for (int i = 0; i < n; ++i)
-        if (b.links[i].size() == 1) plan.segments[b.links[i][0].segment].sole = 1;
+        if (b.places[i].size() == 1) plan.segments[b.places[i][0].segment].sole = 1;
 
     long long total = 0;
     for (int s = 0; s < (int)plan.segments.size(); ++s) {
@@ -117,8 +115,8 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
         for (int m0 = 0; m0 < m_all; m0 += shape.tile_m) {
             PlanTile t = {s, m0, std::min(shape.tile_m, m_all - m0), seg.keys};
             if (seg.causal) {      // the tile's last row sees the most keys
-                const int row = plan.seg_rows[seg.row_off + (m0 + t.m - 1) / shape.group];
-                t.keys = plan.row_position[row] + 1 - seg.start;
+                const PlanRow &row = plan.seg_rows[seg.row_off + (m0 + t.m - 1) / shape.group];
+                t.keys = row.position + 1 - seg.start;
             }
             const int blocks = (t.keys + shape.block - 1) / shape.block;
             const int cost = t.m <= shape.solo_m ? shape.solo_cost : shape.pair_cost;
@@ -126,6 +124,12 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
             plan.tiles.push_back(t);
         }
     }
+    for (int i = 0; i < n; ++i)
+        for (int r = 0; r < members[i].rows; ++r) {
+            for (const Builder::Place &at : b.places[i])
+                plan.chain.push_back({plan.segments[at.segment].tile0, at.index + r});
+            plan.chain_off.push_back((int)plan.chain.size());
+        }
     plan.slots.resize(plan.tiles.size() * (size_t)shape.kv_heads);
 
     // Deal the blocks to the CTAs in order: segment, KV head, tile, so that tiles that read the same keys
@@ -143,7 +147,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                 const int blocks = (tile.keys + shape.block - 1) / shape.block;
                 PlanSlots &slots = plan.slots[(size_t)t * shape.kv_heads + h];
                 slots.first = plan.partials;
-                slots.items = 0;
+                int items = 0;
                 for (int at = 0; at < blocks;) {
                     if (room < shape.item_cost + cost && (int)plan.cta_off.size() < shape.ctas) {
                         plan.cta_off.push_back((int)plan.items.size());
@@ -153,21 +157,24 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                     long long take = (room - shape.item_cost) / cost;
                     if ((int)plan.cta_off.size() == shape.ctas) take = blocks - at;      // the last CTA takes the rest
                     take = std::max<long long>(1, std::min<long long>(take, blocks - at));
-                    plan.items.push_back({t, h, at, (int)take, 0, 0});
-                    ++slots.items;
+                    plan.items.push_back({seg.page_off, seg.row_off, tile.m0, tile.m, tile.keys, seg.causal ? seg.start : -1,
+                                          h, at, (int)take, 0, 0, 0});
+                    ++items;
                     at += (int)take;
                     room -= take * cost + shape.item_cost;
                 }
                 // One item holds every key its rows can see: it writes the rows' outputs.  (Tiles that an
                 // item works on in two halves of its blocks leave two records.)
                 const bool halves = shape.slots_per_item > 1 && tile.m <= shape.solo_m && blocks > 1;
-                const bool direct = seg.sole && slots.items == 1 && !halves;
-                for (int i = 0; i < slots.items; ++i) {
-                    PlanItem &item = plan.items[plan.items.size() - slots.items + i];
+                const bool direct = seg.sole && items == 1 && !halves;
+                for (size_t i = plan.items.size() - (size_t)items; i < plan.items.size(); ++i) {
+                    PlanItem &item = plan.items[i];
                     item.direct = direct;
                     item.slot = direct ? -1 : plan.partials;
                     if (!direct) plan.partials += shape.slots_per_item;
                 }
+                slots.records = plan.partials - slots.first;
+                slots.step = tile.m <= shape.solo_m ? 1 : shape.slots_per_item;
                 if (direct) slots.first = -1;
             }
     }

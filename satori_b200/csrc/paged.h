@@ -66,7 +66,7 @@ struct PlanShape {
     int tile_m, block;                                 // M rows per tile, keys per block
     int ctas;                                          // CTAs that the items are dealt to
     int solo_m;                                        // tiles of at most this many rows cost solo_cost per block
-    int solo_cost, pair_cost, item_cost;               // cost units per block (small / large tile) and per item
+    int solo_cost, pair_cost, item_cost;               // cost of a block (small / large tile) and of an item
     int slots_per_item;                                // partial records an item writes
 };
 
@@ -80,6 +80,9 @@ struct PlanMember {
 struct PlanHeader {
     int rows, segments, tiles, items;
 };
+struct PlanRow {
+    int row, position;                                 // a segment's row: its number in the step and its position
+};
 struct PlanSegment {
     int page_off, keys, start;                         // first entry of plan.pages, keys, position of key 0
     int row_off, rows;                                 // entries of plan.seg_rows
@@ -88,20 +91,23 @@ struct PlanSegment {
 struct PlanTile {
     int segment, m0, m, keys;                          // M range, keys some of its rows can see
 };
-struct PlanItem {
-    int tile, kv_head, block0, blocks;
-    int slot, direct;                                  // first partial record; direct: writes the output itself
+// An item carries what the kernels need of its tile and segment, so that one load leads to the data.
+struct alignas(16) PlanItem {
+    int page_off, row_off, m0, m;
+    int keys, start, kv_head, block0;                  // start: position of key 0, -1 when every row sees every key
+    int blocks, slot, direct, pad;                     // slot: first partial record; direct: writes the output itself
 };
-struct PlanSlots {
-    int first, items;                                  // partial records of (tile, KV head): first + slots_per_item * i
-};
+struct alignas(16) PlanSlots {
+    int first, records, step, pad;                     // partial records of (tile, KV head): every step-th holds a row;
+};                                                     // first -1: the item wrote the output
 struct PlanLink {
-    int segment, index;                                // a row's place in a segment
+    int tile0, index;                                  // a segment's first tile, a row's place in the segment
 };
 
 struct Plan {
     PlanHeader head;
-    std::vector<int> row_position, row_page, row_slot, chain_off, seg_rows, pages, cta_off;
+    std::vector<int> row_position, row_page, row_slot, chain_off, pages, cta_off;
+    std::vector<PlanRow> seg_rows;
     std::vector<PlanLink> chain;
     std::vector<PlanSegment> segments;
     std::vector<PlanTile> tiles;

@@ -27,6 +27,12 @@ def _bad(message: str) -> ArgumentError:
     return ArgumentError(_lib.ERR_ARGUMENT, message)
 
 
+def _open(ctx) -> bool:
+    """A handle whose context has been closed cannot be destroyed any more: its memory went with the process's
+    use of the context."""
+    return ctx is None or bool(ctx._h)
+
+
 def _type(dtype) -> int:
     """'f32' / 'f16' / 'bf16', a torch dtype, or a satori_type."""
     t = _TYPES.get(dtype, _TORCH_TYPES.get(str(dtype), dtype))
@@ -188,7 +194,8 @@ class PagedCache:
 
     def dispose(self) -> None:
         if self._h:
-            _lib.lib().satori_pages_destroy(self._h)
+            if _open(self.ctx):
+                _lib.lib().satori_pages_destroy(self._h)
             self._h = _vp()
 
     def __enter__(self):
@@ -267,7 +274,8 @@ class DecodeBatch:
 
     def dispose(self) -> None:
         if self._h:
-            _lib.lib().satori_batch_destroy(self._h)
+            if _open(self.cache.ctx):
+                _lib.lib().satori_batch_destroy(self._h)
             self._h = _vp()
 
     def __enter__(self):
@@ -307,7 +315,8 @@ class AdapterRows:
 
     def dispose(self) -> None:
         if self._h:
-            _lib.lib().satori_adapter_rows_destroy(self._h)
+            if _open(self.ctx):
+                _lib.lib().satori_adapter_rows_destroy(self._h)
             self._h = _vp()
 
     def __enter__(self):
@@ -395,7 +404,8 @@ class AdapterSet:
 
     def dispose(self) -> None:
         if self._h:
-            _lib.lib().satori_adapters_destroy(self._h)
+            if _open(self.ctx):
+                _lib.lib().satori_adapters_destroy(self._h)
             self._h = _vp()
 
     def __enter__(self):
