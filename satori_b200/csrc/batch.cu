@@ -184,114 +184,158 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, int wid
 }
 
 struct CombineShape {
-    int record_rows, tile_m, by_column, octets;
+    int record_rows, tile_m, by_column, octets, parts;
 };
 
-// out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - max m), over the records of all the row's segments
-// in their order, so the result does not depend on scheduling.  A block takes one row and up to 8 query
-// heads of a KV head: their values lie side by side in the records.  16 threads find a head's records and
-// weights; then all threads add the accumulators, 4 values each.
-template <int TYPE>
-__global__ void __launch_bounds__(128) combine_kernel(const BatchAttn a, const CombineShape c)
+// out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - m), over the records of all the row's segments in a
+// fixed order, so the result does not depend on scheduling; m is the running maximum, raised from one chunk of
+// records to the next.  A block takes one row, up to 8 query heads of a KV head (their values lie side by side
+// in the records) and 256 / SLICES groups of 4 values: a warp per head finds its records and their weights,
+// then each slice of the threads adds every SLICES-th record, and the slices are added.  Latency bounds it
+// (half a dozen loads one after the other before the first value), so loads go out 8 at a time.
+constexpr int kCombineThreads = 256, kCombineHeads = 8, kCombineChunk = 64, kCombineLinks = 32;
+
+template <int TYPE, int SLICES>
+__global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const BatchAttn a, const CombineShape c)
 {
-    constexpr int kHeads = 8, kChunk = 64;
-    __shared__ long long base[kHeads][kChunk];
-    __shared__ float weight[kHeads][kChunk], total[kHeads];
-    __shared__ int count[kHeads];
+    constexpr int kCombineQuads = kCombineThreads / SLICES, kBatch = 8;
+    __shared__ int first[kCombineLinks][kCombineHeads], records[kCombineLinks][kCombineHeads], step[kCombineLinks][kCombineHeads];
+    __shared__ unsigned base[kCombineHeads][kCombineChunk];        // record * rows + row
+    __shared__ float weight[kCombineHeads][kCombineChunk], factor[kCombineHeads], total[kCombineHeads];
+    __shared__ int count[kCombineHeads];
+    __shared__ float4 slices[SLICES][kCombineQuads];
     pdl_wait();      // and no early start for the next launch: its blocks would take the SMs from this one's
     const DevPlan *plan = a.plan;
-    const int tid = threadIdx.x, mine = tid >> 4, lane16 = tid & 15;
+    const int tid = threadIdx.x, mine = tid >> 5, lane = tid & 31;
     const int quads = a.head_dim / 4;
     const int *chain_off = plan_array<int>(plan, plan->chain_off);
     const PlanLink *chain = plan_array<PlanLink>(plan, plan->chain);
     const PlanSlots *slots = plan_array<PlanSlots>(plan, plan->slots);
-    const long long units = (long long)plan->head.rows * a.kv_heads * c.octets;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const int g0 = (int)(u % c.octets) * kHeads, heads = min(kHeads, a.group - g0);
-        const int kv_head = (int)(u / c.octets % a.kv_heads), row = (int)(u / c.octets / a.kv_heads);
+    const float4 *values = reinterpret_cast<const float4 *>(plan->part_o);
+    const float2 *part_ml = plan->part_ml;
+    const int *merges = plan_array<int>(plan, plan->merges);
+    const int units = plan->head.merges * c.octets * c.parts;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        int rest = u;
+        const int part = rest % c.parts;
+        rest /= c.parts;
+        const int g0 = rest % c.octets * kCombineHeads, heads = min(kCombineHeads, a.group - g0);
+        rest /= c.octets;
+        const int merge = merges[rest], kv_head = merge % a.kv_heads, row = merge / a.kv_heads;
         const int c0 = chain_off[row], c1 = chain_off[row + 1];
-        // Calls f(place, row in the record, record) for this thread's records of its head, in order; the number
-        // of the head's records, or -1 where its item wrote the output itself.
-        auto walk = [&](auto f) -> int {
-            int at = 0;
-            for (int k = c0; k < c1; ++k) {
-                const PlanLink link = chain[k];
-                const int m = link.index * a.group + g0 + mine, mt = m % c.tile_m;
+        // This thread's output: 4 values of one head.
+        const int slice = tid / kCombineQuads, i = part * kCombineQuads + tid % kCombineQuads;
+        const bool works = i < heads * quads;
+        const int g = works ? (c.by_column ? i % heads : i / quads) : 0, quad = c.by_column ? i / heads : i % quads;
+        float4 acc = make_float4(0, 0, 0, 0);
+        float ref = -INFINITY, sum = 0;                // this warp's head
+        for (int link0 = c0; link0 < c1; link0 += kCombineLinks) {
+            const int links = min(kCombineLinks, c1 - link0);
+            if (tid < links * kCombineHeads) {
+                const int k = tid / kCombineHeads, h = tid % kCombineHeads;
+                const PlanLink link = chain[link0 + k];
+                const int m = link.index * a.group + g0 + min(h, heads - 1), mt = m % c.tile_m;
                 const PlanSlots s = slots[(link.tile0 + m / c.tile_m) * a.kv_heads + kv_head];
-                if (s.first < 0) return -1;
-                const int first = s.first + mt / c.record_rows;    // a large tile's second record follows its first
-                const int n = s.records / s.step;
-                for (int i = lane16; i < n; i += 16) f(at + i, mt % c.record_rows, first + i * s.step);
-                at += n;
+                // A tile's rows run on into its second record; first -1: the item wrote the output itself.
+                first[k][h] = s.first < 0 ? -1 : s.first * c.record_rows + mt;
+                records[k][h] = s.records / s.step;
+                step[k][h] = s.step * c.record_rows;
             }
-            return at;
-        };
-        const bool active = mine < heads;
-        float top = -INFINITY;
-        int n = -1;
-        if (active)
-            n = walk([&](int, int r, int record) { top = fmaxf(top, plan->part_ml[(long long)record * c.record_rows + r].x); });
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum = 0;
-        float4 acc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = make_float4(0, 0, 0, 0);
-        if (lane16 == 0) count[mine] = n;
-        __syncthreads();
-        int most = 0;
-        for (int g = 0; g < heads; ++g) most = max(most, count[g]);
-        for (int chunk = 0; chunk < most; chunk += kChunk) {
-            if (n > chunk)
-                walk([&](int at, int r, int record) {
-                    if (at < chunk || at >= chunk + kChunk) return;
-                    const float2 ml = plan->part_ml[(long long)record * c.record_rows + r];
-                    const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - ref);  // no key: nothing was stored
-                    sum += w == 0 ? 0.0f : w * ml.y;
-                    weight[mine][at - chunk] = w;
-                    base[mine][at - chunk] = (long long)record * c.record_rows * quads + (c.by_column ? r : r * quads);
-                });
             __syncthreads();
+            const bool written = first[0][mine] < 0;
+            int n = 0;
+            for (int k = 0; k < links; ++k) n += records[k][mine];
+            if (written || mine >= heads) n = 0;
+            if (lane == 0) count[mine] = written ? -1 : n;
+            __syncthreads();
+            int most = 0;
+            for (int h = 0; h < heads; ++h) most = max(most, count[h]);
+            for (int chunk = 0; chunk < most; chunk += kCombineChunk) {
+                unsigned at[kCombineChunk / 32];
+                float2 ml[kCombineChunk / 32];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = tid + j * 128;
-                if (i >= heads * quads) continue;
-                const int g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
-                const long long off = c.by_column ? (long long)quad * c.record_rows : quad;
-                const int end = min(kChunk, count[g] - chunk);
-#pragma unroll 4
-                for (int f = 0; f < end; ++f) {
-                    const float w = weight[g][f];
-                    const float4 v = *(reinterpret_cast<const float4 *>(plan->part_o) + base[g][f] + off);
-                    if (w == 0) continue;
-                    acc[j].x = fmaf(v.x, w, acc[j].x);
-                    acc[j].y = fmaf(v.y, w, acc[j].y);
-                    acc[j].z = fmaf(v.z, w, acc[j].z);
-                    acc[j].w = fmaf(v.w, w, acc[j].w);
+                for (int j = 0; j < kCombineChunk / 32; ++j) {
+                    int rank = chunk + j * 32 + lane, k = 0;
+                    ml[j] = make_float2(-INFINITY, 0.0f);
+                    at[j] = 0;
+                    if (rank < n) {
+                        while (rank >= records[k][mine]) rank -= records[k++][mine];
+                        at[j] = (unsigned)first[k][mine] + (unsigned)rank * (unsigned)step[k][mine];
+                        ml[j] = part_ml[at[j]];
+                    }
                 }
+                float top = ml[0].x;
+#pragma unroll
+                for (int j = 1; j < kCombineChunk / 32; ++j) top = fmaxf(top, ml[j].x);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                top = fmaxf(top, ref);
+                const float keep = top == -INFINITY ? 1.0f : exp2f(ref - top);
+                sum *= keep;
+                ref = top;
+#pragma unroll
+                for (int j = 0; j < kCombineChunk / 32; ++j) {
+                    const float w = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - ref);   // no key: nothing was stored
+                    if (w != 0) sum = fmaf(w, ml[j].y, sum);
+                    weight[mine][j * 32 + lane] = w;
+                    base[mine][j * 32 + lane] = at[j];
+                }
+                if (lane == 0) factor[mine] = keep;
+                __syncthreads();
+                const int end = works ? min(kCombineChunk, count[g] - chunk) : 0;
+                const float scale = factor[g];
+                acc.x *= scale;
+                acc.y *= scale;
+                acc.z *= scale;
+                acc.w *= scale;
+                for (int f0 = slice; f0 < end; f0 += SLICES * kBatch) {
+                    float4 v[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int f = f0 + k * SLICES;
+                        v[k] = make_float4(0, 0, 0, 0);
+                        if (f < end && weight[g][f] != 0) {
+                            const unsigned rr = base[g][f], r = rr % (unsigned)c.record_rows;
+                            v[k] = values[c.by_column ? (size_t)(rr - r) * quads + (size_t)quad * c.record_rows + r
+                                                      : (size_t)rr * quads + quad];
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int f = f0 + k * SLICES;
+                        const float w = f < end ? weight[g][f] : 0.0f;
+                        acc.x = fmaf(v[k].x, w, acc.x);
+                        acc.y = fmaf(v[k].y, w, acc.y);
+                        acc.z = fmaf(v[k].z, w, acc.z);
+                        acc.w = fmaf(v[k].w, w, acc.w);
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (lane16 == 0) total[mine] = sum;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane == 0) total[mine] = sum;
+        if (slice > 0) slices[slice - 1][tid % kCombineQuads] = acc;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = tid + j * 128;
-            if (i >= heads * quads) continue;
-            const int g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
-            if (count[g] < 0) continue;
+        if (slice == 0 && works && count[g] >= 0) {
             const float inverse = 1.0f / total[g];
-            const float v[4] = {acc[j].x * inverse, acc[j].y * inverse, acc[j].z * inverse, acc[j].w * inverse};
+            float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+            for (int k = 0; k < SLICES - 1; ++k) {
+                const float4 more = slices[k][tid];
+                v[0] += more.x;
+                v[1] += more.y;
+                v[2] += more.z;
+                v[3] += more.w;
+            }
             const long long to = (long long)row * a.ldo + (long long)(kv_head * a.group + g0 + g) * a.head_dim + quad * 4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (a.out_f32)
-                    reinterpret_cast<float *>(a.out)[to + e] = v[e];
+                    reinterpret_cast<float *>(a.out)[to + e] = v[e] * inverse;
                 else
-                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + e] = Elem<TYPE>::from_float(v[e]);
+                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + e] = Elem<TYPE>::from_float(v[e] * inverse);
             }
         }
         __syncthreads();
@@ -366,8 +410,12 @@ int upload_plan(satori_batch *b)
     head.cta_off = place(p.cta_off, ints);
     head.slots = place(p.slots, ints);
     head.items = place(p.items, ints);
-    if (ints > 0x7fffffff) return set_error(SATORI_ERR_NOT_SUPPORTED, "the step's plan exceeds Int32 limits");
-    const size_t rows = record_rows(b), record = rows * ((size_t)b->pages->head_dim + 2) * 4;
+    head.merges = place(p.merges, ints);
+    const size_t rows = record_rows(b);
+    if (ints > 0x7fffffff || (size_t)p.partials * rows > 0x7fffffff ||
+        (double)p.merges.size() * b->q_heads * b->pages->head_dim > 2e9)
+        return set_error(SATORI_ERR_NOT_SUPPORTED, "the step's plan exceeds Int32 limits");
+    const size_t record = rows * ((size_t)b->pages->head_dim + 2) * 4;
     const int *old_plan = b->d_plan;
     cudaError_t e = grow(b, b->d_plan, b->plan_ints, ints, 4, 1 << 16);
     b->reallocations += old_plan && old_plan != b->d_plan;
@@ -392,6 +440,7 @@ int upload_plan(satori_batch *b)
     put(stage, head.cta_off, p.cta_off);
     put(stage, head.slots, p.slots);
     put(stage, head.items, p.items);
+    put(stage, head.merges, p.merges);
     e = b->staging.send(b->d_plan, ints * 4, ctx->stream);
     if (e == cudaSuccess && b->rotary && p.head.rows) {
         const long long pairs = (long long)p.head.rows * (b->rotary / 2);
@@ -414,15 +463,28 @@ cudaError_t launch_append(const AppendArgs &a, int rows, int wide_in, int wide_o
 
 }  // namespace
 
-cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int sm_count,
+template <int TYPE>
+static cudaError_t launch_combine_type(const BatchAttn &a, const CombineShape &c, int slices, dim3 grid, cudaStream_t stream)
+{
+    auto kernel = slices == 4 ? combine_kernel<TYPE, 4> : slices == 2 ? combine_kernel<TYPE, 2> : combine_kernel<TYPE, 1>;
+    return launch_overlapped(kernel, grid, kCombineThreads, 0, stream, a, c);
+}
+
+cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int merges, int sm_count,
                                    cudaStream_t stream)
 {
-    const CombineShape c = {record_rows, tile_m, by_column, (a.group + 7) / 8};
-    const dim3 grid((unsigned)(16 * sm_count));
+    // As many slices as a row's values leave threads for, and four when there are too few rows to fill the SMs
+    // (one sequence of 4k tokens over 4 KV heads, 66 records a row: 13 us with one slice, 9 with four).
+    const int outputs = std::min(a.group, kCombineHeads) * a.head_dim / 4, octets = (a.group + kCombineHeads - 1) / kCombineHeads;
+    const int slices = outputs <= 64 || merges * octets < sm_count ? 4 : outputs <= 128 ? 2 : 1;
+    const int quads = kCombineThreads / slices;
+    const CombineShape c = {record_rows, tile_m, by_column, octets, (outputs + quads - 1) / quads};
+    const long long units = (long long)merges * octets * c.parts;
+    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>(units, 8ll * sm_count)));
     switch (a.type) {
-    case SATORI_F32: return launch_overlapped(combine_kernel<SATORI_F32>, grid, 128, 0, stream, a, c);
-    case SATORI_F16: return launch_overlapped(combine_kernel<SATORI_F16>, grid, 128, 0, stream, a, c);
-    default: return launch_overlapped(combine_kernel<SATORI_BF16>, grid, 128, 0, stream, a, c);
+    case SATORI_F32: return launch_combine_type<SATORI_F32>(a, c, slices, grid, stream);
+    case SATORI_F16: return launch_combine_type<SATORI_F16>(a, c, slices, grid, stream);
+    default: return launch_combine_type<SATORI_BF16>(a, c, slices, grid, stream);
     }
 }
 
@@ -607,7 +669,8 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
                         ? launch_tensor_attention(a, p->map, layer * p->tables.pages() * 2 * p->kv_heads, p->ctx->stream)
                         : launch_generic_attention(a, p->ctx->stream);
     if (e == cudaSuccess)
-        e = launch_combine(a, (int)rows, b->shape.tile_m, on_tensor_cores(b), p->ctx->sm_count, p->ctx->stream);
+        e = launch_combine(a, (int)rows, b->shape.tile_m, on_tensor_cores(b), b->plan.head.merges,
+                           p->ctx->sm_count, p->ctx->stream);
     return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "batch attention");
 }
 

@@ -19,7 +19,7 @@ struct DevPlan {
     float2 *part_ml;                 // [record][record_rows]: running maximum (log2 units) and sum
     const double *rope;              // [row][rotary / 2] (cos, sin)
     PlanHeader head;
-    int row_position, row_page, row_slot, chain_off, chain, seg_rows, pages, cta_off, slots, items;
+    int row_position, row_page, row_slot, chain_off, chain, seg_rows, pages, cta_off, slots, items, merges;
 };
 
 template <typename T>
@@ -51,13 +51,14 @@ cudaError_t launch_generic_attention(const BatchAttn &a, cudaStream_t stream);
 bool tensor_attention_takes(int type, int head_dim);
 void tensor_plan_shape(int sm_count, PlanShape &shape);
 int tensor_record_rows();
-// The cache as a 3-D tensor [block][token][dim] of (layer, page, K or V, head) blocks.
+// The cache as a tensor of (layer, page, K or V, head) blocks.
 cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim, int page_tokens, unsigned long long blocks);
 cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
 
 // Merges the partial records of every row that has more than one source and writes its outputs.
 // A record holds record_rows rows; by_column: as [head_dim / 4][row] groups of 4 values, otherwise [row][head_dim].
-cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int sm_count,
+// `merges` (the plan's) chooses the launch's shape; any number is worked through.
+cudaError_t launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int merges, int sm_count,
                            cudaStream_t stream);
 
 // A launch that may start while the kernel before it on the stream still runs; it waits for that kernel's

@@ -3,15 +3,16 @@
 //
 // The same one pass over the keys as the FP32-unit kernel, as two matrix products per block of 64 keys:
 // S = Q K^T and O += P V with P = 2^(s - m).  One CTA per SM works through its share of the plan's items:
-//  * warp 8 loads the pages of a block's K and V with TMA (one box per page and 64 columns, 128-byte swizzle)
-//    into a ring of stages;
-//  * one lane of warp 9 issues the MMAs: S from shared memory (Q and K, both K-major), O with P from tensor
-//    memory and V from shared memory as it lies (MN-major);
-//  * warp 10 clears the rows of V behind a tile's last key;
-//  * warps 0-3 and 4-7 are two softmax groups, each with its own O and two S / P buffers in tensor memory; a
-//    thread owns one row.  A large tile (129..256 rows) gives each group 128 of its rows and every K and V
-//    block serves both; a small one gives each group every other block.  The scores of a group's next block
-//    are computed while it takes the exponentials of this one.
+//  * a thread of warp 16 loads the pages of a block's K and V with TMA (128-byte swizzle) into a ring of stages;
+//  * one lane each of warps 17 and 18 issues the MMAs of a softmax group: S from shared memory (Q and K, both
+//    K-major), O with P from tensor memory and V from shared memory as it lies (MN-major);
+//  * warp 19 clears the rows of V behind a tile's last key;
+//  * warps 0-7 and 8-15 are two softmax groups, each with its own O and two S / P buffers in tensor memory; two
+//    threads share a row, each with half of a block's keys and half of the output's columns.  A large tile
+//    (129..256 rows) gives each group 128 of its rows and every K and V block serves both; a small one gives
+//    each group every other block.  The scores of a group's next block are computed while it takes the
+//    exponentials of this one.  Eight warps a group, not four: the exponentials are a chain of short steps, and
+//    with two warps per scheduler it was idle two thirds of the time.
 // The maximum that the exponentials refer to is raised only when it is exceeded by more than 2^8, so the
 // accumulator in tensor memory is rescaled a few times per row, not at every block; P stays below 2^8 and the
 // result does not depend on it.  P is rounded to the cache's type (half a step, as the operands already are);
@@ -29,7 +30,11 @@ namespace satori {
 namespace {
 
 constexpr int kTileRows = 128, kBlockKeys = 64;
-constexpr int kSoftmaxThreads = 256, kThreads = kSoftmaxThreads + 96;
+constexpr int kGroupThreads = 2 * kTileRows, kThreads = 2 * kGroupThreads + 128;
+#ifndef SATORI_EVERY
+#define SATORI_EVERY 4
+#endif
+constexpr int kEvery = SATORI_EVERY;
 constexpr float kLazy = 8.0f;                  // log2 of what a weight may exceed 1 by
 
 template <int HD>
@@ -37,20 +42,22 @@ struct Layout {
     static constexpr int kQHalf = kTileRows * 128, kHalf = kBlockKeys * 128;       // rows of 64 columns
     static constexpr int kQTile = kQHalf * (HD / 64), kTile = kHalf * (HD / 64);   // Q; K or V
     static constexpr int kStages = HD == 128 ? 10 : 20;
-    static constexpr int kHeader = 1024;
-    static constexpr int kBytes = kHeader + 2 * kQTile + kStages * kTile + 1024;
+    static constexpr int kHeader = 3072;
+    static constexpr int kBytes = kHeader + 2 * kQTile + kStages * kTile;
     static constexpr int kOCol = 4 * kBlockKeys;                   // tensor memory: S / P buffers, then O
 };
 
 constexpr int kMaxStages = 20;
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];           // [group][buffer]: blocks in turn
-    uint64_t q_ready[2], tail_full, tail_clear, drained;
+    uint64_t s_full[2][2], p_ready[2][2];      // [group][buffer]: blocks in turn
+    uint64_t q_ready[2], o_before[2], o_full[2];                   // o_before: all products but the item's last
+    uint64_t tail_full[2], tail_clear[2], drained[2];
     uint32_t tmem;
     volatile int abort;
+    float exchange[2][2][kTileRows];           // [group][half][row]: maximum, then sum
 };
-static_assert(sizeof(Barriers) <= 1024, "header");
+static_assert(sizeof(Barriers) <= 3072, "header");
 
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -92,10 +99,18 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
                  ::"r"(d), "r"(a), "l"(desc(b)), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void *dst, const void *map, int c0, int c1, int c2, uint64_t *bar)
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, int c0, int c1, int c2, uint64_t *bar)
 {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// All 64-column halves of a block of 64 tokens at token c1 of block c3 (the map of pages of 64 tokens and more).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, int token, int block, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(token), "r"(0), "r"(block), "r"(smem_u32(bar))
                  : "memory");
 }
 
@@ -113,12 +128,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *v)
                  : SATORI_R8(v, 0), SATORI_R8(v, 8), SATORI_R8(v, 16), SATORI_R8(v, 24)
                  : "r"(addr));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t *v)
+// 16 columns, waited for.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t *v)
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-                 ::SATORI_W8(v, 0), SATORI_W8(v, 8), SATORI_W8(v, 16), SATORI_W8(v, 24), "r"(addr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : SATORI_R8(v, 0), SATORI_R8(v, 8) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::SATORI_W8(v, 0), SATORI_W8(v, 8), "r"(addr) : "memory");
 }
 // The loaded registers pass through the wait, so that nothing reads them before it.
 #define SATORI_U8(v, i) "+r"((v)[i]), "+r"((v)[i + 1]), "+r"((v)[i + 2]), "+r"((v)[i + 3]), "+r"((v)[i + 4]), \
@@ -137,6 +159,42 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// 2^x on the FP32 units, two at a time, for part of the weights: the special function unit takes 8 clocks for a
+// warp's exponentials and is the scarcer one.  x = n + f with n the nearest integer (left in the low bits of
+// x + 1.5 2^23) and 2^f by a polynomial: the minimax fits on |f| <= 1/2 of degree 3 (relative error 7.5e-5,
+// 1/26 of bf16's half step) and 4 (2.6e-6, for fp16); n goes into the exponent.  x >= -126 is the caller's.
+template <int TYPE>
+__device__ __forceinline__ float2 exp2_poly(float2 x)
+{
+    const float2 magic = make_float2(12582912.0f, 12582912.0f), minus = make_float2(-1.0f, -1.0f);
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const float2 t = __fadd2_rn(x, magic);
+    const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
+    const float2 f = __ffma2_rn(n, minus, x);
+    float2 p;
+    auto pair = [](float v) { return make_float2(v, v); };
+    if (TYPE == SATORI_BF16) {
+        p = __ffma2_rn(pair(0.05517165765016593f), f, pair(0.24261112131938758f));
+        p = __ffma2_rn(p, f, pair(0.6932609875663172f));
+        p = __ffma2_rn(p, f, pair(0.9999280736469822f));
+    } else {
+        p = __ffma2_rn(pair(0.009570100592456837f), f, pair(0.05591786021593906f));
+        p = __ffma2_rn(p, f, pair(0.24024744860429012f));
+        p = __ffma2_rn(p, f, pair(0.6931218147559814f));
+        p = __ffma2_rn(p, f, pair(0.9999992614359087f));
+    }
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float x, float y)
 {
@@ -148,15 +206,36 @@ __device__ __forceinline__ uint32_t pack2(float x, float y)
     return *reinterpret_cast<const uint32_t *>(&b);
 }
 
-// Scores of keys `see` and above of 32 are not the row's to see.
-__device__ __forceinline__ void mask_scores(uint32_t *s, int see)
+// Named barriers of the two warps that share 32 rows.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool mine)
 {
-    if (see < 32) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)mine), "r"(id) : "memory");
+    return any != 0;
+}
+
+// Weights of 32 scores, packed in pairs, and their sum.  Every EVERY-th pair takes the polynomial
+// (0: none).
+template <int TYPE, int EVERY>
+__device__ __forceinline__ float block_weights(const uint32_t (&s)[32], float scale, float base, uint32_t (&p)[16])
+{
+    const float2 scale2 = make_float2(scale, scale), minus_base = make_float2(-base, -base);
+    float2 add[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (e >= see) s[e] = 0xFF800000u;
+    for (int e = 0; e < 32; e += 2) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, minus_base);
+        float2 w;
+        if (EVERY > 0 && (e / 2) % (EVERY > 0 ? EVERY : 1) == 0)
+            w = exp2_poly<TYPE>(x);
+        else
+            w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+        add[e / 2 & 1] = __fadd2_rn(add[e / 2 & 1], w);
+        p[e / 2] = pack2<TYPE>(w.x, w.y);
     }
-    __syncwarp();
+    const float2 sum = __fadd2_rn(add[0], add[1]);
+    return sum.x + sum.y;
 }
 
 struct TensorArgs {
@@ -173,6 +252,8 @@ struct Work {
     // order of use: the leading blocks' K, then V and the next K in turn.
     __device__ __forceinline__ int blocks(int g) const { return pair ? item.blocks : (item.blocks + 1 - g) / 2; }
     __device__ __forceinline__ int lead() const { return min(item.blocks, pair ? 2 : 4); }
+    // The group whose MMA warp asks for the clearing of the last V: its only user, or the first of two.
+    __device__ __forceinline__ int tail_group() const { return pair ? 0 : (item.blocks - 1) & 1; }
     // Keys of the item's last block, when the tile ends inside it; 0: no row of V needs clearing.
     __device__ __forceinline__ int tail() const
     {
@@ -210,6 +291,14 @@ __device__ __forceinline__ Work load_work(const DevPlan *plan, int i)
     for (int k = 0; k < (int)(sizeof(PlanItem) / 16); ++k) dst[k] = __ldg(src + k);
     w.pair = w.item.m > kTileRows;
     return w;
+}
+
+// 16 bytes from any address of 2-byte elements.
+__device__ __noinline__ uint4 load_unaligned(const void *src)
+{
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
+    return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                      h[6] | (uint32_t)h[7] << 16);
 }
 
 // 32 columns of a row's accumulator: its share of the partial record, or of the output.
@@ -260,6 +349,86 @@ __device__ __forceinline__ void store_output(const TensorArgs &t, const DevPlan 
     }
 }
 
+// An item's loads, in the order of use, by one thread.  What it does for a load is on the way of everything else
+// (with the page numbers fetched in line by a lane per box it took 1170 clocks a load, and the kernel waited
+// for nothing else), so the page numbers are fetched a step ahead and a whole block of 64-token pages is one copy.
+template <int HD>
+struct Loads {
+    const TensorArgs &t;
+    const CUtensorMap &map;
+    Barriers *bar;
+    uint32_t stages;
+    const int *pages;
+    int keys, first_block;
+
+    // PER: pages of a block.
+    template <int PER, typename Wait>
+    __device__ __forceinline__ bool run(const Work &w, Ring<Layout<HD>::kStages> &ring, int &units, Wait &wait) const
+    {
+        typedef Layout<HD> L;
+        constexpr int kBox = kBlockKeys / PER;
+        const int shift = __ffs(t.a.page_tokens) - 1, mask = t.a.page_tokens - 1, n = w.item.blocks, lead = w.lead();
+        const int key0 = w.item.block0 * kBlockKeys, page_blocks = 2 * t.a.kv_heads;
+        const int last_boxes = (min(kBlockKeys, keys - key0 - (n - 1) * kBlockKeys) + kBox - 1) / kBox;
+        auto fetch = [&](int j, int (&id)[PER]) {
+#pragma unroll
+            for (int b = 0; b < PER; ++b) {
+                const int key = key0 + j * kBlockKeys + b * kBox;
+                if (key < keys) id[b] = __ldg(pages + (key >> shift));
+            }
+        };
+        auto issue = [&](int j, int kv, const int (&id)[PER]) -> bool {
+            uint64_t *full = &bar->full[ring.stage];
+            if (!wait(&bar->empty[ring.stage], ring.parity ^ 1u)) return false;
+            const uint32_t to = stages + ring.stage * L::kTile;
+            const int boxes = j == n - 1 ? last_boxes : PER, block0 = first_block + kv * t.a.kv_heads;
+            mbar_expect_tx(full, (uint32_t)(boxes * kBox * HD * 2));
+            if (PER == 1) {
+                tma_load_4d(to, &map, (key0 + j * kBlockKeys) & mask, block0 + id[0] * page_blocks, full);
+            } else {
+#pragma unroll
+                for (int b = 0; b < PER; ++b)
+                    if (b < boxes)
+#pragma unroll
+                        for (int half = 0; half < HD / 64; ++half)
+                            tma_load_3d(to + half * L::kHalf + b * kBox * 128, &map, half * 64, 0, block0 + id[b] * page_blocks, full);
+            }
+            ring.next();
+            ++units;
+            return true;
+        };
+        int k_id[PER], v_id[PER];
+#pragma unroll
+        for (int b = 0; b < PER; ++b) k_id[b] = v_id[b] = 0;
+        fetch(0, k_id);
+        fetch(0, v_id);
+        for (int j = 0; j < lead; ++j) {
+            int next[PER];
+#pragma unroll
+            for (int b = 0; b < PER; ++b) next[b] = 0;
+            if (j + 1 < n) fetch(j + 1, next);
+            if (!issue(j, 0, k_id)) return false;
+#pragma unroll
+            for (int b = 0; b < PER; ++b) k_id[b] = next[b];
+        }
+        for (int j = 0; j < n; ++j) {
+            int next_v[PER], next_k[PER];
+#pragma unroll
+            for (int b = 0; b < PER; ++b) next_v[b] = next_k[b] = 0;
+            if (j + 1 < n) fetch(j + 1, next_v);
+            if (j + lead + 1 < n) fetch(j + lead + 1, next_k);
+            if (!issue(j, 1, v_id)) return false;
+            if (j + lead < n && !issue(j + lead, 0, k_id)) return false;
+#pragma unroll
+            for (int b = 0; b < PER; ++b) {
+                v_id[b] = next_v[b];
+                k_id[b] = next_k[b];
+            }
+        }
+        return true;
+    }
+};
+
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const TensorArgs t, const __grid_constant__ CUtensorMap map)
 {
@@ -267,37 +436,41 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
     typedef typename Elem<TYPE>::type T;
     constexpr int NS = L::kStages;
     const BatchAttn &a = t.a;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t smem[];
     Barriers *bar = reinterpret_cast<Barriers *>(smem);
     uint8_t *q_tiles = smem + L::kHeader, *stages = q_tiles + 2 * L::kQTile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if (smem_u32(smem) & 1023u) {              // the swizzle needs it; dynamic shared memory starts there
+        if (tid == 0) atomicOr(a.err, kDevErrTimeout);
+        return;
+    }
     pdl_launch_dependents();
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&bar->full[s], 1);
-            mbar_init(&bar->empty[s], 1);
+            mbar_init(&bar->empty[s], 2);
         }
         for (int g = 0; g < 2; ++g) {
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&bar->s_full[g][b], 1);
-                mbar_init(&bar->p_ready[g][b], kTileRows);
-                mbar_init(&bar->pv_done[g][b], 1);
+                mbar_init(&bar->p_ready[g][b], kGroupThreads);
             }
-            mbar_init(&bar->q_ready[g], kTileRows);
+            mbar_init(&bar->q_ready[g], kGroupThreads);
+            mbar_init(&bar->o_before[g], 1);
+            mbar_init(&bar->o_full[g], 1);
+            mbar_init(&bar->tail_full[g], 1);
+            mbar_init(&bar->tail_clear[g], 32);
+            mbar_init(&bar->drained[g], 1);
         }
-        mbar_init(&bar->tail_full, 1);
-        mbar_init(&bar->tail_clear, 32);
-        mbar_init(&bar->drained, 1);
         bar->abort = 0;
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar->tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp == 8 && lane == 0) prefetch_tensormap(&map);
+    if (warp == 16 && lane == 0) prefetch_tensormap(&map);
     fence_before();
     __syncthreads();
     fence_after();
@@ -317,184 +490,165 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
         return false;
     };
 
-    if (warp == 8) {
-        // ---- loads
-        const int box = min(a.page_tokens, kBlockKeys), shift = __ffs(a.page_tokens) - 1;
-        // Lane l loads 64-column half l % (HD / 64) of box l / (HD / 64) of a block.
-        const int b = lane / (HD / 64), half = lane % (HD / 64);
-        Ring<NS> ring;
-        int units = 0;
-        bool ok = true;
-        for (int i = first; i < last && ok; ++i) {
-            const Work w = load_work(plan, i);
-            const int *pages = plan_array<int>(plan, plan->pages) + w.item.page_off;
-            auto load = [&](int j, int kv) {
-                const int t0 = (w.item.block0 + j) * kBlockKeys, have = min(kBlockKeys, w.item.keys - t0);
-                const int boxes = (have + box - 1) / box, key = t0 + b * box, s = ring.stage;
-                const bool mine = b < boxes;
-                const int page = mine ? __ldg(pages + (key >> shift)) : 0;
-                ok = __all_sync(0xFFFFFFFFu, wait(&bar->empty[s], ring.parity ^ 1u));
-                if (!ok) return;
-                if (lane == 0) mbar_expect_tx(&bar->full[s], (uint32_t)(boxes * box * HD * 2));
-                __syncwarp();
-                if (mine)
-                    tma_load_3d(stages + (size_t)s * L::kTile + half * L::kHalf + b * box * 128, &map, half * 64,
-                                key & (a.page_tokens - 1), t.layer_block + (page * 2 + kv) * a.kv_heads + w.item.kv_head,
-                                &bar->full[s]);
-                ring.next();
-                ++units;
-            };
-            const int lead = w.lead();
-            for (int j = 0; j < lead && ok; ++j) load(j, 0);
-            for (int j = 0; j < w.item.blocks && ok; ++j) {
-                load(j, 1);
-                if (ok && j + lead < w.item.blocks) load(j + lead, 0);
+    if (warp == 16) {
+        // ---- loads, by one thread
+        if (elect_one()) {
+            Ring<NS> ring;
+            int units = 0;
+            bool ok = true;
+            for (int i = first; i < last && ok; ++i) {
+                const Work w = load_work(plan, i);
+                const int *pages = plan_array<int>(plan, plan->pages) + w.item.page_off;
+                const Loads<HD> loads = {t, map, bar, smem_u32(stages), pages, w.item.keys, t.layer_block + w.item.kv_head};
+                ok = a.page_tokens >= kBlockKeys ? loads.template run<1>(w, ring, units, wait)
+                     : a.page_tokens == 32       ? loads.template run<2>(w, ring, units, wait)
+                                                 : loads.template run<4>(w, ring, units, wait);
             }
+            if (!ok)      // the copies in flight land before the CTA may end
+                for (int u = max(0, units - NS); u < units; ++u) mbar_wait_bounded(&bar->full[u % NS], (uint32_t)((u / NS) & 1));
         }
-        if (!ok)      // the copies in flight land before the CTA may end
-            for (int u = max(0, units - NS); u < units; ++u) mbar_wait_bounded(&bar->full[u % NS], (uint32_t)((u / NS) & 1));
-    } else if (warp == 10) {
+        __syncwarp();
+    } else if (warp == 19) {
         // ---- V behind the last key: whatever the stage or the page holds there meets weights of zero, so it
         // must be finite.
         Ring<NS> ring;
-        uint32_t phase = 0;
+        uint32_t phase = 0;                            // bit g: tail_full[g]
         bool ok = true;
         for (int i = first; i < last && ok; ++i) {
             const Work w = load_work(plan, i);
-            const int have = w.tail();
+            const int have = w.tail(), g = w.tail_group();
             ring.advance(2 * w.item.blocks - 1);       // the item's last load
             if (have > 0) {
-                // Warp 9 has seen the load arrive, and waits: the stage keeps its contents meanwhile.
-                ok = __all_sync(0xFFFFFFFFu, wait(&bar->tail_full, phase));
+                // The MMA warp has seen the load arrive, and waits: the stage keeps its contents meanwhile.
+                ok = __all_sync(0xFFFFFFFFu, wait(&bar->tail_full[g], phase >> g & 1u));
                 if (!ok) break;
-                phase ^= 1u;
+                phase ^= 1u << g;
                 uint8_t *v = stages + (size_t)ring.stage * L::kTile + have * 128;
                 for (int c = lane; c < (kBlockKeys - have) * 8; c += 32)
 #pragma unroll
                     for (int h = 0; h < HD / 64; ++h)
                         *reinterpret_cast<uint4 *>(v + h * L::kHalf + c * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&bar->tail_clear);
+                mbar_arrive(&bar->tail_clear[g]);
+                if (w.pair) mbar_arrive(&bar->tail_clear[1]);
             }
             ring.next();
         }
-    } else if (warp == 9) {
-        // ---- matrix products
+    } else if (warp == 17 || warp == 18) {
+        // ---- matrix products of group g
+        const int g = warp - 17;
         if (elect_one()) {
             constexpr uint32_t kFormat = TYPE == SATORI_BF16 ? 1u : 0u;
             // FP32 accumulator, A and B of the cache's type, M = 128; S: N = 64, both K-major; O: N = HD, B MN-major.
             constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((uint32_t)(kTileRows >> 4) << 24);
             constexpr uint32_t kDescS = kBase | ((uint32_t)(kBlockKeys >> 3) << 17);
             constexpr uint32_t kDescO = kBase | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-            const uint32_t q_low = desc_low(smem_u32(q_tiles), 16), k_low = desc_low(smem_u32(stages), 16);
-            const uint32_t v_low = desc_low(smem_u32(stages), L::kHalf);
+            const uint32_t q_low = desc_low(smem_u32(q_tiles) + g * L::kQTile, 16), k_low = desc_low(smem_u32(stages), 16);
+            const uint32_t v_low = desc_low(smem_u32(stages), L::kHalf), s_col = tmem + g * 2 * kBlockKeys;
+            const uint32_t o_col = tmem + L::kOCol + g * HD;
+            // Both groups pass every load in order, and a stage is loaded again when both have released it: so
+            // the parity that a group waits for is never a round ahead of or behind the stage's.
             Ring<NS> ring;
-            uint32_t q_phase = 0, tail_phase = 0;      // bit g of q_phase: group g's parity
-            int done0 = 0, done1 = 0;                  // blocks of each group so far
+            uint32_t q_phase = 0, tail_phase = 0;
+            int done = 0;                              // this group's blocks so far
             bool ok = true, issued = false;
             for (int i = first; i < last && ok; ++i) {
                 const Work w = load_work(plan, i);
-                const int n = w.item.blocks, lead = w.lead();
-                // S = Q K^T of the group's block number `at`.
-                auto scores = [&](int g, int at, int stage) {
-                    const uint32_t d = tmem + (g * 2 + (at & 1)) * kBlockKeys;
-                    const uint32_t q = q_low + g * (L::kQTile >> 4), k = k_low + stage * (L::kTile >> 4);
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        mma_ss(d, q + (ks / 4) * (L::kQHalf >> 4) + (ks % 4) * 2, k + (ks / 4) * (L::kHalf >> 4) + (ks % 4) * 2,
-                               kDescS, ks > 0);
-                    commit(&bar->s_full[g][at & 1]);
+                const int n = w.blocks(g), all = w.item.blocks, lead = w.lead();
+                if (n > 0) {
+                    ok = wait(&bar->q_ready[g], q_phase);
+                    q_phase ^= 1u;
+                    issued = issued || ok;
+                }
+                auto mine = [&](int j) { return w.pair || (j & 1) == g; };
+                auto index = [&](int j) { return w.pair ? j : j >> 1; };
+                int held = -1;                         // a stage of V to release after the next scores
+                auto release_held = [&] {
+                    if (held >= 0) commit(&bar->empty[held]);
+                    held = -1;
                 };
-                // O += P V, once P is there.
-                auto values = [&](int g, int at, int stage, bool add) -> bool {
-                    if (!wait(&bar->p_ready[g][at & 1], (uint32_t)(at >> 1) & 1u)) return false;
-                    fence_after();
-                    const uint32_t p = tmem + (g * 2 + (at & 1)) * kBlockKeys, v = v_low + stage * (L::kTile >> 4);
-#pragma unroll
-                    for (int ks = 0; ks < kBlockKeys / 16; ++ks)
-                        mma_ts(tmem + L::kOCol + g * HD, p + ks * 8, v + ks * (2048 >> 4), kDescO, ks > 0 || add);
-                    commit(&bar->pv_done[g][at & 1]);
-                    return true;
-                };
-                // A small tile's group g has the blocks j = g, g + 2, ..; a large tile's groups have all of them.
-                auto block_scores = [&](int j) -> bool {
+                // S = Q K^T of block j, or K of the other group's block.
+                auto scores = [&](int j) -> bool {
                     if (!wait(&bar->full[ring.stage], ring.parity)) return false;
-                    fence_after();
-                    if (w.pair || (j & 1) == 0) scores(0, done0 + (w.pair ? j : j >> 1), ring.stage);
-                    if (w.pair || (j & 1) == 1) scores(1, done1 + (w.pair ? j : j >> 1), ring.stage);
-                    commit(&bar->empty[ring.stage]);
+                    if (mine(j)) {
+                        const int at = done + index(j);
+                        fence_after();
+                        const uint32_t d = s_col + (at & 1) * kBlockKeys, kd = k_low + ring.stage * (L::kTile >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks)
+                            mma_ss(d, q_low + (ks / 4) * (L::kQHalf >> 4) + (ks % 4) * 2,
+                                   kd + (ks / 4) * (L::kHalf >> 4) + (ks % 4) * 2, kDescS, ks > 0);
+                        commit(&bar->s_full[g][at & 1]);
+                        release_held();
+                        commit(&bar->empty[ring.stage]);
+                    } else {
+                        mbar_arrive(&bar->empty[ring.stage]);
+                    }
                     ring.next();
                     return true;
                 };
-                for (int g = 0; g < 2 && ok; ++g)
-                    if (w.blocks(g) > 0) {
-                        ok = wait(&bar->q_ready[g], q_phase >> g & 1);
-                        q_phase ^= 1u << g;
-                    }
-                fence_after();
-                issued = issued || ok;
-                for (int j = 0; j < lead && ok; ++j) ok = block_scores(j);
-                for (int j = 0; j < n && ok; ++j) {
-                    const int sv = ring.stage, next = j + lead;
-                    ok = wait(&bar->full[sv], ring.parity);
-                    if (ok && j + 1 == n && w.tail() > 0) {
-                        mbar_arrive(&bar->tail_full);
-                        ok = wait(&bar->tail_clear, tail_phase);
-                        tail_phase ^= 1u;
-                    }
-                    if (!ok) break;
-                    ring.next();
-                    if (w.pair) {
-                        // Each group's next scores follow its own O at once, so that it does not wait for the other.
-                        const int sk = ring.stage;
-                        ok = values(0, done0 + j, sv, j > 0);
-                        if (ok && next < n) {
-                            ok = wait(&bar->full[sk], ring.parity);
-                            if (!ok) break;
-                            ring.next();
-                            fence_after();
-                            scores(0, done0 + next, sk);
+                // O += P V of block j, once P is there.
+                auto values = [&](int j) -> bool {
+                    if (!wait(&bar->full[ring.stage], ring.parity)) return false;
+                    if (mine(j)) {
+                        const int k = index(j), at = done + k;
+                        if (j + 1 == all && w.tail() > 0) {
+                            if (w.tail_group() == g) mbar_arrive(&bar->tail_full[g]);
+                            if (!wait(&bar->tail_clear[g], tail_phase)) return false;
+                            tail_phase ^= 1u;
                         }
-                        ok = ok && values(1, done1 + j, sv, j > 0);
-                        if (!ok) break;
-                        commit(&bar->empty[sv]);
-                        if (next < n) {
-                            scores(1, done1 + next, sk);
-                            commit(&bar->empty[sk]);
+                        if (!wait(&bar->p_ready[g][at & 1], (uint32_t)(at >> 1) & 1u)) return false;
+                        fence_after();
+                        const uint32_t p = s_col + (at & 1) * kBlockKeys, vd = v_low + ring.stage * (L::kTile >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < kBlockKeys / 16; ++ks)
+                            mma_ts(o_col, p + ks * 8, vd + ks * (2048 >> 4), kDescO, ks > 0 || k > 0);
+                        // The next scores in this buffer follow O, which has read its weights; with them due, the
+                        // stage is released behind them.
+                        held = ring.stage;
+                        if (k + 2 >= n) {
+                            commit(k + 1 < n ? &bar->o_before[g] : &bar->o_full[g]);
+                            release_held();
                         }
                     } else {
-                        ok = (j & 1) ? values(1, done1 + (j >> 1), sv, j > 1) : values(0, done0 + (j >> 1), sv, j > 1);
-                        if (!ok) break;
-                        commit(&bar->empty[sv]);
-                        if (next < n) ok = block_scores(next);
+                        mbar_arrive(&bar->empty[ring.stage]);
                     }
+                    ring.next();
+                    return true;
+                };
+                for (int j = 0; j < lead && ok; ++j) ok = scores(j);
+                for (int j = 0; j < all && ok; ++j) {
+                    ok = values(j);
+                    if (ok && j + lead < all) ok = scores(j + lead);
                 }
-                done0 += w.blocks(0);
-                done1 += w.blocks(1);
+                done += n;
             }
             // The issued MMAs finish before the tensor memory is freed.
             if (issued) {
-                commit(&bar->drained);
-                mbar_wait_bounded(&bar->drained, 0);
+                commit(&bar->drained[g]);
+                mbar_wait_bounded(&bar->drained[g], 0);
             }
         }
         __syncwarp();
     } else {
-        // ---- softmax: thread r of group g owns tile row r (and tensor memory lane r)
-        const int g = warp >> 2, r = tid & (kTileRows - 1), quad = warp & 3;
+        // ---- softmax: the threads (half 0 and 1, r) of group g own tile row r (and tensor memory lane r).  Their
+        // waits are not left on an expired one: the two warps of a row meet at named barriers, so each goes
+        // on to the end, where every further wait returns at once.
+        const int g = warp >> 3, half = warp >> 2 & 1, quad = warp & 3, r = quad * 32 + lane;
+        const int pair_id = 1 + g * 4 + quad;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t o_addr = lanes + L::kOCol + g * HD;
+        const uint32_t o_addr = lanes + L::kOCol + g * HD + half * (HD / 2);
         uint8_t *q_tile = q_tiles + g * L::kQTile;
         int done = 0;                          // this group's blocks so far
-        bool ok = true;
-        for (int i = first; i < last && ok; ++i) {
+        uint32_t before_phase = 0, full_phase = 0;
+        for (int i = first; i < last; ++i) {
             const Work w = load_work(plan, i);
             const int blocks = w.blocks(g);
             const int m = (w.pair ? g * kTileRows : 0) + r;
             const bool live = m < w.item.m;
             const long long record = (long long)(w.item.slot + g) * kTileRows + r;
             if (blocks == 0) {                 // a small tile's only block is the other group's
-                if (live && !w.item.direct) plan->part_ml[record] = make_float2(-INFINITY, 0.0f);
+                if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(-INFINITY, 0.0f);
                 continue;
             }
             int2 own = make_int2(0, 0);        // the row's number and position
@@ -503,121 +657,122 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                             (w.item.m0 + m) / a.group);
             const int row = own.x, head = w.item.kv_head * a.group + (w.item.m0 + m) % a.group;
             const int limit = !live ? 0 : w.item.start >= 0 ? own.y + 1 - w.item.start : w.item.keys;
-            // Q rows of this warp into shared memory, K-major with the 128-byte swizzle: 16-byte chunk c of row r
-            // lies at chunk c ^ (r % 8).  All loads are in flight before the first store.
-            {
-                constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, STEPS = 32 / ROWS;
-                const long long q_off = live ? (long long)row * a.ldq + (long long)head * HD : -1;
-                const int c = lane % PER_ROW;
+            // Q rows into shared memory (each half 16 of the warp pair's 32), K-major with the 128-byte swizzle:
+            // 16-byte chunk c of row r lies at chunk c ^ (r % 8).  Rows behind the tile keep what was there: their
+            // lanes of S and O are never read.  All loads are in flight before the first store.
+            const int warp_rows = min(32, w.item.m - (m - lane));          // live rows of the warp pair
+            if (half * 16 < warp_rows) {
+                constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, STEPS = 16 / ROWS;
+                const int c = lane % PER_ROW, mine = half * 16 + lane / PER_ROW, q_head = head * HD;
                 uint4 v[STEPS];
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    const long long off = __shfl_sync(0xFFFFFFFFu, q_off, k * ROWS + lane / PER_ROW);
+                    const int from = mine + k * ROWS;
+                    const int r_from = __shfl_sync(0xFFFFFFFFu, row, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
+                    const T *src = reinterpret_cast<const T *>(a.q) + (long long)r_from * a.ldq + h_from + c * 8;
                     v[k] = make_uint4(0, 0, 0, 0);
-                    const T *src = reinterpret_cast<const T *>(a.q) + off + c * 8;
-                    if (off >= 0 && t.wide_q) {
-                        v[k] = __ldg(reinterpret_cast<const uint4 *>(src));
-                    } else if (off >= 0) {
-                        const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
-                        v[k] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16,
-                                          h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-                    }
+                    if (from < warp_rows) v[k] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
                 }
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    const int rr = quad * 32 + k * ROWS + lane / PER_ROW;
-                    *reinterpret_cast<uint4 *>(q_tile + (c / 8) * L::kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) * 16)) = v[k];
+                    const int from = mine + k * ROWS, rr = quad * 32 + from;
+                    if (from < warp_rows)
+                        *reinterpret_cast<uint4 *>(q_tile + (c / 8) * L::kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) * 16)) = v[k];
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&bar->q_ready[g]);
 
-            const bool idle = __ballot_sync(0xFFFFFFFFu, live) == 0;       // the whole warp: rows behind the tile
+            const bool idle = warp_rows <= 0;  // all of the warp pair's rows are behind the tile
             float ref = -INFINITY, sum = 0;    // ref: the maximum (log2 units) that the weights refer to
             for (int k = 0; k < blocks; ++k) {
                 const int block = w.item.block0 + (w.pair ? k : 2 * k + g), at = done + k;
                 const uint32_t s_addr = lanes + (g * 2 + (at & 1)) * kBlockKeys;
-                ok = __all_sync(0xFFFFFFFFu, wait(&bar->s_full[g][at & 1], (uint32_t)(at >> 1) & 1u));
-                if (!ok) break;
-                fence_after();
+                wait(&bar->s_full[g][at & 1], (uint32_t)(at >> 1) & 1u);
                 if (!idle) {
-                    const int see = limit - block * kBlockKeys;            // keys of the block that the row sees
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t s[2][32];
-                    tmem_load32(s_addr, s[0]);
-                    tmem_load32(s_addr + 32, s[1]);
-                    tmem_wait_load(s[0]);
-                    tmem_wait_load(s[1]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        mask_scores(s[c], see - c * 32);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c][e]));
-                    }
-                    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-                    const bool raise = high > ref + kLazy || (k == 0 && high > -INFINITY);
-                    if (k > 0 && __any_sync(0xFFFFFFFFu, raise)) {
-                        // The last block's product may still be adding to O.
-                        ok = __all_sync(0xFFFFFFFFu, wait(&bar->pv_done[g][(at - 1) & 1], (uint32_t)((at - 1) >> 1) & 1u));
-                        if (!ok) break;
-                        fence_after();
-                        const float factor = raise ? exp2_fast(ref - high) : 1.0f;
-#pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t o[32];
-                            tmem_load32(o_addr + c, o);
-                            tmem_wait_load(o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                            tmem_store32(o_addr + c, o);
-                        }
-                        sum *= factor;
-                    }
-                    if (raise) ref = high;
-                    const float base = ref == -INFINITY ? 0.0f : ref;
-                    float add[4] = {0, 0, 0, 0};
-                    uint32_t p[32];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float u = exp2_fast(fmaf(__uint_as_float(s[c][e]), a.scale_log2, -base));
-                            const float v = exp2_fast(fmaf(__uint_as_float(s[c][e + 1]), a.scale_log2, -base));
-                            add[e & 2] += u;
-                            add[(e & 2) + 1] += v;
-                            p[c * 16 + e / 2] = pack2<TYPE>(u, v);
-                        }
-                    sum += (add[0] + add[1]) + (add[2] + add[3]);
                     __syncwarp();
-                    tmem_store32(s_addr, p);
+                    fence_after();
+                    const int see = limit - block * kBlockKeys - half * 32;        // keys of this half that the row sees
+                    uint32_t s[32];
+                    tmem_load32(s_addr + half * 32, s);
+                    tmem_wait_load(s);
+                    const bool masked = __any_sync(0xFFFFFFFFu, see < 32);
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (e >= see) s[e] = 0xFF800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) top[e / 2 & 3] = max3(top[e / 2 & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                    float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
+                    // (The barrier also keeps one half's weights from the scores that the other has yet to read.)
+                    if (pair_any(pair_id, high > ref + kLazy || (k == 0 && high > -INFINITY))) {
+                        bar->exchange[g][half][r] = high;
+                        pair_sync(pair_id);
+                        high = fmaxf(high, bar->exchange[g][half ^ 1][r]);
+                        const bool raise = high > ref + kLazy || (k == 0 && high > -INFINITY);
+                        if (k > 0) {
+                            // The last block's product may still be adding to O.  The next block's scores follow it.
+                            if (k + 1 < blocks)
+                                wait(&bar->s_full[g][(at + 1) & 1], (uint32_t)((at + 1) >> 1) & 1u);
+                            else
+                                wait(&bar->o_before[g], before_phase);
+                            __syncwarp();
+                            fence_after();
+                            const float factor = raise ? exp2_fast(ref - high) : 1.0f;
+#pragma unroll
+                            for (int c = 0; c < HD / 2; c += 16) {
+                                uint32_t o[16];
+                                tmem_load16(o_addr + c, o);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                                tmem_store16(o_addr + c, o);
+                            }
+                            sum *= factor;
+                        }
+                        if (raise) ref = high;
+                    }
+                    const float base = ref == -INFINITY ? 0.0f : ref;
+                    uint32_t p[16];
+                    // A masked key's weight is exactly zero, which the polynomial cannot give.
+                    sum += masked ? block_weights<TYPE, 0>(s, a.scale_log2, base, p)
+                                  : block_weights<TYPE, kEvery>(s, a.scale_log2, base, p);
+                    __syncwarp();
+                    tmem_store16(s_addr + half * 16, p);
                     tmem_wait_store();
                 }
                 fence_before();
                 mbar_arrive(&bar->p_ready[g][at & 1]);
             }
-            if (!ok) break;
             done += blocks;
-            ok = __all_sync(0xFFFFFFFFu, wait(&bar->pv_done[g][(done - 1) & 1], (uint32_t)((done - 1) >> 1) & 1u));
-            if (!ok) break;
-            fence_after();
+            if (blocks > 1) before_phase ^= 1u;
+            wait(&bar->o_full[g], full_phase);
+            full_phase ^= 1u;
             if (idle) continue;
+            bar->exchange[g][half][r] = sum;
+            pair_sync(pair_id);
+            sum += bar->exchange[g][half ^ 1][r];
+            __syncwarp();
+            fence_after();
             const float inverse = 1.0f / sum;
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
+            for (int c = 0; c < HD / 2; c += 32) {
                 uint32_t o[32];
                 tmem_load32(o_addr + c, o);
                 tmem_wait_load(o);
-                if (live) store_output<TYPE, HD>(t, plan, w, o, inverse, row, head, record, c);
+                if (live) store_output<TYPE, HD>(t, plan, w, o, inverse, row, head, record, half * (HD / 2) + c);
                 __syncwarp();
             }
-            if (live && !w.item.direct) plan->part_ml[record] = make_float2(ref, sum);
+            if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(ref, sum);
             // The next item's first O overwrites this one after this group's next p_ready, so these loads are done.
+            // The other half has read this sum before either writes the exchange again (both pass pair_any first).
             fence_before();
         }
     }
     fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 template <int TYPE, int HD>
@@ -658,18 +813,29 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 
 cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim, int page_tokens, unsigned long long blocks)
 {
-    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)page_tokens, (cuuint64_t)blocks};
-    const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)head_dim * 2 * page_tokens};
-    const cuuint32_t box[3] = {64, (cuuint32_t)std::min(page_tokens, kBlockKeys), 1}, ones[3] = {1, 1, 1};
     void *f = nullptr;
     cudaDriverEntryPointQueryResult found;
     cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
     if (e != cudaSuccess) return e;
     if (found != cudaDriverEntryPointSuccess || !f) return cudaErrorNotSupported;
-    const CUresult r = reinterpret_cast<EncodeTiled>(f)(
-        map, type == SATORI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, memory, dims,
-        strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType kind = type == SATORI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t row = (cuuint64_t)head_dim * 2, block = row * page_tokens;
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    CUresult r;
+    if (page_tokens >= kBlockKeys) {       // [block][half][token][64]: a box is a block of keys, half by half
+        const cuuint64_t dims[4] = {64, (cuuint64_t)page_tokens, (cuuint64_t)head_dim / 64, (cuuint64_t)blocks};
+        const cuuint64_t strides[3] = {row, 128, block};
+        const cuuint32_t box[4] = {64, kBlockKeys, (cuuint32_t)head_dim / 64, 1};
+        r = reinterpret_cast<EncodeTiled>(f)(map, kind, 4, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else {                               // [block][token][dim]: a box is one half of a page
+        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)page_tokens, (cuuint64_t)blocks}, strides[2] = {row, block};
+        const cuuint32_t box[3] = {64, (cuuint32_t)page_tokens, 1};
+        r = reinterpret_cast<EncodeTiled>(f)(map, kind, 3, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 

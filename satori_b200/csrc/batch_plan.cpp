@@ -88,6 +88,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
     plan.partials = 0;
 
     Builder b{shape, members, plan, {}, std::vector<int>((size_t)n), std::vector<std::vector<Builder::Place>>((size_t)n)};
+    std::vector<int> alone;                            // members that share no segment
     for (int i = 0; i < n; ++i) {
         b.row0[i] = (int)plan.row_position.size();
         const PlanMember &m = members[i];
@@ -97,13 +98,21 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
             plan.row_page.push_back(m.pages[pos / shape.page_tokens]);
             plan.row_slot.push_back(pos % shape.page_tokens);
         }
-        if (m.rows > 0) b.order.push_back(i);
+        // Rows that fill tiles of their own gain nothing from a shared segment (its keys are read once per tile
+        // either way); with all their keys in one segment most of their tiles need no merge.
+        if (m.rows * shape.group >= shape.tile_m)
+            alone.push_back(i);
+        else if (m.rows > 0)
+            b.order.push_back(i);
     }
     std::stable_sort(b.order.begin(), b.order.end(), [&](int x, int y) {
         return std::lexicographical_compare(members[x].pages, members[x].pages + members[x].n_pages, members[y].pages,
                                             members[y].pages + members[y].n_pages);
     });
-    b.walk(0, (int)b.order.size(), 0, 0);
+    const int sharing = (int)b.order.size();
+    b.walk(0, sharing, 0, 0);
+    b.order.insert(b.order.end(), alone.begin(), alone.end());
+    for (int i = sharing; i < (int)b.order.size(); ++i) b.walk(i, i + 1, 0, 0);
     for (int i = 0; i < n; ++i)
         if (b.places[i].size() == 1) plan.segments[b.places[i][0].segment].sole = 1;
 
@@ -178,11 +187,29 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                 if (direct) slots.first = -1;
             }
     }
+    // Rows whose outputs come from several items: all of those with several segments, and of the others those in
+    // a tile that was cut.
+    plan.merges.clear();
+    for (int i = 0; i < n; ++i)
+        if (b.places[i].size() > 1)
+            for (int r = 0; r < members[i].rows * shape.kv_heads; ++r) plan.merges.push_back(b.row0[i] * shape.kv_heads + r);
+    for (const PlanSegment &seg : plan.segments) {
+        if (!seg.sole) continue;
+        const int tiles = (seg.rows * shape.group + shape.tile_m - 1) / shape.tile_m;
+        for (int h = 0; h < shape.kv_heads; ++h)
+            for (int t = seg.tile0, next = 0; t < seg.tile0 + tiles; ++t) {
+                const PlanTile &tile = plan.tiles[t];
+                if (plan.slots[(size_t)t * shape.kv_heads + h].first < 0) continue;
+                const int end = (tile.m0 + tile.m - 1) / shape.group + 1;
+                for (next = std::max(next, tile.m0 / shape.group); next < end; ++next)
+                    plan.merges.push_back(plan.seg_rows[seg.row_off + next].row * shape.kv_heads + h);
+            }
+    }
     while ((int)plan.cta_off.size() <= shape.ctas) plan.cta_off.push_back((int)plan.items.size());
     plan.head.rows = (int)plan.row_position.size();
     plan.head.segments = (int)plan.segments.size();
-    plan.head.tiles = (int)plan.tiles.size();
     plan.head.items = (int)plan.items.size();
+    plan.head.merges = (int)plan.merges.size();
 }
 
 }  // namespace satori

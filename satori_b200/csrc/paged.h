@@ -78,7 +78,7 @@ struct PlanMember {
 };
 
 struct PlanHeader {
-    int rows, segments, tiles, items;
+    int rows, segments, items, merges;
 };
 struct PlanRow {
     int row, position;                                 // a segment's row: its number in the step and its position
@@ -107,6 +107,7 @@ struct PlanLink {
 struct Plan {
     PlanHeader head;
     std::vector<int> row_position, row_page, row_slot, chain_off, pages, cta_off;
+    std::vector<int> merges;                           // row * kv_heads + KV head of what no single item writes
     std::vector<PlanRow> seg_rows;
     std::vector<PlanLink> chain;
     std::vector<PlanSegment> segments;
