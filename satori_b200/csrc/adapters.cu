@@ -5,7 +5,7 @@
 // batch, the quantized projection once for all rows (satori_matrix_execute_device) and each row's own
 // low-rank term beside it.
 //
-// One launch.  The rows are grouped by slot into items of at most 16 or 32 rows; a thread-block cluster takes
+// One launch.  The rows are grouped by slot into items of up to 16, 32 or 64 rows; a thread-block cluster takes
 // an item: its warps split the columns for t = A x, the partial t meet in shared memory and, across the
 // cluster's CTAs, in distributed shared memory, and the warps split the output rows for B t.  So t never
 // leaves the SMs, x is read once, base and out are touched once, and nothing is added by atomics: the order
@@ -31,7 +31,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kMaxRank = 128, kMaxCluster = 8;
+constexpr int kMaxRank = 128, kMaxCluster = 8, kItemRows = 64;
 
 struct SlotDesc {
     const uint8_t *a, *b;                      // A [rank16][cols32] and B [rows][rank16], zero padded
@@ -43,9 +43,9 @@ struct RowItem {
     int slot, row_off, rows;
 };
 
-// Header of a row plan in device memory; the items for 16- and 32-row tiles and the row list follow.
+// Header of a row plan in device memory; the items and the row list follow.
 struct DevRows {
-    int items[2], item_off[2], rows_off, pad[3];
+    int items, item_off, rows_off, pad;
 };
 
 struct AdapterArgs {
@@ -135,203 +135,256 @@ __device__ __forceinline__ void mma_parts(float *d, const uint32_t (*a)[4], cons
 }
 
 // ------------------------------------------------------------------------------------------- the kernel
-// RM: ranks at most, MT: 16-row tiles of an item.
-template <int RM, int MT>
+// RM: ranks at most.
+template <int RM>
 struct AdapterSmem {
-    static constexpr int TP = 16 * MT;
-    union {
-        float red[kWarps][TP][RM + 4];         // the warps' partial t
-        uint32_t parts[3][TP][RM / 2 + 4];     // t in bf16 parts, pairs of ranks
-    };
-    float t[TP][RM + 4];                       // the CTA's partial t, read by the whole cluster
-    int row[TP];
+    float red[kWarps][16][RM + 4];             // the warps' partial t of a 16-row tile
+    float t[kItemRows][RM + 4];                // the CTA's partial t, read by the whole cluster
+    uint32_t parts[3][kItemRows][RM / 2 + 4];  // t in bf16 parts, pairs of ranks
+    int row[kItemRows];
 };
 
-template <int TYPE, int RM, int MT>
-__global__ void __launch_bounds__(kThreads) adapter_kernel(const AdapterArgs a)
+template <int TYPE, int RM>
+__global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(const AdapterArgs a)
 {
     typedef Weights<TYPE> W;
-    typedef AdapterSmem<RM, MT> Smem;
-    constexpr int TP = Smem::TP, NT = RM / 8;
+    typedef AdapterSmem<RM> Smem;
+    // Tiles of 8 ranks taken together: their weights and sums fit the registers beside x.
+    constexpr int NT = RM / 8 < (TYPE == SATORI_F32 ? 4 : 8) ? RM / 8 : (TYPE == SATORI_F32 ? 4 : 8);
     constexpr int RAW = W::kBytes * 8 / 4;     // words of 8 weights
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
     const int *plan = reinterpret_cast<const int *>(a.plan);
-    const int variant = MT - 1, items = a.plan->items[variant];
-    const RowItem *list = reinterpret_cast<const RowItem *>(plan + a.plan->item_off[variant]);
+    const int items = a.plan->items;
+    const RowItem *list = reinterpret_cast<const RowItem *>(plan + a.plan->item_off);
     const int *rows = plan + a.plan->rows_off;
 
     for (int it = blockIdx.x / ctas; it < items; it += gridDim.x / ctas) {
         const RowItem item = list[it];
         SlotDesc slot = {};
         if (item.slot >= 0) slot = a.slots[item.slot];
-        const int nt = slot.rank16 / 8;
-        if (tid < TP) sm.row[tid] = tid < item.rows ? rows[item.row_off + tid] : -1;
+        const int rank = slot.rank16, tiles = (item.rows + 15) / 16;
+        if (tid < kItemRows) sm.row[tid] = tid < item.rows ? rows[item.row_off + tid] : -1;
         __syncthreads();
-        if (nt > 0) {
-            // t = A x.  Each warp takes every (8 * ctas)-th run of 32 columns.  A lane holds 8 consecutive columns
-            // of a row: the MMA's k index is a permutation of the run's columns, the same for x and A.
-            float acc[MT][NT][4];
+        if (rank > 0) {
+            // t = A x, 16 rows and 8 NT ranks at a time.  Each warp takes every (8 * ctas)-th run of 32 columns.  A
+            // lane holds 8 consecutive columns of a row: the MMA's k index is a permutation of the run's columns,
+            // the same for x and A.
+            for (int i = 0; i < tiles; ++i) {
+                const int row0 = sm.row[i * 16 + g], row1 = sm.row[i * 16 + 8 + g];
+                for (int j0 = 0; j0 * 8 < rank; j0 += NT) {
+                    const int nt = min(NT, rank / 8 - j0);
+                    float acc[NT][4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                        for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+                    for (int k0 = (cta * kWarps + warp) * 32; k0 < a.cols32; k0 += ctas * kWarps * 32) {
+                        const int k = k0 + q * 8;
+                        uint32_t raw[NT][RAW];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
-            for (int k0 = (cta * kWarps + warp) * 32; k0 < a.cols32; k0 += ctas * kWarps * 32) {
-                const int k = k0 + q * 8;
-                float x[MT][2][8];
+                        for (int j = 0; j < NT; ++j)
+                            if (j < nt) {
+                                const uint4 *src = reinterpret_cast<const uint4 *>(
+                                    slot.a + ((long long)((j0 + j) * 8 + g) * a.cols32 + k) * W::kBytes);
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int row = sm.row[i * 16 + h * 8 + g];
-                        const float *src = a.x + row * a.ldx + k;
-                        if (row >= 0 && a.wide_x && k + 8 <= a.cols) {
-#pragma unroll
-                            for (int e = 0; e < 8; e += 4) {
-                                const float4 v = __ldg(reinterpret_cast<const float4 *>(src + e));
-                                x[i][h][e] = v.x;
-                                x[i][h][e + 1] = v.y;
-                                x[i][h][e + 2] = v.z;
-                                x[i][h][e + 3] = v.w;
+                                for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[j][4 * e]) = __ldg(src + e);
                             }
-                        } else {
+                        float x[2][8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[i][h][e] = row >= 0 && k + e < a.cols ? __ldg(src + e) : 0.0f;
+                        for (int h = 0; h < 2; ++h) {
+                            const int row = h ? row1 : row0;
+                            const float *src = a.x + row * a.ldx + k;
+                            if (row >= 0 && a.wide_x && k + 8 <= a.cols) {
+#pragma unroll
+                                for (int e = 0; e < 8; e += 4) {
+                                    const float4 v = __ldg(reinterpret_cast<const float4 *>(src + e));
+                                    x[h][e] = v.x;
+                                    x[h][e + 1] = v.y;
+                                    x[h][e + 2] = v.z;
+                                    x[h][e + 3] = v.w;
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[h][e] = row >= 0 && k + e < a.cols ? __ldg(src + e) : 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            uint32_t xa[3][4];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    uint32_t p[3];
+                                    split<3>(x[h][4 * s + 2 * e], x[h][4 * s + 2 * e + 1], p);
+#pragma unroll
+                                    for (int c = 0; c < 3; ++c) xa[c][2 * e + h] = p[c];
+                                }
+#pragma unroll
+                            for (int j = 0; j < NT; ++j)
+                                if (j < nt) {
+                                    uint32_t wb[W::kParts][2];
+                                    weight_parts<TYPE>(&raw[j][s * RAW / 2], wb);
+                                    mma_parts<W::kParts>(acc[j], xa, wb);
+                                }
                         }
                     }
-                uint32_t raw[NT][RAW];
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    if (j < nt) {
-                        const uint4 *src = reinterpret_cast<const uint4 *>(
-                            slot.a + ((long long)(j * 8 + g) * a.cols32 + k) * W::kBytes);
-#pragma unroll
-                        for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[j][4 * e]) = __ldg(src + e);
-                    }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    uint32_t xa[MT][3][4];
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                uint32_t p[3];
-                                split<3>(x[i][h][4 * s + 2 * e], x[i][h][4 * s + 2 * e + 1], p);
-#pragma unroll
-                                for (int c = 0; c < 3; ++c) xa[i][c][2 * e + h] = p[c];
-                            }
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
                         if (j < nt) {
-                            uint32_t wb[W::kParts][2];
-                            weight_parts<TYPE>(&raw[j][s * RAW / 2], wb);
-#pragma unroll
-                            for (int i = 0; i < MT; ++i) mma_parts<W::kParts>(acc[i][j], xa[i], wb);
+                            float *d = &sm.red[warp][g][(j0 + j) * 8 + 2 * q];
+                            *reinterpret_cast<float2 *>(d) = make_float2(acc[j][0], acc[j][1]);
+                            *reinterpret_cast<float2 *>(d + 8 * (RM + 4)) = make_float2(acc[j][2], acc[j][3]);
                         }
                 }
-            }
+                __syncthreads();
+                for (int e = tid; e < 4 * rank; e += kThreads) {
+                    const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
+                    float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    if (j < nt) {
-                        float *d = &sm.red[warp][i * 16 + g][j * 8 + 2 * q];
-                        *reinterpret_cast<float2 *>(d) = make_float2(acc[i][j][0], acc[i][j][1]);
-                        *reinterpret_cast<float2 *>(d + 8 * (RM + 4)) = make_float2(acc[i][j][2], acc[i][j][3]);
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float4 v = *reinterpret_cast<const float4 *>(&sm.red[w][p][r]);
+                        sum.x += v.x;
+                        sum.y += v.y;
+                        sum.z += v.z;
+                        sum.w += v.w;
                     }
-            __syncthreads();
-            const int rank = nt * 8;
-            for (int i = tid; i < TP * rank; i += kThreads) {
-                const int p = i / rank, r = i % rank;
-                float sum = 0;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += sm.red[w][p][r];
-                sm.t[p][r] = sum;
+                    *reinterpret_cast<float4 *>(&sm.t[i * 16 + p][r]) = sum;
+                }
+                __syncthreads();
             }
             cluster.sync();
             // The whole t, scaled, in bf16 parts.
-            for (int i = tid; i < TP * rank / 2; i += kThreads) {
-                const int p = i / (rank / 2), r = 2 * (i % (rank / 2));
-                float2 sum = make_float2(0, 0);
+            for (int e = tid; e < tiles * 4 * rank; e += kThreads) {
+                const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
+                float4 sum = make_float4(0, 0, 0, 0);
                 for (int c = 0; c < ctas; ++c) {
-                    const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&sm.t[p][r], c));
+                    const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sm.t[p][r], c));
                     sum.x += v.x;
                     sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
                 }
-                uint32_t part[3];
-                split<3>(sum.x * slot.scale, sum.y * slot.scale, part);
+                uint32_t lo[3], hi[3];
+                split<3>(sum.x * slot.scale, sum.y * slot.scale, lo);
+                split<3>(sum.z * slot.scale, sum.w * slot.scale, hi);
 #pragma unroll
-                for (int c = 0; c < 3; ++c) sm.parts[c][p][r / 2] = part[c];
+                for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2 *>(&sm.parts[c][p][r / 2]) = make_uint2(lo[c], hi[c]);
             }
             __syncthreads();
         }
         // out = base + B t: each warp takes runs of 32 output rows.  Lane (g, q) ends up with 8 consecutive
         // outputs, 8 q .. 8 q + 7, of tile rows g and g + 8: column 2 q + e of the MMA's n-tile j stands for
-        // output 8 q + 2 j + e.
+        // output 8 q + 2 j + e.  A run's weights stay in registers for all of the item's rows; ranks go 32 at a
+        // time (a lane holds 8 consecutive ones), the last 16 of an odd number of 16s with 4 a lane.
+        constexpr int C32 = RM / 32 < 2 ? 1 : (TYPE == SATORI_F32 ? 1 : 2);        // runs of 32 ranks held at once
         for (int o0 = (cta * kWarps + warp) * 32; o0 < a.rows; o0 += ctas * kWarps * 32) {
-            float acc[MT][4][4];
+            const int o = o0 + 8 * q;
+            for (int i = 0; i < tiles; ++i) {
+                float base[2][8], acc[4][4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int h = 0; h < 2; ++h) {
+                    const int row = sm.row[i * 16 + h * 8 + g];
+                    const float *src = a.base + row * a.ldbase + o;
+                    if (row >= 0 && a.wide_out && o + 8 <= a.rows) {
+                        *reinterpret_cast<float4 *>(&base[h][0]) = *reinterpret_cast<const float4 *>(src);
+                        *reinterpret_cast<float4 *>(&base[h][4]) = *reinterpret_cast<const float4 *>(src + 4);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) base[h][e] = row >= 0 && o + e < a.rows ? src[e] : 0.0f;
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
-            for (int s = 0; s < nt / 2; ++s) {             // 16 ranks: lane q holds 4 consecutive ones
-                uint32_t ta[MT][3][4];
+                    for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+                for (int r0 = 0; r0 < rank; r0 += 32 * C32) {
+                    uint32_t raw[C32][4][RAW];
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                    for (int c = 0; c < C32; ++c)
 #pragma unroll
-                    for (int c = 0; c < 3; ++c)
+                        for (int j = 0; j < 4; ++j) {
+                            const int out = min(o0 + 8 * (g >> 1) + 2 * j + (g & 1), a.rows - 1), r = r0 + 32 * c;
+                            const uint8_t *src = slot.b + ((long long)out * rank + r) * W::kBytes;
+                            if (r + 32 <= rank) {
+                                const uint4 *from = reinterpret_cast<const uint4 *>(src + q * 8 * W::kBytes);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(&sm.parts[c][i * 16 + h * 8 + g][s * 8 + q * 2]);
-                            ta[i][c][h] = v.x;
-                            ta[i][c][2 + h] = v.y;
+                                for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[c][j][4 * e]) = __ldg(from + e);
+                            } else if (r < rank) {
+                                const uint2 *from = reinterpret_cast<const uint2 *>(src + q * 4 * W::kBytes);
+#pragma unroll
+                                for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint2 *>(&raw[c][j][2 * e]) = __ldg(from + e);
+                            }
                         }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int o = min(o0 + 8 * (g >> 1) + 2 * j + (g & 1), a.rows - 1);
-                    const uint8_t *src = slot.b + ((long long)o * slot.rank16 + s * 16 + q * 4) * W::kBytes;
-                    uint32_t raw[RAW / 2];
+                    for (int c = 0; c < C32; ++c) {
+                        const int r = r0 + 32 * c;
+                        const bool whole = r + 32 <= rank;
+                        if (r >= rank) continue;
+                        // t of this lane's ranks: 8 of them for two steps, or 4 for one.
+                        uint32_t ta[3][2][4];
 #pragma unroll
-                    for (int e = 0; e < RAW / 2; e += 2)
-                        *reinterpret_cast<uint2 *>(&raw[e]) = __ldg(reinterpret_cast<const uint2 *>(src) + e / 2);
-                    uint32_t wb[W::kParts][2];
-                    weight_parts<TYPE>(raw, wb);
+                        for (int p = 0; p < 3; ++p)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) mma_parts<W::kParts>(acc[i][j], ta[i], wb);
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t *src = &sm.parts[p][i * 16 + h * 8 + g][r / 2];
+                                if (whole) {
+                                    const uint4 v = *reinterpret_cast<const uint4 *>(src + q * 4);
+                                    ta[p][h][0] = v.x;
+                                    ta[p][h][1] = v.y;
+                                    ta[p][h][2] = v.z;
+                                    ta[p][h][3] = v.w;
+                                } else {
+                                    const uint2 v = *reinterpret_cast<const uint2 *>(src + q * 2);
+                                    ta[p][h][0] = v.x;
+                                    ta[p][h][1] = v.y;
+                                    ta[p][h][2] = ta[p][h][3] = 0;
+                                }
+                            }
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            if (s == 1 && !whole) continue;
+                            uint32_t frag[3][4];
+#pragma unroll
+                            for (int p = 0; p < 3; ++p) {
+                                frag[p][0] = ta[p][0][2 * s];
+                                frag[p][1] = ta[p][1][2 * s];
+                                frag[p][2] = ta[p][0][2 * s + 1];
+                                frag[p][3] = ta[p][1][2 * s + 1];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t wb[W::kParts][2];
+                                weight_parts<TYPE>(&raw[c][j][s * RAW / 2], wb);
+                                mma_parts<W::kParts>(acc[j], frag, wb);
+                            }
+                        }
+                    }
                 }
-            }
-            const int o = o0 + 8 * q;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = sm.row[i * 16 + h * 8 + g];
                     if (row < 0) continue;
-                    const float *base = a.base + row * a.ldbase + o;
                     float *out = a.out + row * a.ldo + o;
                     if (a.wide_out && o + 8 <= a.rows) {
 #pragma unroll
-                        for (int j = 0; j < 4; j += 2) {
-                            const float4 b = *reinterpret_cast<const float4 *>(base + 2 * j);
+                        for (int j = 0; j < 4; j += 2)
                             *reinterpret_cast<float4 *>(out + 2 * j) =
-                                make_float4(b.x + acc[i][j][2 * h], b.y + acc[i][j][2 * h + 1],
-                                            b.z + acc[i][j + 1][2 * h], b.w + acc[i][j + 1][2 * h + 1]);
-                        }
+                                make_float4(base[h][2 * j] + acc[j][2 * h], base[h][2 * j + 1] + acc[j][2 * h + 1],
+                                            base[h][2 * j + 2] + acc[j + 1][2 * h], base[h][2 * j + 3] + acc[j + 1][2 * h + 1]);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (o + e < a.rows) out[e] = base[e] + acc[i][e / 2][2 * h + (e & 1)];
+                            if (o + e < a.rows) out[e] = base[h][e] + acc[e / 2][2 * h + (e & 1)];
                     }
                 }
+            }
         }
         cluster.sync();                        // nobody still reads this CTA's t
     }
@@ -352,7 +405,7 @@ struct satori_adapters {
 struct satori_adapter_rows {
     satori_ctx *ctx = nullptr;
     int rows = -1, top_slot = -1;              // rows assigned, highest slot used
-    int items[2] = {0, 0};
+    int items = 0;
     int *d_plan = nullptr;
     size_t plan_ints = 0;
     std::vector<void *> outgrown;              // kept for graphs captured before the plan moved
@@ -361,11 +414,11 @@ struct satori_adapter_rows {
 
 namespace {
 
-template <int TYPE, int RM, int MT>
+template <int TYPE, int RM>
 cudaError_t launch_variant(const AdapterArgs &a, int items, int sm_count, cudaStream_t stream)
 {
-    auto kernel = adapter_kernel<TYPE, RM, MT>;
-    const size_t smem = sizeof(AdapterSmem<RM, MT>);
+    auto kernel = adapter_kernel<TYPE, RM>;
+    const size_t smem = sizeof(AdapterSmem<RM>);
     cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
     // The smallest cluster that gives the SMs two CTAs each: few items are spread over many SMs, many items
@@ -378,23 +431,25 @@ cudaError_t launch_variant(const AdapterArgs &a, int items, int sm_count, cudaSt
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <int TYPE>
-cudaError_t launch_adapters(const AdapterArgs &a, int rank, const int *items, int sm_count, cudaStream_t stream)
+cudaError_t launch_adapters(const AdapterArgs &a, int rank, int items, int sm_count, cudaStream_t stream)
 {
-    if (rank <= 16) return launch_variant<TYPE, 16, 2>(a, items[1], sm_count, stream);
-    if (rank <= 32) return launch_variant<TYPE, 32, 2>(a, items[1], sm_count, stream);
-    if (rank <= 64) return launch_variant<TYPE, 64, 2>(a, items[1], sm_count, stream);
-    return launch_variant<TYPE, 128, 1>(a, items[0], sm_count, stream);
+    if (rank <= 16) return launch_variant<TYPE, 16>(a, items, sm_count, stream);
+    if (rank <= 32) return launch_variant<TYPE, 32>(a, items, sm_count, stream);
+    if (rank <= 64) return launch_variant<TYPE, 64>(a, items, sm_count, stream);
+    return launch_variant<TYPE, 128>(a, items, sm_count, stream);
 }
 
 bool overlap(const void *a, size_t na, const void *b, size_t nb)
@@ -519,22 +574,23 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
         std::vector<int> order((size_t)n);
         for (int i = 0; i < n; ++i) order[i] = i;
         std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return slots[x] < slots[y]; });
-        std::vector<RowItem> items[2];
-        for (int i = 0; i < n;) {
-            int end = i;
-            while (end < n && slots[order[end]] == slots[order[i]]) ++end;
-            for (int v = 0; v < 2; ++v)
-                for (int at = i; at < end; at += 16 * (v + 1))
-                    items[v].push_back({slots[order[i]], at, std::min(16 * (v + 1), end - at)});
-            i = end;
+        // The largest items that still give every SM one (an item's rows share the weights' loads): 64, 32 or 16.
+        std::vector<RowItem> items;
+        for (int most = kItemRows; most >= 16; most /= 2) {
+            items.clear();
+            for (int i = 0; i < n;) {
+                int end = i;
+                while (end < n && slots[order[end]] == slots[order[i]]) ++end;
+                for (int at = i; at < end; at += most) items.push_back({slots[order[i]], at, std::min(most, end - at)});
+                i = end;
+            }
+            if ((int)items.size() >= ctx->sm_count) break;
         }
         DevRows head = {};
         size_t ints = sizeof(DevRows) / 4;
-        for (int v = 0; v < 2; ++v) {
-            head.items[v] = (int)items[v].size();
-            head.item_off[v] = (int)ints;
-            ints += items[v].size() * sizeof(RowItem) / 4;
-        }
+        head.items = (int)items.size();
+        head.item_off = (int)ints;
+        ints += items.size() * sizeof(RowItem) / 4;
         head.rows_off = (int)ints;
         ints += (size_t)n;
         if (ints > r->plan_ints) {
@@ -551,15 +607,13 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
         if ((e = r->staging.take(ints * 4, &buffer)) != cudaSuccess) return cuda_fail(e, "stage adapter rows");
         int *stage = static_cast<int *>(buffer);
         memcpy(stage, &head, sizeof head);
-        for (int v = 0; v < 2; ++v)
-            if (n) memcpy(stage + head.item_off[v], items[v].data(), items[v].size() * sizeof(RowItem));
+        if (n) memcpy(stage + head.item_off, items.data(), items.size() * sizeof(RowItem));
         if (n) memcpy(stage + head.rows_off, order.data(), (size_t)n * 4);
         r->rows = -1;
         if ((e = r->staging.send(r->d_plan, ints * 4, ctx->stream)) != cudaSuccess) return cuda_fail(e, "upload adapter rows");
         r->rows = n;
         r->top_slot = top;
-        r->items[0] = head.items[0];
-        r->items[1] = head.items[1];
+        r->items = head.items;
         return SATORI_OK;
     });
 }
