@@ -13,8 +13,11 @@
 //
 // Both products run on the tensor cores at FP32 accuracy: x and t are cut into three bf16 parts each (24
 // bits), a weight into as many as it needs to be exact (bf16 1, fp16 2, fp32 3), and the products of parts
-// above 2^-24 of the whole are added in FP32 (3, 5 and 6 MMAs per step).  Bytes bound it: the weights of the
-// slots in use, x, base and out.
+// above 2^-24 of the whole are added in FP32 (3, 5 and 6 MMAs per step).  Beside fp16 weights t, whose rows are
+// at hand, is scaled by a power of two into fp16's range and cut into two fp16 parts (22 bits and more), which
+// meet the weights as they are: 2 MMAs instead of 5 and no conversions.  Bytes bound it: the weights of the
+// slots in use, x, base and out.  B streams through a ring of each warp's own in shared memory, filled by bulk
+// copies a run or more ahead: a run's weights are contiguous, and the loads' latency was what the warps waited for.
 #include "batch.cuh"
 #include "common.cuh"
 #include "paged_internal.h"
@@ -56,6 +59,7 @@ struct AdapterArgs {
     long long ldx, ldbase, ldo;
     int rows, cols, cols32;                    // output rows, columns, columns rounded up to 32
     int wide_x, wide_out;                      // 16-byte accesses are possible
+    unsigned *err;
 };
 
 // ------------------------------------------------------------------------------------------- bf16 parts
@@ -117,10 +121,17 @@ __device__ __forceinline__ void weight_parts(const uint32_t *raw, uint32_t (*par
 
 __device__ __forceinline__ void mma_bf16(float *d, const uint32_t *a, const uint32_t *b)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+__device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, const uint32_t *b)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
 // All products of parts i (of a, three) and j (of b) with i + j <= 2, small ones first.
@@ -136,19 +147,43 @@ __device__ __forceinline__ void mma_parts(float *d, const uint32_t (*a)[4], cons
 
 // ------------------------------------------------------------------------------------------- the kernel
 // RM: ranks at most.
-template <int RM>
+template <int TYPE, int RM>
 struct AdapterSmem {
-    float red[kWarps][16][RM + 4];             // the warps' partial t of a 16-row tile
-    float t[kItemRows][RM + 4];                // the CTA's partial t, read by the whole cluster
-    uint32_t parts[3][kItemRows][RM / 2 + 4];  // t in bf16 parts, pairs of ranks
+    static constexpr int kRun = 32 * RM * Weights<TYPE>::kBytes;   // weights of 32 outputs at the largest rank
+    static constexpr int kRing = kRun * (kRun <= 8192 ? 2 : 1);   // a warp's ring
+    static constexpr int kSlots = 4;
+    // t in parts, as the A fragments of the second product: [16 ranks][part][16 rows][lane].
+    static constexpr int kParts = TYPE == SATORI_F16 ? 2 : 3;
+    uint4 parts[RM / 16][kParts][kItemRows / 16][32];
+    // FP32 t and the rows' scales, where the parts are made by each CTA for itself.
+    float whole[TYPE == SATORI_F16 ? kItemRows : 1][RM + 4], unscale[kItemRows];
+    union {
+        struct {
+            float red[kWarps][16][RM + 4];     // the warps' partial t of a 16-row tile
+            float t[kItemRows][RM + 4];        // the CTA's partial t, read by the whole cluster
+        };
+        alignas(16) uint8_t ring[kWarps][kRing];
+    };
+    uint64_t full[kWarps][kSlots];
     int row[kItemRows];
 };
 
+// Where ranks r .. r + 3 (r a multiple of 4) of item row p lie in the fragments: the step of 16 ranks, and twice
+// the lane plus the row's half.  In a whole run of 32 ranks lane q of a row holds 8 consecutive ones, 4 for
+// each of two steps; in a last run of 16 it holds 4.
+__device__ __forceinline__ void fragment_place(int rank, int p, int r, int &step, int &at)
+{
+    const int run = r / 32, in = r % 32;
+    const bool both = 32 * run + 32 <= rank;
+    step = 2 * run + (both ? in / 4 % 2 : 0);
+    at = 2 * (p % 8 * 4 + (both ? in / 8 : in / 4)) + p / 8 % 2;
+}
+
 template <int TYPE, int RM>
-__global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(const AdapterArgs a)
+__global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113 * 1024 ? 2 : 1) adapter_kernel(const AdapterArgs a)
 {
     typedef Weights<TYPE> W;
-    typedef AdapterSmem<RM> Smem;
+    typedef AdapterSmem<TYPE, RM> Smem;
     // Tiles of 8 ranks taken together: their weights and sums fit the registers beside x.
     constexpr int NT = RM / 8 < (TYPE == SATORI_F32 ? 4 : 8) ? RM / 8 : (TYPE == SATORI_F32 ? 4 : 8);
     constexpr int RAW = W::kBytes * 8 / 4;     // words of 8 weights
@@ -158,6 +193,9 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
     const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
     pdl_launch_dependents();
+    if (tid < kWarps * Smem::kSlots) mbar_init(&sm.full[tid / Smem::kSlots][tid % Smem::kSlots], 1);
+    if (tid == 0) fence_mbar_init();
+    uint32_t parity = 0;                       // bit s: this warp's slot s
     pdl_wait();
     const int *plan = reinterpret_cast<const int *>(a.plan);
     const int items = a.plan->items;
@@ -169,13 +207,15 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
         SlotDesc slot = {};
         if (item.slot >= 0) slot = a.slots[item.slot];
         const int rank = slot.rank16, tiles = (item.rows + 15) / 16;
+        __syncthreads();                       // the item before is done with the rows and the ring
         if (tid < kItemRows) sm.row[tid] = tid < item.rows ? rows[item.row_off + tid] : -1;
         __syncthreads();
         if (rank > 0) {
-            // t = A x, 16 rows and 8 NT ranks at a time.  Each warp takes every (8 * ctas)-th run of 32 columns.  A
-            // lane holds 8 consecutive columns of a row: the MMA's k index is a permutation of the run's columns,
-            // the same for x and A.
-            for (int i = 0; i < tiles; ++i) {
+            // t = A x, 8 NT ranks at a time.  The warps are dealt to the item's tiles of 16 rows (1, 2 or 4 shares),
+            // and those of a tile, over the cluster, take its runs of 32 columns in turn.  A lane holds 8 consecutive
+            // columns of a row: the MMA's k index is a permutation of the run's columns, the same for x and A.
+            const int shares = tiles > 2 ? 4 : tiles, per_tile = kWarps / shares, i = warp % shares;
+            if (i < tiles) {
                 const int row0 = sm.row[i * 16 + g], row1 = sm.row[i * 16 + 8 + g];
                 for (int j0 = 0; j0 * 8 < rank; j0 += NT) {
                     const int nt = min(NT, rank / 8 - j0);
@@ -184,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[j][e] = 0;
-                    for (int k0 = (cta * kWarps + warp) * 32; k0 < a.cols32; k0 += ctas * kWarps * 32) {
+                    for (int k0 = (cta * per_tile + warp / shares) * 32; k0 < a.cols32; k0 += ctas * per_tile * 32) {
                         const int k = k0 + q * 8;
                         uint32_t raw[NT][RAW];
 #pragma unroll
@@ -243,25 +283,23 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
                             *reinterpret_cast<float2 *>(d + 8 * (RM + 4)) = make_float2(acc[j][2], acc[j][3]);
                         }
                 }
-                __syncthreads();
-                for (int e = tid; e < 4 * rank; e += kThreads) {
-                    const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
-                    float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float4 v = *reinterpret_cast<const float4 *>(&sm.red[w][p][r]);
-                        sum.x += v.x;
-                        sum.y += v.y;
-                        sum.z += v.z;
-                        sum.w += v.w;
-                    }
-                    *reinterpret_cast<float4 *>(&sm.t[i * 16 + p][r]) = sum;
+            }
+            __syncthreads();
+            for (int e = tid; e < tiles * 4 * rank; e += kThreads) {
+                const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
+                float4 sum = make_float4(0, 0, 0, 0);
+                for (int w = p / 16; w < kWarps; w += shares) {
+                    const float4 v = *reinterpret_cast<const float4 *>(&sm.red[w][p % 16][r]);
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
                 }
-                __syncthreads();
+                *reinterpret_cast<float4 *>(&sm.t[p][r]) = sum;
             }
             cluster.sync();
-            // The whole t, scaled, in bf16 parts.
-            for (int e = tid; e < tiles * 4 * rank; e += kThreads) {
+            // Each CTA adds its share of t over the cluster, scales it, cuts it into bf16 parts and hands them to all.
+            for (int e = cta * kThreads + tid; e < tiles * 4 * rank; e += ctas * kThreads) {
                 const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
                 float4 sum = make_float4(0, 0, 0, 0);
                 for (int c = 0; c < ctas; ++c) {
@@ -271,21 +309,84 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
                     sum.z += v.z;
                     sum.w += v.w;
                 }
+                sum.x *= slot.scale;
+                sum.y *= slot.scale;
+                sum.z *= slot.scale;
+                sum.w *= slot.scale;
+                if (TYPE == SATORI_F16) {
+                    for (int c = 0; c < ctas; ++c) *reinterpret_cast<float4 *>(cluster.map_shared_rank(&sm.whole[p][r], c)) = sum;
+                    continue;
+                }
                 uint32_t lo[3], hi[3];
-                split<3>(sum.x * slot.scale, sum.y * slot.scale, lo);
-                split<3>(sum.z * slot.scale, sum.w * slot.scale, hi);
+                split<3>(sum.x, sum.y, lo);
+                split<3>(sum.z, sum.w, hi);
+                int step, at;
+                fragment_place(rank, p, r, step, at);
+                for (int c = 0; c < ctas; ++c)
 #pragma unroll
-                for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2 *>(&sm.parts[c][p][r / 2]) = make_uint2(lo[c], hi[c]);
+                    for (int k = 0; k < 3; ++k) {
+                        uint32_t *to = reinterpret_cast<uint32_t *>(cluster.map_shared_rank(&sm.parts[step][k % Smem::kParts][p / 16][at >> 1], c)) + (at & 1);
+                        to[0] = lo[k];
+                        to[2] = hi[k];
+                    }
             }
-            __syncthreads();
+            // From here on nobody reads another CTA's t, whose place the ring takes; and the parts are only written
+            // again after the next item's first synchronisation, which every CTA of the cluster comes to.
+            cluster.sync();
+            if (TYPE == SATORI_F16) {
+                // The power of two that brings a row's largest |t| into [2^14, 2^15), and its parts.
+                for (int p = warp; p < tiles * 16; p += kWarps) {
+                    float top = 0;
+                    for (int r = lane; r < rank; r += 32) top = fmaxf(top, fabsf(sm.whole[p][r]));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                    int exponent = 0;
+                    if (top > 0 && top < INFINITY) frexpf(top, &exponent);
+                    const float scale = ldexpf(1.0f, min(15 - exponent, 126)), back = ldexpf(1.0f, max(exponent - 15, -126));
+                    if (lane == 0) sm.unscale[p] = back;
+                    for (int r = 4 * lane; r < rank; r += 128) {
+                        const float4 v = *reinterpret_cast<const float4 *>(&sm.whole[p][r]);
+                        int step, at;
+                        fragment_place(rank, p, r, step, at);
+                        float2 a0 = make_float2(v.x * scale, v.y * scale), a1 = make_float2(v.z * scale, v.w * scale);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const __half2 h0 = __floats2half2_rn(a0.x, a0.y), h1 = __floats2half2_rn(a1.x, a1.y);
+                            uint32_t *to = reinterpret_cast<uint32_t *>(&sm.parts[step][k][p / 16][at >> 1]) + (at & 1);
+                            to[0] = *reinterpret_cast<const uint32_t *>(&h0);
+                            to[2] = *reinterpret_cast<const uint32_t *>(&h1);
+                            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                            a0 = make_float2(a0.x - f0.x, a0.y - f0.y);
+                            a1 = make_float2(a1.x - f1.x, a1.y - f1.y);
+                        }
+                    }
+                }
+                __syncthreads();
+            }
         }
         // out = base + B t: each warp takes runs of 32 output rows.  Lane (g, q) ends up with 8 consecutive
         // outputs, 8 q .. 8 q + 7, of tile rows g and g + 8: column 2 q + e of the MMA's n-tile j stands for
-        // output 8 q + 2 j + e.  A run's weights stay in registers for all of the item's rows; ranks go 32 at a
-        // time (a lane holds 8 consecutive ones), the last 16 of an odd number of 16s with 4 a lane.
-        constexpr int C32 = RM / 32 < 2 ? 1 : (TYPE == SATORI_F32 ? 1 : 2);        // runs of 32 ranks held at once
-        for (int o0 = (cta * kWarps + warp) * 32; o0 < a.rows; o0 += ctas * kWarps * 32) {
-            const int o = o0 + 8 * q;
+        // output 8 q + 2 j + e.  Ranks go 32 at a time (a lane holds 8 consecutive ones), the last 16 of an odd
+        // number of 16s with 4 a lane.
+        constexpr int C32 = 1;                 // runs of 32 ranks held at once
+        const int run_bytes = 32 * rank * W::kBytes, slots = rank ? min(Smem::kSlots, Smem::kRing / run_bytes) : 1;
+        const int runs = (a.rows + 31) / 32, stride = ctas * kWarps, first = cta * kWarps + warp;
+        auto fetch = [&](int run, int s) {
+            const int bytes = min(32, a.rows - run * 32) * rank * W::kBytes;
+            mbar_expect_tx(&sm.full[warp][s], (uint32_t)bytes);
+            bulk_g2s(&sm.ring[warp][s * run_bytes], slot.b + (long long)run * run_bytes, (uint32_t)bytes, &sm.full[warp][s]);
+        };
+        if (rank > 0 && lane == 0) {
+            // The ring's memory was last touched by ordinary accesses.
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            for (int s = 0; s < slots; ++s)
+                if (first + s * stride < runs) fetch(first + s * stride, s);
+        }
+        int s = 0;
+        for (int run = first; run < runs; run += stride, s = s + 1 == slots ? 0 : s + 1) {
+            const int o0 = run * 32, o = o0 + 8 * q;
+            const uint8_t *weights = &sm.ring[warp][s * run_bytes];
+            bool arrived = rank == 0;
             for (int i = 0; i < tiles; ++i) {
                 float base[2][8], acc[4][4];
 #pragma unroll
@@ -304,69 +405,61 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+                if (!arrived && !mbar_wait_bounded(&sm.full[warp][s], parity >> s & 1u)) atomicOr(a.err, kDevErrTimeout);
                 for (int r0 = 0; r0 < rank; r0 += 32 * C32) {
                     uint32_t raw[C32][4][RAW];
 #pragma unroll
-                    for (int c = 0; c < C32; ++c)
+                        for (int c = 0; c < C32; ++c)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int out = min(o0 + 8 * (g >> 1) + 2 * j + (g & 1), a.rows - 1), r = r0 + 32 * c;
-                            const uint8_t *src = slot.b + ((long long)out * rank + r) * W::kBytes;
-                            if (r + 32 <= rank) {
-                                const uint4 *from = reinterpret_cast<const uint4 *>(src + q * 8 * W::kBytes);
+                            for (int j = 0; j < 4; ++j) {
+                                // (Rows behind the last output hold an earlier run's weights; their sums are not stored.)
+                                const int r = r0 + 32 * c;
+                                const uint8_t *src = weights + ((8 * (g >> 1) + 2 * j + (g & 1)) * rank + r) * W::kBytes;
+                                if (r + 32 <= rank) {
+                                    const uint4 *from = reinterpret_cast<const uint4 *>(src + q * 8 * W::kBytes);
 #pragma unroll
-                                for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[c][j][4 * e]) = __ldg(from + e);
-                            } else if (r < rank) {
-                                const uint2 *from = reinterpret_cast<const uint2 *>(src + q * 4 * W::kBytes);
+                                    for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint4 *>(&raw[c][j][4 * e]) = from[e];
+                                } else if (r < rank) {
+                                    const uint2 *from = reinterpret_cast<const uint2 *>(src + q * 4 * W::kBytes);
 #pragma unroll
-                                for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint2 *>(&raw[c][j][2 * e]) = __ldg(from + e);
-                            }
-                        }
-#pragma unroll
-                    for (int c = 0; c < C32; ++c) {
-                        const int r = r0 + 32 * c;
-                        const bool whole = r + 32 <= rank;
-                        if (r >= rank) continue;
-                        // t of this lane's ranks: 8 of them for two steps, or 4 for one.
-                        uint32_t ta[3][2][4];
-#pragma unroll
-                        for (int p = 0; p < 3; ++p)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t *src = &sm.parts[p][i * 16 + h * 8 + g][r / 2];
-                                if (whole) {
-                                    const uint4 v = *reinterpret_cast<const uint4 *>(src + q * 4);
-                                    ta[p][h][0] = v.x;
-                                    ta[p][h][1] = v.y;
-                                    ta[p][h][2] = v.z;
-                                    ta[p][h][3] = v.w;
-                                } else {
-                                    const uint2 v = *reinterpret_cast<const uint2 *>(src + q * 2);
-                                    ta[p][h][0] = v.x;
-                                    ta[p][h][1] = v.y;
-                                    ta[p][h][2] = ta[p][h][3] = 0;
+                                    for (int e = 0; e < RAW / 4; ++e) *reinterpret_cast<uint2 *>(&raw[c][j][2 * e]) = from[e];
                                 }
                             }
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            if (s == 1 && !whole) continue;
-                            uint32_t frag[3][4];
+                    for (int c = 0; c < C32; ++c)
 #pragma unroll
-                            for (int p = 0; p < 3; ++p) {
-                                frag[p][0] = ta[p][0][2 * s];
-                                frag[p][1] = ta[p][1][2 * s];
-                                frag[p][2] = ta[p][0][2 * s + 1];
-                                frag[p][3] = ta[p][1][2 * s + 1];
-                            }
+                        for (int step = 0; step < 2; ++step) {
+                            const int r = r0 + 32 * c + 16 * step;
+                            if (r >= rank) continue;
+                            uint32_t frag[Smem::kParts][4];
+#pragma unroll
+                            for (int p = 0; p < Smem::kParts; ++p)
+                                *reinterpret_cast<uint4 *>(frag[p]) = sm.parts[r / 16][p][i][lane];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                uint32_t wb[W::kParts][2];
-                                weight_parts<TYPE>(&raw[c][j][s * RAW / 2], wb);
-                                mma_parts<W::kParts>(acc[j], frag, wb);
+                                const uint32_t *words = &raw[c][j][step * RAW / 2];
+                                if (TYPE == SATORI_F16) {
+                                    mma_f16(acc[j], frag[1], words);
+                                    mma_f16(acc[j], frag[0], words);
+                                } else {
+                                    uint32_t wb[W::kParts][2];
+                                    weight_parts<TYPE>(words, wb);
+                                    mma_parts<W::kParts>(acc[j], frag, wb);
+                                }
                             }
                         }
-                    }
                 }
+                if (!arrived) {
+                    parity ^= 1u << s;
+                    arrived = true;
+                }
+                if (TYPE == SATORI_F16 && rank > 0)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float back = sm.unscale[i * 16 + (e >> 1) * 8 + g];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j][e] *= back;
+                    }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = sm.row[i * 16 + h * 8 + g];
@@ -385,8 +478,14 @@ __global__ void __launch_bounds__(kThreads, RM <= 64 ? 2 : 1) adapter_kernel(con
                     }
                 }
             }
+            if (rank > 0) {
+                __syncwarp();                  // the warp has read the slot
+                if (lane == 0 && run + slots * stride < runs) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    fetch(run + slots * stride, s);
+                }
+            }
         }
-        cluster.sync();                        // nobody still reads this CTA's t
     }
 }
 
@@ -418,13 +517,13 @@ template <int TYPE, int RM>
 cudaError_t launch_variant(const AdapterArgs &a, int items, int sm_count, cudaStream_t stream)
 {
     auto kernel = adapter_kernel<TYPE, RM>;
-    const size_t smem = sizeof(AdapterSmem<RM>);
+    const size_t smem = sizeof(AdapterSmem<TYPE, RM>);
     cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    // The smallest cluster that gives the SMs two CTAs each: few items are spread over many SMs, many items
-    // exchange less.
-    int cluster = 1;
-    while (cluster < kMaxCluster && items * cluster < 2 * sm_count) cluster *= 2;
+    // The largest cluster with which all items are resident at once (two CTAs an SM): few items are spread over
+    // many SMs, many items exchange less, and there is no second wave.
+    int cluster = kMaxCluster;
+    while (cluster > 1 && items * cluster > 2 * sm_count) cluster /= 2;
     const int clusters = std::max(1, std::min(items, 8 * sm_count / cluster));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * cluster));
@@ -574,7 +673,7 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
         std::vector<int> order((size_t)n);
         for (int i = 0; i < n; ++i) order[i] = i;
         std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return slots[x] < slots[y]; });
-        // The largest items that still give every SM one (an item's rows share the weights' loads): 64, 32 or 16.
+        // The largest items (their rows share the weights' loads) whose clusters still give the SMs two CTAs each.
         std::vector<RowItem> items;
         for (int most = kItemRows; most >= 16; most /= 2) {
             items.clear();
@@ -584,7 +683,7 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
                 for (int at = i; at < end; at += most) items.push_back({slots[order[i]], at, std::min(most, end - at)});
                 i = end;
             }
-            if ((int)items.size() >= ctx->sm_count) break;
+            if ((int)items.size() * kMaxCluster >= 2 * ctx->sm_count) break;
         }
         DevRows head = {};
         size_t ints = sizeof(DevRows) / 4;
@@ -666,6 +765,7 @@ extern "C" int satori_adapters_apply_device(satori_adapters *s, const satori_ada
     a.cols32 = s->cols32();
     a.wide_x = (uintptr_t)x % 16 == 0 && ldx % 4 == 0;
     a.wide_out = ((uintptr_t)base | (uintptr_t)out) % 16 == 0 && ldbase % 4 == 0 && ldo % 4 == 0;
+    a.err = s->ctx->d_err;
     const int sms = s->ctx->sm_count;
     cudaError_t e;
     switch (s->type) {
@@ -696,3 +796,4 @@ extern "C" int satori_matrix_execute_adapted_device(satori_matrix *m, satori_ada
     int rc = satori_matrix_execute_device(m, dx, dy, r->rows, order);
     return rc ? rc : satori_adapters_apply_device(s, r, dx, 0, dy, 0, dy, 0);
 }
+
