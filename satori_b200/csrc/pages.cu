@@ -20,8 +20,8 @@ using namespace satori;
 namespace {
 
 // Page pairs travel as a kernel parameter (at most 32,764 bytes), so a copy needs no upload that a later
-// call could overwrite.  Two sizes: the launch cost grows with the parameter.
-constexpr int kFewPairs = 56, kManyPairs = 4000;
+// call could overwrite.  Three sizes: the launch's cost on the host grows with the parameter.
+constexpr int kFewPairs = 56, kSomePairs = 480, kManyPairs = 4000;
 template <int N>
 struct PagePairs {
     int from[N], to[N];
@@ -77,8 +77,10 @@ int copy_pages(satori_pages *p)
     for (int i = 0; i < n; i += kManyPairs) {
         const int some = std::min(n - i, kManyPairs);
         const int *pairs = p->copies.data() + 2 * (size_t)i;
-        cudaError_t e = some <= kFewPairs ? launch_copy<kFewPairs>(p, pairs, some, p->ctx->stream)
-                                          : launch_copy<kManyPairs>(p, pairs, some, p->ctx->stream);
+        cudaStream_t stream = p->ctx->stream;
+        cudaError_t e = some <= kFewPairs    ? launch_copy<kFewPairs>(p, pairs, some, stream)
+                        : some <= kSomePairs ? launch_copy<kSomePairs>(p, pairs, some, stream)
+                                             : launch_copy<kManyPairs>(p, pairs, some, stream);
         if (e != cudaSuccess) return cuda_fail(e, "copy pages");
     }
     return SATORI_OK;

@@ -10,6 +10,7 @@ request beside a shared projection).  Device vectors are torch CUDA tensors, or 
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -41,32 +42,66 @@ def _type(dtype) -> int:
     return t
 
 
-def _ints(values, name: str) -> np.ndarray:
-    a = np.asarray(values)
-    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
-        raise _bad(f"{name} must be a list of integers")
-    if a.size and (a.min() < -0x80000000 or a.max() > 0x7FFFFFFF):
-        raise _bad(f"{name} exceeds Int32 limits")
-    return np.ascontiguousarray(a, np.int32)
+_kinds: dict = {}                                             # torch dtype -> satori_type or None
+
+
+def _kind(dtype):
+    try:
+        return _kinds[dtype]
+    except KeyError:
+        kind = _kinds[dtype] = _TORCH_TYPES.get(str(dtype))
+        return kind
+
+
+class _Ints:
+    """Integers as a C int array: `size`, `address`, and what owns the memory."""
+    __slots__ = ("size", "address", "owner")
+
+    def __init__(self, values, name: str):
+        if isinstance(values, (list, tuple, range)):
+            try:
+                self.owner = a = array("i", values)
+            except TypeError:
+                raise _bad(f"{name} must be a list of integers") from None
+            except OverflowError:
+                raise _bad(f"{name} exceeds Int32 limits") from None
+            self.address, self.size = a.buffer_info()
+            return
+        a = np.asarray(values)
+        if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+            raise _bad(f"{name} must be a list of integers")
+        if a.size and (a.min() < -0x80000000 or a.max() > 0x7FFFFFFF):
+            raise _bad(f"{name} exceeds Int32 limits")
+        self.owner = a = np.ascontiguousarray(a, np.int32)
+        self.address, self.size = a.ctypes.data, a.size
+
+
+def _new_ints(n: int) -> tuple:
+    """(array, address) of n integers to be filled in."""
+    a = array("i", bytes(4 * n))
+    return a, a.buffer_info()[0]
 
 
 def _rows(t, rows: int, width: int, name: str, device: int, types) -> tuple:
     """(address, row stride, satori_type) of a device matrix of `rows` rows of `width` values."""
-    kind = _TORCH_TYPES.get(str(t.dtype))
-    if kind not in types:
+    kind = _kind(t.dtype)
+    if kind is None or kind not in types:
         raise _bad(f"{name} has type {t.dtype}")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise _bad(f"{name} is not on device {device}")
-    shape, stride = tuple(t.shape), tuple(t.stride())
-    # Trailing dimensions are one packed row.
-    n, at, packed = 1, len(shape), True
-    while at > 1:
-        at -= 1
-        packed = packed and (shape[at] == 1 or stride[at] == n)
-        n *= shape[at]
-    if not shape or shape[0] != rows or n != width or not packed:
-        raise _bad(f"{name} must be {rows} rows of {width} packed values, got shape {shape} with strides {stride}")
-    ld = stride[0] if rows > 1 else width
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2 and shape[0] == rows and shape[1] == width and stride[1] == 1:
+        ld = stride[0] if rows > 1 else width
+    else:
+        # Trailing dimensions are one packed row.
+        n, at, packed = 1, len(shape), True
+        while at > 1:
+            at -= 1
+            packed = packed and (shape[at] == 1 or stride[at] == n)
+            n *= shape[at]
+        if len(shape) == 0 or shape[0] != rows or n != width or not packed:
+            raise _bad(f"{name} must be {rows} rows of {width} packed values, got shape {tuple(shape)} with strides {stride}")
+        ld = stride[0] if rows > 1 else width
     if ld < width:
         raise _bad(f"{name}: rows overlap (row stride {ld})")
     return t.data_ptr(), ld, kind
@@ -88,7 +123,7 @@ class PagedCache:
         if memory is not None:
             if self.ctx is None:
                 raise _bad("memory without a context")
-            if _TORCH_TYPES.get(str(memory.dtype)) != self.type:
+            if _kind(memory.dtype) != self.type:
                 raise _bad(f"memory has type {memory.dtype}")
             if not memory.is_cuda or memory.device.index != self.ctx.device or not memory.is_contiguous():
                 raise _bad("memory must be a contiguous tensor on the context's device")
@@ -96,6 +131,9 @@ class PagedCache:
                 raise _bad("memory does not match the cache's shape")
             address = memory.data_ptr()
         self.memory = memory
+        self._count = C.c_int()
+        self._count_ref = C.byref(self._count)
+        self._grow_scratch(1024)
         h = _vp()
         check(_lib.lib().satori_pages_create(self.ctx.handle if self.ctx else None, layers, pages, page_tokens, kv_heads,
                                              head_dim, self.type, address, C.byref(h)), "pages_create")
@@ -111,14 +149,14 @@ class PagedCache:
         """Ids of n new empty sequences."""
         if n < 0:
             raise _bad("n must not be negative")
-        ids = np.empty(n, np.int32)
-        check(_lib.lib().satori_pages_new(self.handle, n, ids.ctypes.data), "pages_new")
+        ids, address = _new_ints(n)
+        check(_lib.lib().satori_pages_new(self.handle, n, address), "pages_new")
         return ids.tolist()
 
     def extend(self, seqs, counts) -> None:
         """Room for counts[i] more (unwritten) tokens at the end of each sequence."""
         s, c = self._pair(seqs, counts, "counts")
-        check(_lib.lib().satori_pages_extend(self.handle, s.size, s.ctypes.data, c.ctypes.data), "pages_extend")
+        check(_lib.lib().satori_pages_extend(self.handle, s.size, s.address, c.address), "pages_extend")
 
     def fork(self, parents, positions=None) -> list:
         """New sequences that share the parents' first positions[i] tokens (default: all of them)."""
@@ -130,22 +168,22 @@ class PagedCache:
 
     def _fork(self, parents, positions, share: int) -> list:
         if positions is None:
-            s, at = _ints(parents, "parents"), None
+            s, at = _Ints(parents, "parents"), None
         else:
             s, at = self._pair(parents, positions, "positions")
-        ids = np.empty(s.size, np.int32)
-        check(_lib.lib().satori_pages_fork(self.handle, s.size, s.ctypes.data, at.ctypes.data if at is not None else None,
-                                           share, ids.ctypes.data), "pages_fork")
+        ids, address = _new_ints(s.size)
+        check(_lib.lib().satori_pages_fork(self.handle, s.size, s.address, at.address if at is not None else None, share,
+                                           address), "pages_fork")
         return ids.tolist()
 
     def rewind(self, seqs, positions) -> None:
         """Discards the tokens at and after positions[i]."""
         s, at = self._pair(seqs, positions, "positions")
-        check(_lib.lib().satori_pages_rewind(self.handle, s.size, s.ctypes.data, at.ctypes.data), "pages_rewind")
+        check(_lib.lib().satori_pages_rewind(self.handle, s.size, s.address, at.address), "pages_rewind")
 
     def free(self, seqs) -> None:
-        s = _ints(seqs, "seqs")
-        check(_lib.lib().satori_pages_free(self.handle, s.size, s.ctypes.data), "pages_free")
+        s = _Ints(seqs, "seqs")
+        check(_lib.lib().satori_pages_free(self.handle, s.size, s.address), "pages_free")
 
     def compact(self) -> int:
         """Moves the live pages to the lowest numbers; the number of pages moved."""
@@ -155,14 +193,17 @@ class PagedCache:
 
     def table(self, seq: int) -> np.ndarray:
         """The sequence's page numbers."""
-        length, count = C.c_int(), C.c_int()
-        L, h = _lib.lib(), self.handle
-        pages = np.empty(64, np.int32)
-        check(L.satori_pages_table(h, seq, C.byref(length), pages.ctypes.data, pages.size, C.byref(count)), "pages_table")
-        if count.value > pages.size:
-            pages = np.empty(count.value, np.int32)
-            check(L.satori_pages_table(h, seq, None, pages.ctypes.data, pages.size, None), "pages_table")
-        return pages[:count.value]
+        check(_lib.lib().satori_pages_table(self.handle, seq, None, self._scratch_at, self._scratch_size, self._count_ref),
+              "pages_table")
+        n = self._count.value
+        if n > self._scratch_size:
+            self._grow_scratch(2 * n)
+            return self.table(seq)
+        return self._scratch[:n].copy()
+
+    def _grow_scratch(self, n: int) -> None:
+        self._scratch = np.empty(n, np.int32)
+        self._scratch_at, self._scratch_size = self._scratch.ctypes.data, n
 
     def length(self, seq: int) -> int:
         """The sequence's tokens."""
@@ -187,7 +228,7 @@ class PagedCache:
 
     @staticmethod
     def _pair(seqs, values, name: str) -> tuple:
-        s, v = _ints(seqs, "seqs"), _ints(values, name)
+        s, v = _Ints(seqs, "seqs"), _Ints(values, name)
         if s.size != v.size:
             raise _bad(f"{s.size} sequences, {v.size} {name}")
         return s, v
@@ -233,8 +274,8 @@ class DecodeBatch:
     def step(self, seqs, counts) -> None:
         """Extends each sequence by counts[i] new tokens; the step's rows are these tokens in order."""
         s, c = PagedCache._pair(seqs, counts, "counts")
-        check(_lib.lib().satori_batch_step(self.handle, s.size, s.ctypes.data, c.ctypes.data), "batch_step")
-        self.rows = int(c.sum())
+        check(_lib.lib().satori_batch_step(self.handle, s.size, s.address, c.address), "batch_step")
+        self.rows = int(sum(c.owner))
 
     def append_device(self, layer: int, k, v, q=None, q_out=None) -> None:
         """k and v (rows x kv_heads * head_dim; k is rotated) into the layer's pages; q rotated into q_out.
@@ -309,8 +350,8 @@ class AdapterRows:
         return self._h
 
     def assign(self, slots) -> None:
-        s = _ints(slots, "slots")
-        check(_lib.lib().satori_adapter_rows_assign(self.handle, s.size, s.ctypes.data), "adapter_rows_assign")
+        s = _Ints(slots, "slots")
+        check(_lib.lib().satori_adapter_rows_assign(self.handle, s.size, s.address), "adapter_rows_assign")
         self.rows = s.size
 
     def dispose(self) -> None:
@@ -375,7 +416,7 @@ class AdapterSet:
                 raise _bad(f"{name} has type {w.dtype}")
             w = np.ascontiguousarray(w)
             return w.ctypes.data, w.shape[1], w
-        if _TORCH_TYPES.get(str(w.dtype)) != self.type:
+        if _kind(w.dtype) != self.type:
             raise _bad(f"{name} has type {w.dtype}")
         if w.is_cuda and w.device.index != self.ctx.device:
             raise _bad(f"{name} is not on device {self.ctx.device}")
