@@ -385,10 +385,11 @@ cudaError_t grow(satori_batch *b, P *&buffer, size_t &have, size_t need, size_t 
 }
 
 bool on_tensor_cores(const satori_batch *b) { return tensor_attention_takes(b->pages->type, b->pages->head_dim); }
+bool on_f32_tiles(const satori_batch *b) { return f32_attention_takes(b->pages->type, b->pages->head_dim); }
 
 size_t record_rows(const satori_batch *b)
 {
-    return (size_t)(on_tensor_cores(b) ? tensor_record_rows() : generic_record_rows());
+    return (size_t)(on_tensor_cores(b) ? tensor_record_rows() : on_f32_tiles(b) ? f32_record_rows() : generic_record_rows());
 }
 
 int upload_plan(satori_batch *b)
@@ -511,6 +512,8 @@ extern "C" int satori_batch_create(satori_pages *pages, int q_heads, double rope
         const int sms = pages->ctx ? pages->ctx->sm_count : 148;
         if (on_tensor_cores(b))
             tensor_plan_shape(sms, b->shape);
+        else if (on_f32_tiles(b))
+            f32_plan_shape(pages->head_dim, sms, b->shape);
         else
             generic_plan_shape(pages->type, pages->head_dim, sms, b->shape);
         ++pages->users;
@@ -665,9 +668,10 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
     a.scale_log2 = (float)(1.4426950408889634 / sqrt((double)p->head_dim));
     a.ctas = b->shape.ctas;
     a.err = p->ctx->d_err;
-    cudaError_t e = on_tensor_cores(b)
-                        ? launch_tensor_attention(a, p->map, layer * p->tables.pages() * 2 * p->kv_heads, p->ctx->stream)
-                        : launch_generic_attention(a, p->ctx->stream);
+    const int layer_block = layer * p->tables.pages() * 2 * p->kv_heads;
+    cudaError_t e = on_tensor_cores(b) ? launch_tensor_attention(a, p->map, layer_block, p->ctx->stream)
+                    : on_f32_tiles(b)  ? launch_f32_attention(a, p->map, layer_block, p->ctx->stream)
+                                       : launch_generic_attention(a, p->ctx->stream);
     if (e == cudaSuccess)
         e = launch_combine(a, (int)rows, b->shape.tile_m, on_tensor_cores(b), b->plan.head.merges,
                            p->ctx->sm_count, p->ctx->stream);

@@ -55,6 +55,12 @@ int tensor_record_rows();
 cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim, int page_tokens, unsigned long long blocks);
 cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
 
+// The FP32 kernel of heads of 32, 64, 96 and 128.
+bool f32_attention_takes(int type, int head_dim);
+void f32_plan_shape(int head_dim, int sm_count, PlanShape &shape);
+int f32_record_rows();
+cudaError_t launch_f32_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
+
 // Merges the partial records of every row that has more than one source and writes its outputs.
 // A record holds record_rows rows; by_column: as [head_dim / 4][row] groups of 4 values, otherwise [row][head_dim].
 // `merges` (the plan's) chooses the launch's shape; any number is worked through.

@@ -1,6 +1,5 @@
-// batch_attn_generic.cu -- attention of a batch over a paged cache on the FP32 units: FP32 caches (whose
-// products the tensor cores would round), and the head sizes of 16-bit caches that the tensor-core kernel
-// does not take.
+// batch_attn_generic.cu -- attention of a batch over a paged cache on the FP32 units, for the head sizes that
+// neither the tensor-core kernel (16-bit caches, 64 and 128) nor the FP32 one (multiples of 32 up to 128) takes.
 //
 // For a query row r and its visible keys t: out_r = sum_t p_rt v_t / sum_t p_rt, p_rt = 2^(s_rt - m_r),
 // s_rt = (q_r . k_t) log2(e) / sqrt(d), m_r the running maximum.  One pass over the keys; the running

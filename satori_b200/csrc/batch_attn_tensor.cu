@@ -818,20 +818,23 @@ cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim
     cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
     if (e != cudaSuccess) return e;
     if (found != cudaDriverEntryPointSuccess || !f) return cudaErrorNotSupported;
-    const CUtensorMapDataType kind = type == SATORI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const cuuint64_t row = (cuuint64_t)head_dim * 2, block = row * page_tokens;
+    const CUtensorMapDataType kind = type == SATORI_F16   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : type == SATORI_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint32_t size = type == SATORI_F32 ? 4 : 2, columns = 128 / size;      // columns of a 128-byte tile row
+    const cuuint64_t row = (cuuint64_t)head_dim * size, block = row * page_tokens;
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     CUresult r;
-    if (page_tokens >= kBlockKeys) {       // [block][half][token][64]: a box is a block of keys, half by half
-        const cuuint64_t dims[4] = {64, (cuuint64_t)page_tokens, (cuuint64_t)head_dim / 64, (cuuint64_t)blocks};
+    if (page_tokens >= kBlockKeys) {       // [block][part][token][columns]: a box is a block of keys, part by part
+        const cuuint64_t dims[4] = {columns, (cuuint64_t)page_tokens, (cuuint64_t)head_dim / columns, (cuuint64_t)blocks};
         const cuuint64_t strides[3] = {row, 128, block};
-        const cuuint32_t box[4] = {64, kBlockKeys, (cuuint32_t)head_dim / 64, 1};
+        const cuuint32_t box[4] = {columns, kBlockKeys, (cuuint32_t)head_dim / columns, 1};
         r = reinterpret_cast<EncodeTiled>(f)(map, kind, 4, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    } else {                               // [block][token][dim]: a box is one half of a page
+    } else {                               // [block][token][dim]: a box is 128 bytes of a page's rows
         const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)page_tokens, (cuuint64_t)blocks}, strides[2] = {row, block};
-        const cuuint32_t box[3] = {64, (cuuint32_t)page_tokens, 1};
+        const cuuint32_t box[3] = {columns, (cuuint32_t)page_tokens, 1};
         r = reinterpret_cast<EncodeTiled>(f)(map, kind, 3, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -229,7 +229,7 @@ extern "C" int satori_pages_create(satori_ctx *ctx, int layers, int pages, int p
             }
             p->owned = true;
         }
-        if (ctx && tensor_attention_takes(type, head_dim)) {
+        if (ctx && (tensor_attention_takes(type, head_dim) || f32_attention_takes(type, head_dim))) {
             DeviceScope scope(ctx->device);
             cudaError_t e = make_page_map(&p->map, p->memory, type, head_dim, page_tokens,
                                           (unsigned long long)layers * pages * 2 * kv_heads);
