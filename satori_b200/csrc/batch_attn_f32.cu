@@ -6,17 +6,18 @@
 // arithmetic of this one.  One CTA per SM works through its share of the plan's items; warp 8's elected thread
 // loads each block of 64 keys as a K and a V tile (TMA, 32 columns of 128 bytes a row with the 128-byte swizzle:
 // 8 threads that read 16 bytes of 8 consecutive rows, or of one row, meet 8 different bank groups), warps 0-7
-// compute:
-//  * tiles of at most 8 rows (the query heads of one KV head of one request): for the scores a lane owns a key
-//    and its warp two rows, so that a dot product needs no exchange; for the outputs a warp owns 8 keys, with a
-//    running maximum of its own.  HBM bounds it (64 KB a block of 128-wide heads against about 1000 issue slots).
-//  * tiles of up to 64 rows (a shared prefix, a prompt): 4 x 4 scores and 4 x HD / 16 outputs per thread.  The
-//    FP32 units bound it: 8192 clocks a block at 128 columns.
-// Products are packed two to an instruction (FFMA2), which halves the issue slots, not the arithmetic.
-//
-// Measured, 32 heads of 128 over 8 KV heads, against the kernel for other caches on the same call: one request of
-// 300 tokens 11.1 us (20 us there, where each warp waits for its own loads), 16 requests that share 8192 tokens
-// 51 us (55 us there), of which the FP32 units are busy about 30 us.
+// compute.  By the rows of the item's tile:
+//  * at most 8 rows (the query heads of one KV head of one request): each warp takes 8 keys of every block on its
+//    own, with a running maximum of its own and no barrier among warps.  A lane holds 4 columns of the queries
+//    and of the outputs; the 64 partial dot products meet in a halving exchange (62 shuffles) that leaves each
+//    lane one key and two rows.  HBM bounds it: 64 KB a block of 128-wide heads are 2800 clocks, its
+//    instructions about 1700.
+//  * up to 64, 96 or 128 rows (a shared prefix, a prompt): 4, 6 or 8 rows x 4 scores and x HD / 16 outputs per
+//    thread.  A 16-byte read of shared memory takes a warp 4 clocks, or 2 where each half of it reads one address
+//    (the queries, the weights), a packed product 2 clocks of one of four units: with 8 rows the products take
+//    longer than the reads (256 : 256 clocks for 4 columns of the scores, 512 : 384 for 4 keys of the outputs),
+//    with 4 rows the reads take longer, for half the work (192 : 128, 320 : 256).
+// Products are packed two to an instruction, which halves the issue slots, not the arithmetic.
 #include "batch.cuh"
 #include "common.cuh"
 
@@ -26,26 +27,26 @@ namespace satori {
 
 namespace {
 
-constexpr int kWarps = 8, kCompute = kWarps * 32, kThreads = kCompute + 32;
-constexpr int kTileM = 64, kBlock = 64, kFewRows = 8;
+constexpr int kWarps = 8, kCompute = kWarps * 32, kThreads = kCompute + 128;
+constexpr int kTileM = 128, kBlock = 64, kFewRows = 8;
+// The 65536 registers: 168 a thread at the launch, of which the loader's four warps hand most to the others.
+constexpr int kLoaderRegs = 40, kComputeRegs = 232;
+static_assert(128 * kLoaderRegs + kCompute * kComputeRegs <= kThreads * 168, "registers");
 
 template <int HD>
 struct Layout {
     static constexpr int kSub = kBlock * 128;                      // 64 rows of 32 columns
     static constexpr int kTile = kSub * (HD / 32);
-    static constexpr int kStages = HD <= 64 ? 8 : HD <= 96 ? 6 : 5;
+    static constexpr int kStages = HD <= 64 ? 8 : HD <= 96 ? 6 : 4;
 };
 
 template <int HD>
 struct alignas(1024) Smem {
     uint8_t stages[Layout<HD>::kStages][Layout<HD>::kTile];
-    float q[kTileM][HD + 4];
+    float q[kTileM * HD];                              // see q_chunk
     union {
-        float p[kTileM][kBlock + 4];
-        struct {
-            float s[2][kBlock][kFewRows];              // scores of a block, two buffers
-            float w[kWarps][kFewRows + 1][kFewRows];   // a warp's weights [key][row], then the rows' factors
-        } few;
+        float p[kTileM * kBlock];                      // weights, see p_at
+        float few[kWarps][kFewRows + 1][kFewRows];     // a warp's weights [key][row], then the rows' factors
     };
     float few_m[kWarps][kFewRows], few_l[kWarps][kFewRows];
     uint64_t full[Layout<HD>::kStages], empty[Layout<HD>::kStages];
@@ -102,6 +103,13 @@ __device__ __forceinline__ float4 tile_chunk(const uint8_t *tile, int key, int c
 {
     return *reinterpret_cast<const float4 *>(tile + (c >> 3) * (kBlock * 128) + key * 128 + (((c ^ key) & 7) << 4));
 }
+
+// Rows of the queries and of the weights change their order by RI rows, so that the two rows that a warp reads
+// (RI apart) lie in different banks without padding.
+template <int HD, int RI>
+__device__ __forceinline__ int q_chunk(int row, int c) { return row * HD + (c ^ ((row / RI) & 1)) * 4; }
+template <int RI>
+__device__ __forceinline__ int p_at(int row, int key) { return row * kBlock + (key ^ (((row / RI) & 1) << 4)); }
 
 __device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
@@ -166,7 +174,7 @@ __device__ __forceinline__ void store_out(const BatchAttn &a, int row, int head,
 }
 
 // Rows' indices and limits, and their queries times log2(e) / sqrt(d).
-template <int HD>
+template <int HD, int RI>
 __device__ __forceinline__ void load_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item, Smem<HD> &sm, int rows)
 {
     const int tid = threadIdx.x;
@@ -180,9 +188,18 @@ __device__ __forceinline__ void load_rows(const BatchAttn &a, const DevPlan *pla
         sm.limit[tid] = !live ? 0 : item.start >= 0 ? own.y + 1 - item.start : item.keys;
     }
     compute_sync();
-    for (int i = tid; i < rows * HD; i += kCompute) {
-        const int r = i / HD, d = i % HD;
-        sm.q[r][d] = r < item.m ? reinterpret_cast<const float *>(a.q)[(long long)sm.row[r] * a.ldq + sm.head[r] * HD + d] * a.scale_log2 : 0.0f;
+    const float *q = reinterpret_cast<const float *>(a.q);
+    const bool aligned = !((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(a.ldq * 4)) & 15);
+#pragma unroll 8
+    for (int i = tid; i < rows * (HD / 4); i += kCompute) {
+        const int r = i / (HD / 4), c = i % (HD / 4);
+        float4 v = make_float4(0, 0, 0, 0);
+        if (r < item.m) {
+            const float *from = q + (long long)sm.row[r] * a.ldq + sm.head[r] * HD + c * 4;
+            v = aligned ? *reinterpret_cast<const float4 *>(from) : make_float4(from[0], from[1], from[2], from[3]);
+        }
+        const float f = a.scale_log2;
+        *reinterpret_cast<float4 *>(&sm.q[q_chunk<HD, RI>(r, c)]) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
     }
     compute_sync();
 }
@@ -191,99 +208,140 @@ template <int HD, typename Wait>
 __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item, Smem<HD> &sm, Ring<HD> &ring, Wait &wait)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    load_rows<HD>(a, plan, item, sm, kFewRows);
-    const int half = warp & 1, r0 = warp & ~1;         // scores: this warp's 32 keys and rows r0, r0 + 1
-    const bool scores = r0 < item.m;
-    const int row8 = lane & 7, least = sm.limit[0];
-    const int own_limit = sm.limit[row8];
-    const bool works = lane * 4 < HD;
-    float m = -INFINITY, l = 0;                        // row row8 over this warp's keys (four lanes alike)
+    load_rows<HD, kTileM>(a, plan, item, sm, kFewRows);
+    const bool works = lane * 4 < HD;                  // this lane's 4 columns exist
+    const int chunk = works ? lane : 0, k0 = warp * 8;
+    // After the exchange: this lane's key of the warp's 8, and its two rows.
+    const int own_key = k0 + (lane >> 2), row0 = (lane & 3) * 2;
+    const int limit0 = sm.limit[row0], limit1 = sm.limit[row0 + 1], least = sm.limit[0];
+    float4 q[kFewRows];
     float2 acc[kFewRows][2];
 #pragma unroll
-    for (int r = 0; r < kFewRows; ++r) acc[r][0] = acc[r][1] = make_float2(0, 0);
+    for (int r = 0; r < kFewRows; ++r) {
+        q[r] = works ? *reinterpret_cast<const float4 *>(&sm.q[q_chunk<HD, kTileM>(r, lane)]) : make_float4(0, 0, 0, 0);
+        acc[r][0] = acc[r][1] = make_float2(0, 0);
+    }
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0, l1 = 0;
+    float (&w)[kFewRows + 1][kFewRows] = sm.few[warp];
     for (int j = 0; j < item.blocks; ++j) {
-        const int t0 = (item.block0 + j) * kBlock, buffer = j & 1;
+        const int t0 = (item.block0 + j) * kBlock;
         // ---- scores
         wait(&sm.full[ring.stage], ring.parity);
-        if (scores) {
-            const int key = half * 32 + lane;
-            const uint8_t *tile = sm.stages[ring.stage];
-            float2 s0 = make_float2(0, 0), s1 = s0, u0 = s0, u1 = s0;
-#pragma unroll 8
-            for (int c = 0; c < HD / 4; ++c) {
-                const float4 k = tile_chunk(tile, key, c);
-                const float4 qa = *reinterpret_cast<const float4 *>(&sm.q[r0][c * 4]);
-                const float4 qb = *reinterpret_cast<const float4 *>(&sm.q[r0 + 1][c * 4]);
-                s0 = __ffma2_rn(lo2(qa), lo2(k), s0);
-                u0 = __ffma2_rn(hi2(qa), hi2(k), u0);
-                s1 = __ffma2_rn(lo2(qb), lo2(k), s1);
-                u1 = __ffma2_rn(hi2(qb), hi2(k), u1);
+        const uint8_t *tile = sm.stages[ring.stage];
+        float s[2];
+        {
+            const bool upper = lane & 16, mid = lane & 8, low = lane & 4, row_hi = lane & 2, row_lo = lane & 1;
+            auto dots = [&](int key, float (&d)[kFewRows]) {
+                const float4 k = tile_chunk(tile, k0 + key, chunk);
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r) {
+                    const float2 t = __ffma2_rn(hi2(q[r]), hi2(k), __fmul2_rn(lo2(q[r]), lo2(k)));
+                    d[r] = t.x + t.y;
+                }
+            };
+            // The lanes with `mine` set keep b of (a, b), the others a, each summed with its partner's.
+            auto meet = [&](bool mine, int mask, float a, float b) {
+                return (mine ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, mine ? a : b, mask);
+            };
+            float quarter[2][kFewRows];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {              // key bit 0
+                float half[2][kFewRows];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {          // key bit 1
+                    float a[kFewRows], b[kFewRows];
+                    dots(e + 2 * g, a);
+                    dots(e + 2 * g + 4, b);
+#pragma unroll
+                    for (int r = 0; r < kFewRows; ++r) half[g][r] = meet(upper, 16, a[r], b[r]);
+                }
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r) quarter[e][r] = meet(mid, 8, half[0][r], half[1][r]);
             }
-            const float2 a0 = __fadd2_rn(s0, u0), a1 = __fadd2_rn(s1, u1);
-            *reinterpret_cast<float2 *>(&sm.few.s[buffer][key][r0]) = make_float2(a0.x + a0.y, a1.x + a1.y);
+            float rows[kFewRows], four[4];
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) rows[r] = meet(low, 4, quarter[0][r], quarter[1][r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) four[r] = meet(row_hi, 2, rows[r], rows[r + 4]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) s[r] = meet(row_lo, 1, four[r], four[r + 2]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[ring.stage]);
         ring.next();
-        compute_sync();
-        // ---- weights of this warp's 8 keys: lane (key & 3, row)
-        const int k0 = warp * 8, ka = k0 + (lane >> 3);
-        float sa = row8 < item.m && t0 + ka < own_limit ? sm.few.s[buffer][ka][row8] : -INFINITY;
-        float sb = row8 < item.m && t0 + ka + 4 < own_limit ? sm.few.s[buffer][ka + 4][row8] : -INFINITY;
-        float top = fmaxf(sa, sb);
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-        top = fmaxf(top, m);
-        const float base = top == -INFINITY ? 0.0f : top;
-        const float keep = exp2f(m - base), pa = exp2f(sa - base), pb = exp2f(sb - base);
-        m = top;
-        l = fmaf(l, keep, pa + pb);                    // this lane's keys only; the four lanes are added at the end
-        sm.few.w[warp][lane >> 3][row8] = pa;
-        sm.few.w[warp][(lane >> 3) + 4][row8] = pb;
-        if (lane < 8) sm.few.w[warp][8][lane] = keep;
-        __syncwarp();
-        {
-            const float4 ka4 = *reinterpret_cast<const float4 *>(&sm.few.w[warp][8][0]);
-            const float4 kb4 = *reinterpret_cast<const float4 *>(&sm.few.w[warp][8][4]);
-            const float f[8] = {ka4.x, ka4.y, ka4.z, ka4.w, kb4.x, kb4.y, kb4.z, kb4.w};
+        // ---- weights
+        const float s0 = t0 + own_key < limit0 ? s[0] : -INFINITY, s1 = t0 + own_key < limit1 ? s[1] : -INFINITY;
+        float top0 = s0, top1 = s1;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            top0 = fmaxf(top0, __shfl_xor_sync(0xFFFFFFFFu, top0, o));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xFFFFFFFFu, top1, o));
+        }
+        top0 = fmaxf(top0, m0);
+        top1 = fmaxf(top1, m1);
+        const bool grown = top0 > m0 || top1 > m1;
+        const float base0 = top0 == -INFINITY ? 0.0f : top0, base1 = top1 == -INFINITY ? 0.0f : top1;
+        const float p0 = exp2f(s0 - base0), p1 = exp2f(s1 - base1);
+        *reinterpret_cast<float2 *>(&w[lane >> 2][row0]) = make_float2(p0, p1);
+        if (__any_sync(0xFFFFFFFFu, grown)) {
+            const float keep0 = exp2f(m0 - base0), keep1 = exp2f(m1 - base1);
+            l0 *= keep0;
+            l1 *= keep1;
+            if (lane < 4) *reinterpret_cast<float2 *>(&w[kFewRows][row0]) = make_float2(keep0, keep1);
+            __syncwarp();
+            const float4 fa = *reinterpret_cast<const float4 *>(&w[kFewRows][0]), fb = *reinterpret_cast<const float4 *>(&w[kFewRows][4]);
+            const float f[kFewRows] = {fa.x, fa.y, fa.z, fa.w, fb.x, fb.y, fb.z, fb.w};
 #pragma unroll
             for (int r = 0; r < kFewRows; ++r) {
                 acc[r][0] = __fmul2_rn(acc[r][0], both(f[r]));
                 acc[r][1] = __fmul2_rn(acc[r][1], both(f[r]));
             }
         }
-        // ---- outputs: lane owns 4 columns
+        m0 = top0;
+        m1 = top1;
+        l0 += p0;                                      // this lane's keys only; the lanes are added at the end
+        l1 += p1;
+        __syncwarp();
+        // ---- outputs
         wait(&sm.full[ring.stage], ring.parity);
-        const uint8_t *tile = sm.stages[ring.stage];
-        const bool masked = t0 + k0 + 8 > least;       // some row does not see some of these keys
-        const int have = item.keys - t0;               // (the tile's rows from there on hold anything)
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-            if (k0 + kk >= have) break;
-            const float4 v = works ? tile_chunk(tile, k0 + kk, lane) : make_float4(0, 0, 0, 0);
-            const float4 wa = *reinterpret_cast<const float4 *>(&sm.few.w[warp][kk][0]);
-            const float4 wb = *reinterpret_cast<const float4 *>(&sm.few.w[warp][kk][4]);
-            const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+        tile = sm.stages[ring.stage];
+        // Rows that do not see a key skip it, whatever V holds there (the tile's rows behind the segment's keys
+        // hold anything).
+        const bool masked = t0 + k0 + 8 > least || t0 + k0 + 8 > item.keys;
+        auto add = [&](int key, auto seen) {
+            const float4 v = tile_chunk(tile, k0 + key, chunk);
+            const float4 wa = *reinterpret_cast<const float4 *>(&w[key][0]), wb = *reinterpret_cast<const float4 *>(&w[key][4]);
+            const float f[kFewRows] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
             for (int r = 0; r < kFewRows; ++r) {
-                if (masked && t0 + k0 + kk >= sm.limit[r]) continue;           // whatever V holds there
-                acc[r][0] = __ffma2_rn(both(w[r]), lo2(v), acc[r][0]);
-                acc[r][1] = __ffma2_rn(both(w[r]), hi2(v), acc[r][1]);
+                if (!seen(r)) continue;
+                acc[r][0] = __ffma2_rn(both(f[r]), lo2(v), acc[r][0]);
+                acc[r][1] = __ffma2_rn(both(f[r]), hi2(v), acc[r][1]);
             }
+        };
+        if (!masked) {
+#pragma unroll
+            for (int key = 0; key < 8; ++key) add(key, [](int) { return true; });
+        } else {
+#pragma unroll 1
+            for (int key = 0; key < min(8, item.keys - t0 - k0); ++key)
+                add(key, [&](int r) { return t0 + k0 + key < sm.limit[r]; });
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[ring.stage]);
         ring.next();
     }
-    // Merge the warps: their accumulators lie behind the 8 query rows, over the scores.
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
-    compute_sync();
-    float *merged = &sm.q[kFewRows][0];                // [warp][row][HD]
-    static_assert(sizeof(float) * kWarps * kFewRows * HD <= sizeof(float) * (kTileM - kFewRows) * (HD + 4) + sizeof(float) * kTileM * (kBlock + 4), "room");
-    if (lane < 8) {
-        sm.few_m[warp][lane] = m;
-        sm.few_l[warp][lane] = l;
+    // Merge the warps: their accumulators lie behind the 8 query rows.
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, o);
+        l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, o);
+    }
+    float *merged = &sm.q[kFewRows * HD];              // [warp][row][HD]
+    static_assert(kWarps * kFewRows <= kTileM - kFewRows, "room");
+    if (lane < 4) {
+        *reinterpret_cast<float2 *>(&sm.few_m[warp][row0]) = make_float2(m0, m1);
+        *reinterpret_cast<float2 *>(&sm.few_l[warp][row0]) = make_float2(l0, l1);
     }
     if (works)
 #pragma unroll
@@ -316,18 +374,18 @@ __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem
     compute_sync();
 }
 
-template <int HD, typename Wait>
+template <int HD, int RI, typename Wait>
 __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item, Smem<HD> &sm, Ring<HD> &ring, Wait &wait)
 {
     constexpr int OC = (HD + 63) / 64;                 // groups of 4 output columns per thread
     const int tid = threadIdx.x, lane = tid & 31, tx = tid & 15, ty = tid >> 4;
-    load_rows<HD>(a, plan, item, sm, kTileM);
-    float m[4], l[4];
-    float2 acc[4][OC][2];
-    int limit[4];
+    load_rows<HD, RI>(a, plan, item, sm, RI * 16);
+    float m[RI], l[RI];
+    float2 acc[RI][OC][2];
+    int limit[RI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        limit[i] = sm.limit[ty * 4 + i];
+    for (int i = 0; i < RI; ++i) {
+        limit[i] = sm.limit[ty * RI + i];
         m[i] = -INFINITY;
         l[i] = 0;
 #pragma unroll
@@ -338,31 +396,31 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
         const int t0 = block * kBlock;
         wait(&sm.full[ring.stage], ring.parity);
         const uint8_t *tile = sm.stages[ring.stage];
-        float2 s2[4][4];
+        float2 s2[RI][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < RI; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0, 0);
 #pragma unroll 4
         for (int c = 0; c < HD / 4; ++c) {
-            float4 q[4], k[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * 4 + i][c * 4]);
+            float4 k[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) k[j] = tile_chunk(tile, tx + 16 * j, c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RI; ++i) {
+                const float4 q = *reinterpret_cast<const float4 *>(&sm.q[q_chunk<HD, RI>(ty * RI + i, c)]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s2[i][j] = __ffma2_rn(lo2(q[i]), lo2(k[j]), s2[i][j]);
-                    s2[i][j] = __ffma2_rn(hi2(q[i]), hi2(k[j]), s2[i][j]);
+                    s2[i][j] = __ffma2_rn(lo2(q), lo2(k[j]), s2[i][j]);
+                    s2[i][j] = __ffma2_rn(hi2(q), hi2(k[j]), s2[i][j]);
                 }
+            }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[ring.stage]);
         ring.next();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RI; ++i) {
             float s[4], top = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -378,7 +436,7 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
             for (int j = 0; j < 4; ++j) {
                 const float p = exp2f(s[j] - base);
                 sum += p;
-                sm.p[ty * 4 + i][tx + 16 * j] = p;
+                sm.p[p_at<RI>(ty * RI + i, tx + 16 * j)] = p;
             }
             l[i] = fmaf(l[i], keep, sum);              // this thread's keys only
 #pragma unroll
@@ -387,31 +445,45 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
                 acc[i][c][1] = __fmul2_rn(acc[i][c][1], both(keep));
             }
         }
-        __syncwarp();                                  // a warp's 8 rows of weights are its own
+        __syncwarp();                                  // a warp's rows of weights are its own
         wait(&sm.full[ring.stage], ring.parity);
         tile = sm.stages[ring.stage];
-        const bool masked = t0 + kBlock > least;       // some row does not see some key of the block
-        const int have = min(kBlock, item.keys - t0);  // (the tile's rows from there on hold anything)
-#pragma unroll 2
-        for (int t = 0; t < have; t += 4) {
-            float4 p[4];
+        // Rows that do not see a key skip it, whatever V holds there (the tile's rows behind the segment's keys
+        // hold anything).
+        auto add = [&](int key, const float (&w)[RI], auto seen) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4 *>(&sm.p[ty * 4 + i][t]);
+            for (int c = 0; c < OC; ++c) {
+                if (HD % 64 && c * 16 + tx >= HD / 4) continue;
+                const float4 v = tile_chunk(tile, key, c * 16 + tx);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (t + u >= have) break;
-#pragma unroll
-                for (int c = 0; c < OC; ++c) {
-                    if (HD % 64 && c * 16 + tx >= HD / 4) continue;
-                    const float4 v = tile_chunk(tile, t + u, c * 16 + tx);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-                        if (masked && t0 + t + u >= limit[i]) continue;        // whatever V holds there
-                        acc[i][c][0] = __ffma2_rn(both(w), lo2(v), acc[i][c][0]);
-                        acc[i][c][1] = __ffma2_rn(both(w), hi2(v), acc[i][c][1]);
-                    }
+                for (int i = 0; i < RI; ++i) {
+                    if (!seen(i)) continue;
+                    acc[i][c][0] = __ffma2_rn(both(w[i]), lo2(v), acc[i][c][0]);
+                    acc[i][c][1] = __ffma2_rn(both(w[i]), hi2(v), acc[i][c][1]);
                 }
+            }
+        };
+        if (t0 + kBlock <= least && t0 + kBlock <= item.keys) {
+#pragma unroll 2
+            for (int t = 0; t < kBlock; t += 4) {
+                float4 p[RI];
+#pragma unroll
+                for (int i = 0; i < RI; ++i) p[i] = *reinterpret_cast<const float4 *>(&sm.p[p_at<RI>(ty * RI + i, t)]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float w[RI];
+#pragma unroll
+                    for (int i = 0; i < RI; ++i) w[i] = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+                    add(t + u, w, [](int) { return true; });
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < min(kBlock, item.keys - t0); ++t) {
+                float w[RI];
+#pragma unroll
+                for (int i = 0; i < RI; ++i) w[i] = sm.p[p_at<RI>(ty * RI + i, t)];
+                add(t, w, [&](int i) { return t0 + t < limit[i]; });
             }
         }
         __syncwarp();
@@ -419,10 +491,10 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
         ring.next();
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RI; ++i) {
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], o);
-        const int r = ty * 4 + i;
+        const int r = ty * RI + i;
         if (r < item.m) {
             const float inverse = 1.0f / l[i];
 #pragma unroll
@@ -480,8 +552,9 @@ __global__ void __launch_bounds__(kThreads, 1) f32_attention_kernel(const Args t
         return false;
     };
     Ring<HD> ring;
-    if (warp == kWarps) {
-        if (elect_one()) {
+    if (warp >= kWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
+        if (warp == kWarps && elect_one()) {
             int units = 0;
             bool ok = true;
             for (int i = first; i < last && ok; ++i) {
@@ -498,12 +571,17 @@ __global__ void __launch_bounds__(kThreads, 1) f32_attention_kernel(const Args t
         }
         __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
         for (int i = first; i < last; ++i) {
             const PlanItem item = load_item(plan, i);
             if (item.m <= kFewRows)
                 few_rows<HD>(a, plan, item, sm, ring, wait);
+            else if (item.m <= 64)
+                many_rows<HD, 4>(a, plan, item, sm, ring, wait);
+            else if (item.m <= 96)
+                many_rows<HD, 6>(a, plan, item, sm, ring, wait);
             else
-                many_rows<HD>(a, plan, item, sm, ring, wait);
+                many_rows<HD, 8>(a, plan, item, sm, ring, wait);
         }
     }
     __syncthreads();
@@ -531,9 +609,11 @@ void f32_plan_shape(int head_dim, int sm_count, PlanShape &shape)
     shape.block = kBlock;
     shape.ctas = sm_count;
     shape.solo_m = kFewRows;
-    // Hundreds of clocks: a block's bytes at HBM's share, its products on the FP32 units, an item's start and end.
-    shape.solo_cost = std::max(1, 28 * head_dim / 128);
-    shape.pair_cost = std::max(1, 100 * head_dim / 128);
+    // Hundreds of clocks: a block's bytes at an SM's share of HBM, its products on the FP32 units, an item's start
+    // and end.
+    shape.solo_cost = std::max(1, 30 * head_dim / 128);
+    shape.pair_cost = std::max(1, 140 * head_dim / 128);
+    shape.more_cost = 140 * head_dim / 128;
     shape.item_cost = 60;
     shape.slots_per_item = 1;
 }

@@ -128,7 +128,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                 t.keys = row.position + 1 - seg.start;
             }
             const int blocks = (t.keys + shape.block - 1) / shape.block;
-            const int cost = t.m <= shape.solo_m ? shape.solo_cost : shape.pair_cost;
+            const int cost = shape.block_cost(t.m);
             total += (long long)shape.kv_heads * (blocks * cost + shape.item_cost);
             plan.tiles.push_back(t);
         }
@@ -152,7 +152,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
         for (int h = 0; h < shape.kv_heads; ++h)
             for (int t = seg.tile0; t < seg.tile0 + tiles; ++t) {
                 const PlanTile &tile = plan.tiles[t];
-                const int cost = tile.m <= shape.solo_m ? shape.solo_cost : shape.pair_cost;
+                const int cost = shape.block_cost(tile.m);
                 const int blocks = (tile.keys + shape.block - 1) / shape.block;
                 PlanSlots &slots = plan.slots[(size_t)t * shape.kv_heads + h];
                 slots.first = plan.partials;
