@@ -6,7 +6,9 @@
 //  * a thread of warp 16 loads the pages of a block's K and V with TMA (128-byte swizzle) into a ring of stages;
 //  * one lane each of warps 17 and 18 issues the MMAs of a softmax group: S from shared memory (Q and K, both
 //    K-major), O with P from tensor memory and V from shared memory as it lies (MN-major);
-//  * warp 19 clears the rows of V behind a tile's last key;
+//  * warp 19 looks through the rows of V that not every row of the tile sees: it clears those behind the last key,
+//    and takes infinities and NaN out of the others, which the rows that do see them get back at the end (a
+//    weight of zero would turn them into NaN);
 //  * warps 0-7 and 8-15 are two softmax groups, each with its own O and two S / P buffers in tensor memory; two
 //    threads share a row, each with half of a block's keys and half of the output's columns.  A large tile
 //    (129..256 rows) gives each group 128 of its rows and every K and V block serves both; a small one gives
@@ -31,10 +33,9 @@ namespace {
 
 constexpr int kTileRows = 128, kBlockKeys = 64;
 constexpr int kGroupThreads = 2 * kTileRows, kThreads = 2 * kGroupThreads + 128;
-#ifndef SATORI_EVERY
-#define SATORI_EVERY 4
-#endif
-constexpr int kEvery = SATORI_EVERY;
+// One pair of exponentials in four by a polynomial on the FP32 units: at 36 requests on 4096 shared keys and at 64 on
+// 131072 about 6 % less time than with none, and no less with one in two or three.
+constexpr int kEvery = 4;
 constexpr float kLazy = 8.0f;                  // log2 of what a weight may exceed 1 by
 
 template <int HD>
@@ -52,10 +53,14 @@ struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t s_full[2][2], p_ready[2][2];      // [group][buffer]: blocks in turn
     uint64_t q_ready[2], o_before[2], o_full[2];                   // o_before: all products but the item's last
-    uint64_t tail_full[2], tail_clear[2], drained[2];
+    uint64_t edge_full[2], edge_clear[2], drained[2];
     uint32_t tmem;
     volatile int abort;
     float exchange[2][2][kTileRows];           // [group][half][row]: maximum, then sum
+    // What warp 19 took out of V: the item (+ 1) that it concerns, and by column the first key, counted from the
+    // first that not every row sees, with an infinity of either sign (with both: a NaN); 255: none.
+    volatile int strange[2];
+    volatile uint8_t first_strange[2][2][128];
 };
 static_assert(sizeof(Barriers) <= 3072, "header");
 
@@ -252,14 +257,15 @@ struct Work {
     // order of use: the leading blocks' K, then V and the next K in turn.
     __device__ __forceinline__ int blocks(int g) const { return pair ? item.blocks : (item.blocks + 1 - g) / 2; }
     __device__ __forceinline__ int lead() const { return min(item.blocks, pair ? 2 : 4); }
-    // The group whose MMA warp asks for the clearing of the last V: its only user, or the first of two.
-    __device__ __forceinline__ int tail_group() const { return pair ? 0 : (item.blocks - 1) & 1; }
-    // Keys of the item's last block, when the tile ends inside it; 0: no row of V needs clearing.
-    __device__ __forceinline__ int tail() const
+    // Keys of the tile that every row of it sees.
+    __device__ __forceinline__ int seen_by_all(const DevPlan *plan, int group) const
     {
-        const int have = item.keys - (item.block0 + item.blocks - 1) * kBlockKeys;
-        return have < kBlockKeys ? have : 0;
+        if (item.start < 0 || item.m0 % group + item.m <= group) return item.keys;
+        const int2 row = __ldg(reinterpret_cast<const int2 *>(plan_array<PlanRow>(plan, plan->seg_rows) + item.row_off) + item.m0 / group);
+        return row.y + 1 - item.start;
     }
+    // The item's first block with keys that not every row sees, or with none; item.blocks or more: no such block.
+    __device__ __forceinline__ int edge(int seen) const { return max(0, seen - item.block0 * kBlockKeys) / kBlockKeys; }
 };
 
 // A place in the ring of stages, and the parity of its turn.
@@ -299,6 +305,58 @@ __device__ __noinline__ uint4 load_unaligned(const void *src)
     const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
     return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
                       h[6] | (uint32_t)h[7] << 16);
+}
+
+// Whether any of 8 values is infinite or NaN: an exponent of ones carries into the sign's place.
+template <int TYPE>
+__device__ __forceinline__ bool not_finite(uint4 v)
+{
+    constexpr uint32_t kExponent = TYPE == SATORI_BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = TYPE == SATORI_BF16 ? 0x00800080u : 0x04000400u;
+    return (((v.x & kExponent) + kOne) | ((v.y & kExponent) + kOne) | ((v.z & kExponent) + kOne) | ((v.w & kExponent) + kOne)) & 0x80008000u;
+}
+
+// Notes for group g the infinities and NaN in rows lo .. have - 1 of a block of V, whose row 0 is `key` keys behind
+// the first that not every row sees, and (unless they are to be noted for the other group too) sets them to zero.
+// A tile's rows stand for at most 256 tokens, so a key that one of them sees and another does not is at most the
+// 255th; a later row of the block is seen by none.  Called by a whole warp; each lane has columns of its own.
+template <int TYPE, int HD>
+__device__ __noinline__ void take_out(Barriers *bar, int g, int tag, uint8_t *v, int lo, int have, int key, bool again)
+{
+    const int lane = threadIdx.x & 31;
+    const bool fresh = bar->strange[g] != tag;
+    __syncwarp();
+    for (int c = lane; c < HD; c += 32) {
+        int first[2] = {255, 255};
+        if (!fresh) {
+            first[0] = bar->first_strange[g][0][c];
+            first[1] = bar->first_strange[g][1][c];
+        }
+        for (int r = lo; r < have; ++r) {
+            uint16_t *at = reinterpret_cast<uint16_t *>(v + c / 64 * Layout<HD>::kHalf + r * 128 + ((((c % 64) / 8) ^ (r & 7)) * 16) + c % 8 * 2);
+            const uint32_t x = *at, exponent = TYPE == SATORI_BF16 ? 0x7F80u : 0x7C00u;
+            if ((x & exponent) != exponent) continue;
+            const bool nan = x & ~exponent & 0x7FFFu;
+            if (nan || !(x & 0x8000u)) first[0] = min(first[0], key + r);
+            if (nan || (x & 0x8000u)) first[1] = min(first[1], key + r);
+            if (!again) *at = 0;
+        }
+        bar->first_strange[g][0][c] = (uint8_t)first[0];
+        bar->first_strange[g][1][c] = (uint8_t)first[1];
+    }
+    if (lane == 0) bar->strange[g] = tag;
+    __syncwarp();
+}
+
+// Adds what take_out noted to 32 columns of a row that sees `keys` of the keys that not every row sees.
+__device__ __forceinline__ void put_back(const Barriers *bar, int g, int keys, int c, uint32_t *o)
+{
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        float v = __uint_as_float(o[e]);
+        if (keys > bar->first_strange[g][0][c + e]) v += INFINITY;
+        if (keys > bar->first_strange[g][1][c + e]) v -= INFINITY;
+        o[e] = __float_as_uint(v);
+    }
 }
 
 // 32 columns of a row's accumulator: its share of the partial record, or of the output.
@@ -459,11 +517,11 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             mbar_init(&bar->q_ready[g], kGroupThreads);
             mbar_init(&bar->o_before[g], 1);
             mbar_init(&bar->o_full[g], 1);
-            mbar_init(&bar->tail_full[g], 1);
-            mbar_init(&bar->tail_clear[g], 32);
+            mbar_init(&bar->edge_full[g], 1);
+            mbar_init(&bar->edge_clear[g], 32);
             mbar_init(&bar->drained[g], 1);
         }
-        bar->abort = 0;
+        bar->abort = bar->strange[0] = bar->strange[1] = 0;
         fence_mbar_init();
     }
     if (warp == 17) {
@@ -509,30 +567,46 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
         }
         __syncwarp();
     } else if (warp == 19) {
-        // ---- V behind the last key: whatever the stage or the page holds there meets weights of zero, so it
-        // must be finite.
+        // ---- V at the edge of what the rows see
         Ring<NS> ring;
-        uint32_t phase = 0;                            // bit g: tail_full[g]
+        uint32_t phase = 0;                            // bit g: edge_full[g]
         bool ok = true;
         for (int i = first; i < last && ok; ++i) {
             const Work w = load_work(plan, i);
-            const int have = w.tail(), g = w.tail_group();
-            ring.advance(2 * w.item.blocks - 1);       // the item's last load
-            if (have > 0) {
-                // The MMA warp has seen the load arrive, and waits: the stage keeps its contents meanwhile.
-                ok = __all_sync(0xFFFFFFFFu, wait(&bar->tail_full[g], phase >> g & 1u));
+            const int n = w.item.blocks, lead = w.lead(), seen = w.seen_by_all(plan, a.group);
+            int at = 0;                                // the item's loads passed
+            for (int j = w.edge(seen); j < n; ++j) {
+                const int unit = lead + j + min(j, n - lead);
+                ring.advance(unit - at);
+                at = unit;
+                // The MMA warps that use the block have seen the load arrive, and wait: the stage keeps its contents,
+                // and the groups are done with the last item's findings.
+                for (int g = 0; g < 2 && ok; ++g) {
+                    if (!w.pair && g != (j & 1)) continue;
+                    ok = __all_sync(0xFFFFFFFFu, wait(&bar->edge_full[g], phase >> g & 1u));
+                    phase ^= 1u << g;
+                }
                 if (!ok) break;
-                phase ^= 1u << g;
-                uint8_t *v = stages + (size_t)ring.stage * L::kTile + have * 128;
-                for (int c = lane; c < (kBlockKeys - have) * 8; c += 32)
+                const int key0 = (w.item.block0 + j) * kBlockKeys, have = min(kBlockKeys, w.item.keys - key0);
+                const int lo = min(have, max(0, seen - key0));
+                uint8_t *v = stages + (size_t)ring.stage * L::kTile;
+                bool strange = false;
+                for (int c = lane; c < (have - lo) * 8; c += 32)
 #pragma unroll
                     for (int h = 0; h < HD / 64; ++h)
-                        *reinterpret_cast<uint4 *>(v + h * L::kHalf + c * 16) = make_uint4(0, 0, 0, 0);
+                        strange |= not_finite<TYPE>(*reinterpret_cast<const uint4 *>(v + h * L::kHalf + lo * 128 + c * 16));
+                if (__any_sync(0xFFFFFFFFu, strange)) {
+                    for (int g = 0; g < 2; ++g)
+                        if (w.pair || g == (j & 1)) take_out<TYPE, HD>(bar, g, i + 1, v, lo, have, key0 - seen, w.pair && g == 0);
+                }
+                for (int c = have * 8 + lane; c < kBlockKeys * 8; c += 32)
+#pragma unroll
+                    for (int h = 0; h < HD / 64; ++h) *reinterpret_cast<uint4 *>(v + h * L::kHalf + c * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&bar->tail_clear[g]);
-                if (w.pair) mbar_arrive(&bar->tail_clear[1]);
+                for (int g = 0; g < 2; ++g)
+                    if (w.pair || g == (j & 1)) mbar_arrive(&bar->edge_clear[g]);
             }
-            ring.next();
+            ring.advance(2 * n - at);
         }
     } else if (warp == 17 || warp == 18) {
         // ---- matrix products of group g
@@ -549,12 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             // Both groups pass every load in order, and a stage is loaded again when both have released it: so
             // the parity that a group waits for is never a round ahead of or behind the stage's.
             Ring<NS> ring;
-            uint32_t q_phase = 0, tail_phase = 0;
+            uint32_t q_phase = 0, edge_phase = 0;
             int done = 0;                              // this group's blocks so far
             bool ok = true, issued = false;
             for (int i = first; i < last && ok; ++i) {
                 const Work w = load_work(plan, i);
-                const int n = w.blocks(g), all = w.item.blocks, lead = w.lead();
+                const int n = w.blocks(g), all = w.item.blocks, lead = w.lead(), edge = w.edge(w.seen_by_all(plan, a.group));
                 if (n > 0) {
                     ok = wait(&bar->q_ready[g], q_phase);
                     q_phase ^= 1u;
@@ -592,10 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     if (!wait(&bar->full[ring.stage], ring.parity)) return false;
                     if (mine(j)) {
                         const int k = index(j), at = done + k;
-                        if (j + 1 == all && w.tail() > 0) {
-                            if (w.tail_group() == g) mbar_arrive(&bar->tail_full[g]);
-                            if (!wait(&bar->tail_clear[g], tail_phase)) return false;
-                            tail_phase ^= 1u;
+                        if (j >= edge) {
+                            mbar_arrive(&bar->edge_full[g]);
+                            if (!wait(&bar->edge_clear[g], edge_phase)) return false;
+                            edge_phase ^= 1u;
                         }
                         if (!wait(&bar->p_ready[g][at & 1], (uint32_t)(at >> 1) & 1u)) return false;
                         fence_after();
@@ -756,11 +830,14 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             __syncwarp();
             fence_after();
             const float inverse = 1.0f / sum;
+            const bool strange = bar->strange[g] == i + 1;
+            const int seen = strange ? w.seen_by_all(plan, a.group) : 0;
 #pragma unroll
             for (int c = 0; c < HD / 2; c += 32) {
                 uint32_t o[32];
                 tmem_load32(o_addr + c, o);
                 tmem_wait_load(o);
+                if (strange) put_back(bar, g, limit - seen, half * (HD / 2) + c, o);
                 if (live) store_output<TYPE, HD>(t, plan, w, o, inverse, row, head, record, half * (HD / 2) + c);
                 __syncwarp();
             }

@@ -534,3 +534,53 @@ def test_random_serving_run(env):
             counts = [int(rng.choice([1, 1, 1, 0, 25])) for _ in order]
             q = m.step(order, counts)
             m.check(order, counts, q)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,kv_heads,group,page", [(128, 2, 4, 32), (64, 2, 1, 64), (64, 1, 7, 16), (96, 1, 3, 16), (128, 1, 1, 128)])
+@pytest.mark.parametrize("before,count", [(0, 2), (0, 70), (61, 9), (200, 300)])
+def test_infinities_and_nan_in_masked_places(env, kind, dim, kv_heads, group, page, before, count):
+    """What a token's K and V hold reaches the rows of the same step from that token on and no others: each column of
+    the output takes the infinities and NaN of that column of the V it sees."""
+    torch = env[1]
+    m = Model(env, kind, dim, kv_heads, group, page, pages=64)
+    s, other = m.new(), m.new()
+    if before:
+        m.step([s, other], [before, 3])
+    counts = [count, 4]
+    queries = m.step([s, other], counts)
+    total = before + count
+    inf = math.inf
+    # (token, head, column, value); the second token's weight is above zero: scores are small.
+    marks = [(before + 1, 0, 3, inf), (total - 1, 0, 3, -inf), (before + count // 2, kv_heads - 1, dim - 1, math.nan),
+             (before + max(1, count // 3), 0, 40, -inf), (total - 1, kv_heads - 1, 17, math.nan)]
+    table = m.cache.table(s)
+    held = {(t, h, c): v for t, h, c, v in marks}      # (a later mark of the same place replaces it)
+    for (t, h, c), v in held.items():
+        m.pool[0, int(table[t // page]), 1, h, t % page, c] = v
+    m.pool[1, int(table[(total - 1) // page]), 0, 0, (total - 1) % page, 5] = math.nan     # a key: its own row only
+    keys, values = m.tokens[s][0].copy(), m.tokens[s][1].copy()
+    for layer, q in enumerate(queries):
+        out = torch.full((sum(counts), kv_heads * group * dim), 7.0, dtype=torch.float32, device="cuda")
+        m.batch.attention_device(layer, q, out)
+        got = out.double().cpu().numpy().reshape(-1, kv_heads, group, dim)
+        qd = q.double().cpu().numpy().reshape(-1, kv_heads, group, dim)
+        assert np.isfinite(got[count:]).all()
+        for r in range(count):
+            t = before + r + 1
+            exact, size, scores = m.formula(qd[r], keys[layer, :t], values[layer, :t])
+            special = np.zeros((kv_heads, dim))
+            if layer == 0:
+                with np.errstate(invalid="ignore"):
+                    for (at, h, c), v in held.items():
+                        if at < t:
+                            special[h, c] += v
+            elif r == count - 1:
+                special[0] = math.nan
+            special = np.broadcast_to(special[:, None], got[r].shape)
+            strange = ~np.isfinite(special)
+            assert np.array_equal(got[r][strange], special[strange], equal_nan=True), (layer, r)
+            tol = (2 * (dim + 4) * scores[..., None] + 2 * (t + 16)) * U * size
+            if kind != "f32":
+                tol = tol + torch.finfo(m.dtype).eps / 2 * size
+            assert np.all(np.abs(got[r] - exact)[~strange] <= tol[~strange]), (layer, r)
