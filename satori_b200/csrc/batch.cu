@@ -204,7 +204,9 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const Batch
     __shared__ float weight[kCombineHeads][kCombineChunk], factor[kCombineHeads], total[kCombineHeads];
     __shared__ int count[kCombineHeads];
     __shared__ float4 slices[SLICES][kCombineQuads];
-    pdl_wait();      // and no early start for the next launch: its blocks would take the SMs from this one's
+    // What it reads before pdl_wait is the plan's, which lay there when the attention kernel started: a copy on the
+    // stream brought it, and no launch behind a copy starts before it.  And no early start for the next launch: its
+    // blocks would take the SMs from this one's.
     const DevPlan *plan = a.plan;
     const int tid = threadIdx.x, mine = tid >> 5, lane = tid & 31;
     const int quads = a.head_dim / 4;
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const Batch
             __syncthreads();
             int most = 0;
             for (int h = 0; h < heads; ++h) most = max(most, count[h]);
+            pdl_wait();
             for (int chunk = 0; chunk < most; chunk += kCombineChunk) {
                 unsigned at[kCombineChunk / 32];
                 float2 ml[kCombineChunk / 32];
@@ -339,6 +342,117 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const Batch
             }
         }
         __syncthreads();
+    }
+}
+
+// The same with a warp for a row and up to 8 query heads, for launches with thousands of rows: no barriers, and the
+// loads that wait for one another are those of 24 rows an SM at a time, not of 4.  Lane (s, h) finds every fourth
+// record of head h; the records' weights meet in shuffles.  ITEMS: groups of 4 output values a lane.
+template <int TYPE, int ITEMS>
+__global__ void __launch_bounds__(kCombineThreads, ITEMS > 8 ? 2 : 3) combine_rows_kernel(const BatchAttn a, const CombineShape c)
+{
+    constexpr int kLanes = 32 / kCombineHeads;         // of a head
+    const DevPlan *plan = a.plan;
+    const int lane = threadIdx.x & 31, h = lane % kCombineHeads, quads = a.head_dim / 4;
+    const int *chain_off = plan_array<int>(plan, plan->chain_off), *merges = plan_array<int>(plan, plan->merges);
+    const PlanLink *chain = plan_array<PlanLink>(plan, plan->chain);
+    const PlanSlots *slots = plan_array<PlanSlots>(plan, plan->slots);
+    const float4 *values = reinterpret_cast<const float4 *>(plan->part_o);
+    const float2 *part_ml = plan->part_ml;
+    const int units = plan->head.merges * c.octets, warps = gridDim.x * (kCombineThreads / 32);
+    for (int u = blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
+        const int g0 = u % c.octets * kCombineHeads, heads = min(kCombineHeads, a.group - g0);
+        const int merge = merges[u / c.octets], kv_head = merge % a.kv_heads, row = merge / a.kv_heads;
+        const int c0 = chain_off[row], c1 = chain_off[row + 1];
+        int link = c0, rank = lane / kCombineHeads, records = 0;
+        unsigned first = 0, step = 0;
+        bool direct = false;                           // the item wrote the head's output itself
+        auto enter = [&] {
+            const PlanLink l = chain[link];
+            const int m = l.index * a.group + g0 + min(h, heads - 1), mt = m % c.tile_m;
+            const PlanSlots s = slots[(l.tile0 + m / c.tile_m) * a.kv_heads + kv_head];
+            direct = direct || s.first < 0;
+            first = (unsigned)(s.first * c.record_rows + mt);
+            records = s.records / s.step;
+            step = (unsigned)(s.step * c.record_rows);
+        };
+        enter();
+        pdl_wait();
+        float4 acc[ITEMS];
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) acc[k] = make_float4(0, 0, 0, 0);
+        const int n = heads * quads;
+        float ref = -INFINITY, sum = 0;
+        for (;;) {
+            while (link < c1 && rank >= records) {
+                rank -= records;
+                if (++link < c1) enter();
+            }
+            const bool has = link < c1 && h < heads && !direct;
+            if (!__any_sync(0xFFFFFFFFu, has)) break;
+            const unsigned at = has ? first + (unsigned)rank * step : 0;
+            const float2 ml = has ? part_ml[at] : make_float2(-INFINITY, 0.0f);
+            float top = ml.x;
+#pragma unroll
+            for (int o = kCombineHeads; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            top = fmaxf(top, ref);
+            const float keep = top == -INFINITY ? 1.0f : exp2f(ref - top);
+            const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);      // no key: nothing was stored
+            sum *= keep;
+            if (w != 0) sum = fmaf(w, ml.y, sum);
+            ref = top;
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                const int i = k * 32 + lane, g = c.by_column ? i % heads : i / quads;
+                const float f = __shfl_sync(0xFFFFFFFFu, keep, g);
+                acc[k].x *= f;
+                acc[k].y *= f;
+                acc[k].z *= f;
+                acc[k].w *= f;
+            }
+#pragma unroll 1
+            for (int s = 0; s < kLanes; ++s) {
+                if (!__any_sync(0xFFFFFFFFu, lane / kCombineHeads == s && w != 0)) continue;
+                float4 v[ITEMS];
+                float weight[ITEMS];
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k) {
+                    const int i = k * 32 + lane, g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
+                    weight[k] = __shfl_sync(0xFFFFFFFFu, w, s * kCombineHeads + g);
+                    const unsigned rr = __shfl_sync(0xFFFFFFFFu, at, s * kCombineHeads + g), r = rr % (unsigned)c.record_rows;
+                    v[k] = make_float4(0, 0, 0, 0);
+                    if (i < n && weight[k] != 0)
+                        v[k] = values[c.by_column ? (size_t)(rr - r) * quads + (size_t)quad * c.record_rows + r : (size_t)rr * quads + quad];
+                }
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k) {
+                    acc[k].x = fmaf(v[k].x, weight[k], acc[k].x);
+                    acc[k].y = fmaf(v[k].y, weight[k], acc[k].y);
+                    acc[k].z = fmaf(v[k].z, weight[k], acc[k].z);
+                    acc[k].w = fmaf(v[k].w, weight[k], acc[k].w);
+                }
+            }
+            rank += kLanes;
+        }
+#pragma unroll
+        for (int o = kCombineHeads; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const float inverse = 1.0f / sum;
+        const unsigned written = __ballot_sync(0xFFFFFFFFu, direct);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int i = k * 32 + lane, g = c.by_column ? i % heads : i / quads, quad = c.by_column ? i / heads : i % quads;
+            const float f = __shfl_sync(0xFFFFFFFFu, inverse, g);
+            if (i >= n || (written >> g & 1u)) continue;
+            const float v[4] = {acc[k].x * f, acc[k].y * f, acc[k].z * f, acc[k].w * f};
+            const long long to = (long long)row * a.ldo + (long long)(kv_head * a.group + g0 + g) * a.head_dim + quad * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (a.out_f32)
+                    reinterpret_cast<float *>(a.out)[to + e] = v[e];
+                else
+                    reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + e] = Elem<TYPE>::from_float(v[e]);
+            }
+        }
     }
 }
 
@@ -467,6 +581,11 @@ cudaError_t launch_append(const AppendArgs &a, int rows, int wide_in, int wide_o
 template <int TYPE>
 static cudaError_t launch_combine_type(const BatchAttn &a, const CombineShape &c, int slices, dim3 grid, cudaStream_t stream)
 {
+    if (slices == 0) {       // a warp for a row
+        const int items = (std::min(a.group, kCombineHeads) * a.head_dim / 4 + 31) / 32;
+        auto kernel = items <= 4 ? combine_rows_kernel<TYPE, 4> : items <= 8 ? combine_rows_kernel<TYPE, 8> : combine_rows_kernel<TYPE, 16>;
+        return launch_overlapped(kernel, grid, kCombineThreads, 0, stream, a, c);
+    }
     auto kernel = slices == 4 ? combine_kernel<TYPE, 4> : slices == 2 ? combine_kernel<TYPE, 2> : combine_kernel<TYPE, 1>;
     return launch_overlapped(kernel, grid, kCombineThreads, 0, stream, a, c);
 }
@@ -474,14 +593,20 @@ static cudaError_t launch_combine_type(const BatchAttn &a, const CombineShape &c
 cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile_m, bool by_column, int merges, int sm_count,
                                    cudaStream_t stream)
 {
-    // As many slices as a row's values leave threads for, and four when there are too few rows to fill the SMs
-    // (one sequence of 4k tokens over 4 KV heads, 66 records a row: 13 us with one slice, 9 with four).
+    // From 2048 rows of a KV head on there are enough for a warp each (the prompts of 8 requests, 10k rows: the call
+    // 137 us, with a block for each 172; 512 requests over 8 KV heads 235 and 247, 64 over 32 KV heads 134 and 138);
+    // with fewer, their records are better dealt to whole blocks (256 requests over 4 KV heads 83 us, with a warp
+    // for each 99; 64 behind 32k tokens 81 and 132).  There as many slices as a row's values leave threads for, and
+    // four when there are too few rows to fill the SMs (one sequence of 4k tokens over 4 KV heads, 66 records a
+    // row: 13 us with one slice, 9 with four).
     const int outputs = std::min(a.group, kCombineHeads) * a.head_dim / 4, octets = (a.group + kCombineHeads - 1) / kCombineHeads;
-    const int slices = outputs <= 64 || merges * octets < sm_count ? 4 : outputs <= 128 ? 2 : 1;
-    const int quads = kCombineThreads / slices;
+    const long long rows = (long long)merges * octets;
+    const bool warps = rows >= 2048;
+    const int slices = warps ? 0 : outputs <= 64 || rows < sm_count ? 4 : outputs <= 128 ? 2 : 1;
+    const int quads = warps ? outputs : kCombineThreads / slices;
     const CombineShape c = {record_rows, tile_m, by_column, octets, (outputs + quads - 1) / quads};
-    const long long units = (long long)merges * octets * c.parts;
-    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>(units, 8ll * sm_count)));
+    const long long blocks = warps ? (rows + kCombineThreads / 32 - 1) / (kCombineThreads / 32) : rows * c.parts;
+    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>(blocks, (warps ? 3ll : 8ll) * sm_count)));
     switch (a.type) {
     case SATORI_F32: return launch_combine_type<SATORI_F32>(a, c, slices, grid, stream);
     case SATORI_F16: return launch_combine_type<SATORI_F16>(a, c, slices, grid, stream);
