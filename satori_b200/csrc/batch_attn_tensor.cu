@@ -8,7 +8,8 @@
 //    K-major), O with P from tensor memory and V from shared memory as it lies (MN-major);
 //  * warp 19 looks through the rows of V that not every row of the tile sees: it clears those behind the last key,
 //    and takes infinities and NaN out of the others, which the rows that do see them get back at the end (a
-//    weight of zero would turn them into NaN);
+//    weight of zero would turn them into NaN).  It also brings the queries of items of at most 24 rows (the usual
+//    step of a request) while the item before is worked on, so that their first scores wait for nothing;
 //  * warps 0-7 and 8-15 are two softmax groups, each with its own O and two S / P buffers in tensor memory; two
 //    threads share a row, each with half of a block's keys and half of the output's columns.  A large tile
 //    (129..256 rows) gives each group 128 of its rows and every K and V block serves both; a small one gives
@@ -32,6 +33,7 @@ namespace satori {
 namespace {
 
 constexpr int kTileRows = 128, kBlockKeys = 64;
+constexpr int kSmallRows = 24;                 // rows of an item whose queries are brought ahead
 constexpr int kGroupThreads = 2 * kTileRows, kThreads = 2 * kGroupThreads + 128;
 // One pair of exponentials in four by a polynomial on the FP32 units: at 36 requests on 4096 shared keys and at 64 on
 // 131072 about 6 % less time than with none, and no less with one in two or three.
@@ -42,9 +44,12 @@ template <int HD>
 struct Layout {
     static constexpr int kQHalf = kTileRows * 128, kHalf = kBlockKeys * 128;       // rows of 64 columns
     static constexpr int kQTile = kQHalf * (HD / 64), kTile = kHalf * (HD / 64);   // Q; K or V
-    static constexpr int kStages = HD == 128 ? 10 : 20;
-    static constexpr int kHeader = 3072;
-    static constexpr int kBytes = kHeader + 2 * kQTile + kStages * kTile;
+    static constexpr int kSmallHalf = kSmallRows * 128, kSmall = kSmallHalf * (HD / 64);       // Q brought ahead
+    static constexpr int kStages = HD == 128 ? 9 : 20;
+    static constexpr int kHeader = 4096;
+    // header, 2 small Qs, 2 Q tiles, stages.  The MMAs read 128 rows from a small Q on, whatever lies behind it.
+    static constexpr int kBytes = kHeader + 2 * kSmall + 2 * kQTile + kStages * kTile;
+    static_assert((kHeader + 2 * kSmall) % 1024 == 0 && kSmallHalf % 1024 == 0, "swizzle");
     static constexpr int kOCol = 4 * kBlockKeys;                   // tensor memory: S / P buffers, then O
 };
 
@@ -54,6 +59,7 @@ struct Barriers {
     uint64_t s_full[2][2], p_ready[2][2];      // [group][buffer]: blocks in turn
     uint64_t q_ready[2], o_before[2], o_full[2];                   // o_before: all products but the item's last
     uint64_t edge_full[2], edge_clear[2], drained[2];
+    uint64_t small_full[2], small_free[2];     // a small Q is there, or read
     uint32_t tmem;
     volatile int abort;
     float exchange[2][2][kTileRows];           // [group][half][row]: maximum, then sum
@@ -62,7 +68,7 @@ struct Barriers {
     volatile int strange[2];
     volatile uint8_t first_strange[2][2][128];
 };
-static_assert(sizeof(Barriers) <= 3072, "header");
+static_assert(sizeof(Barriers) <= 4096, "header");
 
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -253,10 +259,14 @@ struct TensorArgs {
 struct Work {
     PlanItem item;
     bool pair;
+    int flip;            // items in turn give their first block to group 0 and 1, so that two short ones run at once
     // Blocks of each softmax group, and how many blocks ahead of O the scores run.  An item's loads are in the
     // order of use: the leading blocks' K, then V and the next K in turn.
-    __device__ __forceinline__ int blocks(int g) const { return pair ? item.blocks : (item.blocks + 1 - g) / 2; }
+    __device__ __forceinline__ int blocks(int g) const { return pair ? item.blocks : (item.blocks + 1 - (g ^ flip)) / 2; }
+    __device__ __forceinline__ bool takes(int g, int j) const { return pair || ((j ^ flip) & 1) == g; }
+    __device__ __forceinline__ int block(int g, int k) const { return item.block0 + (pair ? k : 2 * k + (g ^ flip)); }
     __device__ __forceinline__ int lead() const { return min(item.blocks, pair ? 2 : 4); }
+    __device__ __forceinline__ bool small() const { return item.m <= kSmallRows; }
     // Keys of the tile that every row of it sees.
     __device__ __forceinline__ int seen_by_all(const DevPlan *plan, int group) const
     {
@@ -296,6 +306,7 @@ __device__ __forceinline__ Work load_work(const DevPlan *plan, int i)
 #pragma unroll
     for (int k = 0; k < (int)(sizeof(PlanItem) / 16); ++k) dst[k] = __ldg(src + k);
     w.pair = w.item.m > kTileRows;
+    w.flip = i & 1;
     return w;
 }
 
@@ -496,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
     const BatchAttn &a = t.a;
     extern __shared__ __align__(1024) uint8_t smem[];
     Barriers *bar = reinterpret_cast<Barriers *>(smem);
-    uint8_t *q_tiles = smem + L::kHeader, *stages = q_tiles + 2 * L::kQTile;
+    uint8_t *small_q = smem + L::kHeader, *q_tiles = small_q + 2 * L::kSmall, *stages = q_tiles + 2 * L::kQTile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (smem_u32(smem) & 1023u) {              // the swizzle needs it; dynamic shared memory starts there
@@ -520,6 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             mbar_init(&bar->edge_full[g], 1);
             mbar_init(&bar->edge_clear[g], 32);
             mbar_init(&bar->drained[g], 1);
+            mbar_init(&bar->small_full[g], 1);
+            mbar_init(&bar->small_free[g], 2);
         }
         bar->abort = bar->strange[0] = bar->strange[1] = 0;
         fence_mbar_init();
@@ -567,10 +580,50 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
         }
         __syncwarp();
     } else if (warp == 19) {
-        // ---- V at the edge of what the rows see
+        // ---- V at the edge of what the rows see, and small Qs ahead
         Ring<NS> ring;
         uint32_t phase = 0;                            // bit g: edge_full[g]
         bool ok = true;
+        int smalls = 0;                                // small items so far
+        auto bring = [&](int i) -> bool {
+            if (i >= last) return true;
+            const Work w = load_work(plan, i);
+            if (!w.small()) return true;
+            constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, BATCH = 6, BATCHES = kSmallRows / (ROWS * BATCH);
+            static_assert(BATCHES * ROWS * BATCH == kSmallRows, "rows");
+            const int b = smalls & 1, m = w.item.m0 + lane;
+            int row = 0;
+            if (lane < w.item.m)
+                row = __ldg(&(plan_array<PlanRow>(plan, plan->seg_rows) + w.item.row_off + m / a.group)->row);
+            const int q_head = (w.item.kv_head * a.group + m % a.group) * HD, c = lane % PER_ROW;
+            uint8_t *q_tile = small_q + b * L::kSmall;
+            const bool free = __all_sync(0xFFFFFFFFu, wait(&bar->small_free[b], (uint32_t)((smalls >> 1) & 1) ^ 1u));
+            if (!free) return false;
+#pragma unroll
+            for (int k = 0; k < BATCHES; ++k) {
+                if (k * BATCH * ROWS >= w.item.m) break;
+                uint4 v[BATCH];
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    const int from = (k * BATCH + e) * ROWS + lane / PER_ROW;
+                    const int r_from = __shfl_sync(0xFFFFFFFFu, row, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
+                    const T *src = reinterpret_cast<const T *>(a.q) + (long long)r_from * a.ldq + h_from + c * 8;
+                    v[e] = make_uint4(0, 0, 0, 0);
+                    if (from < w.item.m) v[e] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
+                }
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    const int from = (k * BATCH + e) * ROWS + lane / PER_ROW;
+                    *reinterpret_cast<uint4 *>(q_tile + (c / 8) * L::kSmallHalf + from * 128 + (((c & 7) ^ (from & 7)) * 16)) = v[e];
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->small_full[b]);
+            ++smalls;
+            return true;
+        };
+        ok = bring(first) && bring(first + 1);
         for (int i = first; i < last && ok; ++i) {
             const Work w = load_work(plan, i);
             const int n = w.item.blocks, lead = w.lead(), seen = w.seen_by_all(plan, a.group);
@@ -582,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                 // The MMA warps that use the block have seen the load arrive, and wait: the stage keeps its contents,
                 // and the groups are done with the last item's findings.
                 for (int g = 0; g < 2 && ok; ++g) {
-                    if (!w.pair && g != (j & 1)) continue;
+                    if (!w.takes(g, j)) continue;
                     ok = __all_sync(0xFFFFFFFFu, wait(&bar->edge_full[g], phase >> g & 1u));
                     phase ^= 1u << g;
                 }
@@ -597,16 +650,17 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                         strange |= not_finite<TYPE>(*reinterpret_cast<const uint4 *>(v + h * L::kHalf + lo * 128 + c * 16));
                 if (__any_sync(0xFFFFFFFFu, strange)) {
                     for (int g = 0; g < 2; ++g)
-                        if (w.pair || g == (j & 1)) take_out<TYPE, HD>(bar, g, i + 1, v, lo, have, key0 - seen, w.pair && g == 0);
+                        if (w.takes(g, j)) take_out<TYPE, HD>(bar, g, i + 1, v, lo, have, key0 - seen, w.pair && g == 0);
                 }
                 for (int c = have * 8 + lane; c < kBlockKeys * 8; c += 32)
 #pragma unroll
                     for (int h = 0; h < HD / 64; ++h) *reinterpret_cast<uint4 *>(v + h * L::kHalf + c * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 for (int g = 0; g < 2; ++g)
-                    if (w.pair || g == (j & 1)) mbar_arrive(&bar->edge_clear[g]);
+                    if (w.takes(g, j)) mbar_arrive(&bar->edge_clear[g]);
             }
             ring.advance(2 * n - at);
+            ok = ok && bring(i + 2);                   // (its Q takes this one's place when the scores are there)
         }
     } else if (warp == 17 || warp == 18) {
         // ---- matrix products of group g
@@ -624,17 +678,30 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             // the parity that a group waits for is never a round ahead of or behind the stage's.
             Ring<NS> ring;
             uint32_t q_phase = 0, edge_phase = 0;
-            int done = 0;                              // this group's blocks so far
+            int done = 0, smalls = 0;                  // this group's blocks, and the small items, so far
             bool ok = true, issued = false;
             for (int i = first; i < last && ok; ++i) {
                 const Work w = load_work(plan, i);
-                const int n = w.blocks(g), all = w.item.blocks, lead = w.lead(), edge = w.edge(w.seen_by_all(plan, a.group));
-                if (n > 0) {
+                const int n = w.blocks(g), all = w.item.blocks, lead = w.lead(), seen = w.seen_by_all(plan, a.group);
+                const int edge = w.edge(seen), b = smalls & 1;
+                const bool small = w.small();
+                uint32_t q = q_low;
+                const uint32_t q_half = small ? L::kSmallHalf >> 4 : L::kQHalf >> 4;
+                if (small) {
+                    q = desc_low(smem_u32(small_q) + b * L::kSmall, 16);
+                    // (A group without a block waits too: its next wait is for the next turn's parity.)
+                    ok = wait(&bar->small_full[b], (uint32_t)(smalls >> 1) & 1u);
+                    if (n == 0)
+                        mbar_arrive(&bar->small_free[b]);
+                    else
+                        issued = issued || ok;
+                    ++smalls;
+                } else if (n > 0) {
                     ok = wait(&bar->q_ready[g], q_phase);
                     q_phase ^= 1u;
                     issued = issued || ok;
                 }
-                auto mine = [&](int j) { return w.pair || (j & 1) == g; };
+                auto mine = [&](int j) { return w.takes(g, j); };
                 auto index = [&](int j) { return w.pair ? j : j >> 1; };
                 int held = -1;                         // a stage of V to release after the next scores
                 auto release_held = [&] {
@@ -650,9 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                         const uint32_t d = s_col + (at & 1) * kBlockKeys, kd = k_low + ring.stage * (L::kTile >> 4);
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ++ks)
-                            mma_ss(d, q_low + (ks / 4) * (L::kQHalf >> 4) + (ks % 4) * 2,
+                            mma_ss(d, q + (ks / 4) * q_half + (ks % 4) * 2,
                                    kd + (ks / 4) * (L::kHalf >> 4) + (ks % 4) * 2, kDescS, ks > 0);
                         commit(&bar->s_full[g][at & 1]);
+                        if (small && index(j) == n - 1) commit(&bar->small_free[b]);
                         release_held();
                         commit(&bar->empty[ring.stage]);
                     } else {
@@ -667,6 +735,8 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     if (mine(j)) {
                         const int k = index(j), at = done + k;
                         if (j >= edge) {
+                            // What warp 19 takes out is noted when the group is done with the last item's notes.
+                            if (small && seen < w.item.keys && !wait(&bar->p_ready[g][at & 1], (uint32_t)(at >> 1) & 1u)) return false;
                             mbar_arrive(&bar->edge_full[g]);
                             if (!wait(&bar->edge_clear[g], edge_phase)) return false;
                             edge_phase ^= 1u;
@@ -735,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             // 16-byte chunk c of row r lies at chunk c ^ (r % 8).  Rows behind the tile keep what was there: their
             // lanes of S and O are never read.  All loads are in flight before the first store.
             const int warp_rows = min(32, w.item.m - (m - lane));          // live rows of the warp pair
-            if (half * 16 < warp_rows) {
+            if (half * 16 < warp_rows && !w.small()) {
                 constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, STEPS = 16 / ROWS;
                 const int c = lane % PER_ROW, mine = half * 16 + lane / PER_ROW, q_head = head * HD;
                 uint4 v[STEPS];
@@ -754,13 +824,15 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                         *reinterpret_cast<uint4 *>(q_tile + (c / 8) * L::kQHalf + rr * 128 + (((c & 7) ^ (rr & 7)) * 16)) = v[k];
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&bar->q_ready[g]);
+            if (!w.small()) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&bar->q_ready[g]);
+            }
 
             const bool idle = warp_rows <= 0;  // all of the warp pair's rows are behind the tile
             float ref = -INFINITY, sum = 0;    // ref: the maximum (log2 units) that the weights refer to
             for (int k = 0; k < blocks; ++k) {
-                const int block = w.item.block0 + (w.pair ? k : 2 * k + g), at = done + k;
+                const int block = w.block(g, k), at = done + k;
                 const uint32_t s_addr = lanes + (g * 2 + (at & 1)) * kBlockKeys;
                 wait(&bar->s_full[g][at & 1], (uint32_t)(at >> 1) & 1u);
                 if (!idle) {
