@@ -67,6 +67,9 @@ struct Barriers {
     // first that not every row sees, with an infinity of either sign (with both: a NaN); 255: none.
     volatile int strange[2];
     volatile uint8_t first_strange[2][2][128];
+    // Numbers and visible keys of the rows of the last small items.  Four: the scores of the second next come after
+    // both groups have used these.
+    int2 small_row[4][kSmallRows];
 };
 static_assert(sizeof(Barriers) <= 4096, "header");
 
@@ -310,6 +313,14 @@ __device__ __forceinline__ Work load_work(const DevPlan *plan, int i)
     return w;
 }
 
+// The number of a segment's row and how many of its keys the row sees.
+__device__ __forceinline__ int2 find_row(const DevPlan *plan, const Work &w, int group, int m)
+{
+    int2 own = __ldg(reinterpret_cast<const int2 *>(plan_array<PlanRow>(plan, plan->seg_rows) + w.item.row_off) + m / group);
+    own.y = w.item.start >= 0 ? own.y + 1 - w.item.start : w.item.keys;
+    return own;
+}
+
 // 16 bytes from any address of 2-byte elements.
 __device__ __noinline__ uint4 load_unaligned(const void *src)
 {
@@ -358,25 +369,25 @@ __device__ __noinline__ void take_out(Barriers *bar, int g, int tag, uint8_t *v,
     __syncwarp();
 }
 
-// Adds what take_out noted to 32 columns of a row that sees `keys` of the keys that not every row sees.
-__device__ __forceinline__ void put_back(const Barriers *bar, int g, int keys, int c, uint32_t *o)
+// Adds what take_out noted to `n` columns from c on of a row that sees `keys` of the keys that not every row sees,
+// where this thread has just stored them: floats `step` apart for every 4, or outputs.
+template <typename T>
+__device__ __noinline__ void put_back(const Barriers *bar, int g, int keys, int c, int n, T *at, int step)
 {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        float v = __uint_as_float(o[e]);
+    for (int e = 0; e < n; ++e) {
+        T *to = at + e / 4 * step + e % 4;
+        float v = (float)*to;
         if (keys > bar->first_strange[g][0][c + e]) v += INFINITY;
         if (keys > bar->first_strange[g][1][c + e]) v -= INFINITY;
-        o[e] = __float_as_uint(v);
+        *to = (T)v;
     }
 }
 
-// 32 columns of a row's accumulator: its share of the partial record, or of the output.
+// 32 columns of a row's accumulator: its share of the partial record, or of an output with 16-byte accesses.
 template <int TYPE, int HD>
-__device__ __forceinline__ void store_output(const TensorArgs &t, const DevPlan *plan, const Work &w, uint32_t *o,
+__device__ __forceinline__ void store_output(const BatchAttn &a, const DevPlan *plan, const Work &w, uint32_t *o,
                                              float inverse, int row, int head, long long record, int c)
 {
-    typedef typename Elem<TYPE>::type T;
-    const BatchAttn &a = t.a;
     if (!w.item.direct) {
         // [column / 4][row]: the warp's rows are neighbours.
         const int r = (int)(record % kTileRows);
@@ -389,32 +400,33 @@ __device__ __forceinline__ void store_output(const TensorArgs &t, const DevPlan 
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inverse);
     if (a.out_f32) {
-        float *dst = reinterpret_cast<float *>(a.out) + to;
+        uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<float *>(a.out) + to);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-            if (t.wide_out) {
-                *reinterpret_cast<uint4 *>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            } else {
-#pragma unroll
-                for (int f = 0; f < 4; ++f) dst[e + f] = __uint_as_float(o[e + f]);
-            }
-        }
+        for (int e = 0; e < 32; e += 4) dst[e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     } else {
-        T *dst = reinterpret_cast<T *>(a.out) + to;
+        uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<typename Elem<TYPE>::type *>(a.out) + to);
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
-            if (t.wide_out) {
-                uint4 v;
-                v.x = pack2<TYPE>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
-                v.y = pack2<TYPE>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-                v.z = pack2<TYPE>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
-                v.w = pack2<TYPE>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
-                *reinterpret_cast<uint4 *>(dst + e) = v;
-            } else {
-#pragma unroll
-                for (int f = 0; f < 8; ++f) dst[e + f] = Elem<TYPE>::from_float(__uint_as_float(o[e + f]));
-            }
+            uint4 v;
+            v.x = pack2<TYPE>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+            v.y = pack2<TYPE>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+            v.z = pack2<TYPE>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
+            v.w = pack2<TYPE>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
+            dst[e / 8] = v;
         }
+    }
+}
+
+// 16 columns of an output row at any address.
+template <int TYPE>
+__device__ __noinline__ void store_anywhere(const BatchAttn &a, const uint32_t *o, float inverse, long long to)
+{
+    for (int e = 0; e < 16; ++e) {
+        const float v = __uint_as_float(o[e]) * inverse;
+        if (a.out_f32)
+            reinterpret_cast<float *>(a.out)[to + e] = v;
+        else
+            reinterpret_cast<typename Elem<TYPE>::type *>(a.out)[to + e] = Elem<TYPE>::from_float(v);
     }
 }
 
@@ -592,13 +604,13 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, BATCH = 6, BATCHES = kSmallRows / (ROWS * BATCH);
             static_assert(BATCHES * ROWS * BATCH == kSmallRows, "rows");
             const int b = smalls & 1, m = w.item.m0 + lane;
-            int row = 0;
-            if (lane < w.item.m)
-                row = __ldg(&(plan_array<PlanRow>(plan, plan->seg_rows) + w.item.row_off + m / a.group)->row);
+            const int2 own = lane < w.item.m ? find_row(plan, w, a.group, m) : make_int2(0, 0);
+            const int row = own.x;
             const int q_head = (w.item.kv_head * a.group + m % a.group) * HD, c = lane % PER_ROW;
             uint8_t *q_tile = small_q + b * L::kSmall;
             const bool free = __all_sync(0xFFFFFFFFu, wait(&bar->small_free[b], (uint32_t)((smalls >> 1) & 1) ^ 1u));
             if (!free) return false;
+            if (lane < kSmallRows) bar->small_row[smalls & 3][lane] = own;
 #pragma unroll
             for (int k = 0; k < BATCHES; ++k) {
                 if (k * BATCH * ROWS >= w.item.m) break;
@@ -783,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t o_addr = lanes + L::kOCol + g * HD + half * (HD / 2);
         uint8_t *q_tile = q_tiles + g * L::kQTile;
-        int done = 0;                          // this group's blocks so far
+        int done = 0, smalls = 0;              // this group's blocks, and the small items, so far
         uint32_t before_phase = 0, full_phase = 0;
         for (int i = first; i < last; ++i) {
             const Work w = load_work(plan, i);
@@ -791,16 +803,21 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const int m = (w.pair ? g * kTileRows : 0) + r;
             const bool live = m < w.item.m;
             const long long record = (long long)(w.item.slot + g) * kTileRows + r;
+            int2 own = make_int2(0, 0);        // the row's number and the keys it sees
+            if (w.small()) {
+                if (quad == 0) {
+                    wait(&bar->small_full[smalls & 1], (uint32_t)(smalls >> 1) & 1u);
+                    if (live) own = bar->small_row[smalls & 3][r];
+                }
+                ++smalls;
+            } else if (live) {
+                own = find_row(plan, w, a.group, w.item.m0 + m);
+            }
             if (blocks == 0) {                 // a small tile's only block is the other group's
                 if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(-INFINITY, 0.0f);
                 continue;
             }
-            int2 own = make_int2(0, 0);        // the row's number and position
-            if (live)
-                own = __ldg(reinterpret_cast<const int2 *>(plan_array<PlanRow>(plan, plan->seg_rows) + w.item.row_off) +
-                            (w.item.m0 + m) / a.group);
-            const int row = own.x, head = w.item.kv_head * a.group + (w.item.m0 + m) % a.group;
-            const int limit = !live ? 0 : w.item.start >= 0 ? own.y + 1 - w.item.start : w.item.keys;
+            const int row = own.x, limit = own.y, head = w.item.kv_head * a.group + (w.item.m0 + m) % a.group;
             // Q rows into shared memory (each half 16 of the warp pair's 32), K-major with the 128-byte swizzle:
             // 16-byte chunk c of row r lies at chunk c ^ (r % 8).  Rows behind the tile keep what was there: their
             // lanes of S and O are never read.  All loads are in flight before the first store.
@@ -867,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                             __syncwarp();
                             fence_after();
                             const float factor = raise ? exp2_fast(ref - high) : 1.0f;
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < HD / 2; c += 16) {
                                 uint32_t o[16];
                                 tmem_load16(o_addr + c, o);
@@ -903,15 +920,35 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             fence_after();
             const float inverse = 1.0f / sum;
             const bool strange = bar->strange[g] == i + 1;
-            const int seen = strange ? w.seen_by_all(plan, a.group) : 0;
-#pragma unroll
-            for (int c = 0; c < HD / 2; c += 32) {
-                uint32_t o[32];
-                tmem_load32(o_addr + c, o);
-                tmem_wait_load(o);
-                if (strange) put_back(bar, g, limit - seen, half * (HD / 2) + c, o);
-                if (live) store_output<TYPE, HD>(t, plan, w, o, inverse, row, head, record, half * (HD / 2) + c);
-                __syncwarp();
+            const int c0 = half * (HD / 2);
+            const long long to = (long long)row * a.ldo + (long long)head * HD + c0;
+            // (Rolled, like the rescaling above: this code runs once an item, and fetching it took most of its time.)
+            if (w.item.direct && !t.wide_out) {
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o_addr + c, o);
+                    if (live) store_anywhere<TYPE>(a, o, inverse, to + c);
+                    __syncwarp();
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_addr + c, o);
+                    tmem_wait_load(o);
+                    if (live) store_output<TYPE, HD>(a, plan, w, o, inverse, row, head, record, c0 + c);
+                    __syncwarp();
+                }
+            }
+            if (strange && live) {
+                const int keys = limit - w.seen_by_all(plan, a.group);
+                if (!w.item.direct)
+                    put_back(bar, g, keys, c0, HD / 2, plan->part_o + ((record - r) * HD + c0 * kTileRows + r * 4), kTileRows * 4);
+                else if (a.out_f32)
+                    put_back(bar, g, keys, c0, HD / 2, reinterpret_cast<float *>(a.out) + to, 4);
+                else
+                    put_back(bar, g, keys, c0, HD / 2, reinterpret_cast<T *>(a.out) + to, 4);
             }
             if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(ref, sum);
             // The next item's first O overwrites this one after this group's next p_ready, so these loads are done.
