@@ -67,8 +67,9 @@ struct Barriers {
     // first that not every row sees, with an infinity of either sign (with both: a NaN); 255: none.
     volatile int strange[2];
     volatile uint8_t first_strange[2][2][128];
-    // Numbers and visible keys of the rows of the last small items.  Four: the scores of the second next come after
-    // both groups have used these.
+    // Numbers and visible keys of the rows of the last small items.  Four: the second next is written when the scores
+    // of this one are there, and the one in this one's place when those of the second next are, which follow this
+    // one's weights in either group.
     int2 small_row[4][kSmallRows];
 };
 static_assert(sizeof(Barriers) <= 4096, "header");
@@ -803,21 +804,20 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const int m = (w.pair ? g * kTileRows : 0) + r;
             const bool live = m < w.item.m;
             const long long record = (long long)(w.item.slot + g) * kTileRows + r;
-            int2 own = make_int2(0, 0);        // the row's number and the keys it sees
-            if (w.small()) {
-                if (quad == 0) {
-                    wait(&bar->small_full[smalls & 1], (uint32_t)(smalls >> 1) & 1u);
-                    if (live) own = bar->small_row[smalls & 3][r];
-                }
+            // The row's number and the keys it sees.  A small item's are read behind its first scores, which came after
+            // warp 19 had written them: a wait of the group's own for them might come two turns late, when its
+            // parity is that of a turn still to come.
+            int2 own = make_int2(0, 0);
+            const int small = smalls & 3;
+            if (w.small())
                 ++smalls;
-            } else if (live) {
+            else if (live)
                 own = find_row(plan, w, a.group, w.item.m0 + m);
-            }
             if (blocks == 0) {                 // a small tile's only block is the other group's
                 if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(-INFINITY, 0.0f);
                 continue;
             }
-            const int row = own.x, limit = own.y, head = w.item.kv_head * a.group + (w.item.m0 + m) % a.group;
+            const int head = w.item.kv_head * a.group + (w.item.m0 + m) % a.group;
             // Q rows into shared memory (each half 16 of the warp pair's 32), K-major with the 128-byte swizzle:
             // 16-byte chunk c of row r lies at chunk c ^ (r % 8).  Rows behind the tile keep what was there: their
             // lanes of S and O are never read.  All loads are in flight before the first store.
@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
                     const int from = mine + k * ROWS;
-                    const int r_from = __shfl_sync(0xFFFFFFFFu, row, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
+                    const int r_from = __shfl_sync(0xFFFFFFFFu, own.x, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
                     const T *src = reinterpret_cast<const T *>(a.q) + (long long)r_from * a.ldq + h_from + c * 8;
                     v[k] = make_uint4(0, 0, 0, 0);
                     if (from < warp_rows) v[k] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
@@ -855,7 +855,8 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                 if (!idle) {
                     __syncwarp();
                     fence_after();
-                    const int see = limit - block * kBlockKeys - half * 32;        // keys of this half that the row sees
+                    if (k == 0 && live && w.small()) own = bar->small_row[small][r];
+                    const int see = own.y - block * kBlockKeys - half * 32;        // keys of this half that the row sees
                     uint32_t s[32];
                     tmem_load32(s_addr + half * 32, s);
                     tmem_wait_load(s);
@@ -921,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const float inverse = 1.0f / sum;
             const bool strange = bar->strange[g] == i + 1;
             const int c0 = half * (HD / 2);
-            const long long to = (long long)row * a.ldo + (long long)head * HD + c0;
+            const long long to = (long long)own.x * a.ldo + (long long)head * HD + c0;
             // (Rolled, like the rescaling above: this code runs once an item, and fetching it took most of its time.)
             if (w.item.direct && !t.wide_out) {
 #pragma unroll 1
@@ -937,12 +938,12 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     uint32_t o[32];
                     tmem_load32(o_addr + c, o);
                     tmem_wait_load(o);
-                    if (live) store_output<TYPE, HD>(a, plan, w, o, inverse, row, head, record, c0 + c);
+                    if (live) store_output<TYPE, HD>(a, plan, w, o, inverse, own.x, head, record, c0 + c);
                     __syncwarp();
                 }
             }
             if (strange && live) {
-                const int keys = limit - w.seen_by_all(plan, a.group);
+                const int keys = own.y - w.seen_by_all(plan, a.group);
                 if (!w.item.direct)
                     put_back(bar, g, keys, c0, HD / 2, plan->part_o + ((record - r) * HD + c0 * kTileRows + r * 4), kTileRows * 4);
                 else if (a.out_f32)

@@ -584,3 +584,44 @@ def test_infinities_and_nan_in_masked_places(env, kind, dim, kv_heads, group, pa
             if kind != "f32":
                 tol = tol + torch.finfo(m.dtype).eps / 2 * size
             assert np.all(np.abs(got[r] - exact)[~strange] <= tol[~strange]), (layer, r)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,kv_heads,group", [(128, 4, 7), (64, 8, 1), (64, 2, 24), (128, 1, 25)])
+@pytest.mark.parametrize("n,prefix,own", [(64, 1536, 1), (64, 1536, 130), (200, 0, 1), (150, 0, 64), (40, 260, 70)])
+def test_many_short_segments_behind_long_ones(env, kind, dim, kv_heads, group, n, prefix, own):
+    """Launches whose CTAs work through many one-block items between tiles of a shared prefix, run again and again:
+    every run ends, with the same bits, and a sample of the rows is checked."""
+    torch = env[1]
+    page = 64
+    m = Model(env, kind, dim, kv_heads, group, page, pages=-(-prefix // page) + n * (own // page + 2) + 8, layers=1)
+    m.pool.copy_(m.normal(*m.pool.shape).to(m.dtype))         # contents enough: nothing is appended here
+    if prefix:
+        root = m.cache.create(1)
+        m.cache.extend(root, [prefix])
+        seqs = m.cache.fork(root * n)
+    else:
+        seqs = m.cache.create(n)
+    if own > 1:
+        m.cache.extend(seqs, [own - 1 - i % min(own - 1, 50) for i in range(n)])
+    m.batch.step(seqs, [1] * n)
+    q = m.normal(n, kv_heads * group * dim).to(m.dtype)
+    out = torch.empty_like(q)
+    m.batch.attention_device(0, q, out)
+    torch.cuda.synchronize()
+    for _ in range(30):
+        again = torch.empty_like(q)
+        m.batch.attention_device(0, q, again)
+        assert torch.equal(out, again)
+    rows = list(range(0, n, 13))
+    for s in rows:
+        m.tokens[seqs[s]] = m.read(seqs[s])
+    qd, got = q.double().cpu().numpy(), out.double().cpu().numpy()
+    half = torch.finfo(m.dtype).eps / 2
+    for s in rows:
+        k, v = m.tokens[seqs[s]][:, 0]
+        exact, size, scores = m.formula(qd[s].reshape(kv_heads, group, dim), k, v)
+        tol = (2 * (dim + 4) * scores[..., None] + 2 * (len(k) + 16)) * U * size
+        if kind != "f32":
+            tol = tol + half * size + half * np.abs(exact) + torch.finfo(m.dtype).smallest_normal * half * 2
+        assert np.all(np.abs(got[s].reshape(exact.shape) - exact) <= tol), s
