@@ -503,7 +503,7 @@ bool on_f32_tiles(const satori_batch *b) { return f32_attention_takes(b->pages->
 
 size_t record_rows(const satori_batch *b)
 {
-    return (size_t)(on_tensor_cores(b) ? tensor_record_rows() : on_f32_tiles(b) ? f32_record_rows() : generic_record_rows());
+    return (size_t)(on_tensor_cores(b) ? tensor_record_rows() : on_f32_tiles(b) ? f32_record_rows() : wide_record_rows());
 }
 
 int upload_plan(satori_batch *b)
@@ -640,7 +640,7 @@ extern "C" int satori_batch_create(satori_pages *pages, int q_heads, double rope
         else if (on_f32_tiles(b))
             f32_plan_shape(pages->head_dim, sms, b->shape);
         else
-            generic_plan_shape(pages->type, pages->head_dim, sms, b->shape);
+            wide_plan_shape(sms, b->shape);
         ++pages->users;
         *out = b;
         return SATORI_OK;
@@ -796,7 +796,7 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
     const int layer_block = layer * p->tables.pages() * 2 * p->kv_heads;
     cudaError_t e = on_tensor_cores(b) ? launch_tensor_attention(a, p->map, layer_block, p->ctx->stream)
                     : on_f32_tiles(b)  ? launch_f32_attention(a, p->map, layer_block, p->ctx->stream)
-                                       : launch_generic_attention(a, p->ctx->stream);
+                                       : launch_wide_attention(a, p->ctx->stream);
     if (e == cudaSuccess)
         e = launch_combine(a, (int)rows, b->shape.tile_m, on_tensor_cores(b), b->plan.head.merges,
                            p->ctx->sm_count, p->ctx->stream);

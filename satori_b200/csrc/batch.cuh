@@ -43,11 +43,11 @@ struct BatchAttn {
 };
 
 // The kernels' share of PlanShape: tile and block sizes, costs and the CTAs a GPU holds at once.
-void generic_plan_shape(int type, int head_dim, int sm_count, PlanShape &shape);
-int generic_record_rows();
-cudaError_t launch_generic_attention(const BatchAttn &a, cudaStream_t stream);
+void wide_plan_shape(int sm_count, PlanShape &shape);
+int wide_record_rows();
+cudaError_t launch_wide_attention(const BatchAttn &a, cudaStream_t stream);
 
-// The tensor-core kernel of 16-bit caches with heads of 64 or 128.
+// The tensor-core kernel of 16-bit caches with heads of up to 128.
 bool tensor_attention_takes(int type, int head_dim);
 void tensor_plan_shape(int sm_count, PlanShape &shape);
 int tensor_record_rows();
@@ -55,7 +55,7 @@ int tensor_record_rows();
 cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim, int page_tokens, unsigned long long blocks);
 cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, int layer_block, cudaStream_t stream);
 
-// The FP32 kernel of heads of 32, 64, 96 and 128.
+// The kernel of FP32 caches with heads of up to 128.
 bool f32_attention_takes(int type, int head_dim);
 void f32_plan_shape(int head_dim, int sm_count, PlanShape &shape);
 int f32_record_rows();

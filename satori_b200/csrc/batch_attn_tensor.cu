@@ -1,5 +1,6 @@
-// batch_attn_tensor.cu -- attention of a batch over a paged 16-bit cache on the 5th-generation tensor cores
-// (heads of 64 and 128).
+// batch_attn_tensor.cu -- attention of a batch over a paged 16-bit cache on the 5th-generation tensor cores, for
+// heads of up to 128.  HD below is 64 or 128: columns from the head's own size on are zeros (the copies of K and V
+// fill them in) and are neither read from q nor written.
 //
 // The same one pass over the keys as the FP32-unit kernel, as two matrix products per block of 64 keys:
 // S = Q K^T and O += P V with P = 2^(s - m).  One CTA per SM works through its share of the plan's items:
@@ -385,25 +386,27 @@ __device__ __noinline__ void put_back(const Barriers *bar, int g, int keys, int 
 }
 
 // 32 columns of a row's accumulator: its share of the partial record, or of an output with 16-byte accesses.
-template <int TYPE, int HD>
+template <int TYPE>
 __device__ __forceinline__ void store_output(const BatchAttn &a, const DevPlan *plan, const Work &w, uint32_t *o,
                                              float inverse, int row, int head, long long record, int c)
 {
     if (!w.item.direct) {
         // [column / 4][row]: the warp's rows are neighbours.
         const int r = (int)(record % kTileRows);
-        uint4 *dst = reinterpret_cast<uint4 *>(plan->part_o) + (record - r) * (HD / 4) + (c / 4) * kTileRows + r;
+        uint4 *dst = reinterpret_cast<uint4 *>(plan->part_o) + (record - r) * (a.head_dim / 4) + (c / 4) * kTileRows + r;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) dst[e / 4 * kTileRows] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (int e = 0; e < 32; e += 4)
+            if (c + e < a.head_dim) dst[e / 4 * kTileRows] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         return;
     }
-    const long long to = (long long)row * a.ldo + (long long)head * HD + c;
+    const long long to = (long long)row * a.ldo + (long long)head * a.head_dim + c;
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inverse);
     if (a.out_f32) {
         uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<float *>(a.out) + to);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) dst[e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (int e = 0; e < 32; e += 4)
+            if (c + e < a.head_dim) dst[e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     } else {
         uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<typename Elem<TYPE>::type *>(a.out) + to);
 #pragma unroll
@@ -413,16 +416,16 @@ __device__ __forceinline__ void store_output(const BatchAttn &a, const DevPlan *
             v.y = pack2<TYPE>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
             v.z = pack2<TYPE>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
             v.w = pack2<TYPE>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
-            dst[e / 8] = v;
+            if (c + e < a.head_dim) dst[e / 8] = v;
         }
     }
 }
 
-// 16 columns of an output row at any address.
+// Up to 16 columns of an output row at any address.
 template <int TYPE>
-__device__ __noinline__ void store_anywhere(const BatchAttn &a, const uint32_t *o, float inverse, long long to)
+__device__ __noinline__ void store_anywhere(const BatchAttn &a, const uint32_t *o, float inverse, long long to, int n)
 {
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < min(16, n); ++e) {
         const float v = __uint_as_float(o[e]) * inverse;
         if (a.out_f32)
             reinterpret_cast<float *>(a.out)[to + e] = v;
@@ -465,7 +468,7 @@ struct Loads {
             const uint32_t to = stages + ring.stage * L::kTile;
             const int boxes = j == n - 1 ? last_boxes : PER, block0 = first_block + kv * t.a.kv_heads;
             mbar_expect_tx(full, (uint32_t)(boxes * kBox * HD * 2));
-            if (PER == 1) {
+            if (PER == 1 && t.a.head_dim % 64 == 0) {
                 tma_load_4d(to, &map, (key0 + j * kBlockKeys) & mask, block0 + id[0] * page_blocks, full);
             } else {
 #pragma unroll
@@ -473,7 +476,8 @@ struct Loads {
                     if (b < boxes)
 #pragma unroll
                         for (int half = 0; half < HD / 64; ++half)
-                            tma_load_3d(to + half * L::kHalf + b * kBox * 128, &map, half * 64, 0, block0 + id[b] * page_blocks, full);
+                            tma_load_3d(to + half * L::kHalf + b * kBox * 128, &map, half * 64,
+                                        PER == 1 ? (key0 + j * kBlockKeys) & mask : 0, block0 + id[b] * page_blocks, full);
             }
             ring.next();
             ++units;
@@ -607,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const int b = smalls & 1, m = w.item.m0 + lane;
             const int2 own = lane < w.item.m ? find_row(plan, w, a.group, m) : make_int2(0, 0);
             const int row = own.x;
-            const int q_head = (w.item.kv_head * a.group + m % a.group) * HD, c = lane % PER_ROW;
+            const int q_head = (w.item.kv_head * a.group + m % a.group) * a.head_dim, c = lane % PER_ROW;
             uint8_t *q_tile = small_q + b * L::kSmall;
             const bool free = __all_sync(0xFFFFFFFFu, wait(&bar->small_free[b], (uint32_t)((smalls >> 1) & 1) ^ 1u));
             if (!free) return false;
@@ -622,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     const int r_from = __shfl_sync(0xFFFFFFFFu, row, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
                     const T *src = reinterpret_cast<const T *>(a.q) + (long long)r_from * a.ldq + h_from + c * 8;
                     v[e] = make_uint4(0, 0, 0, 0);
-                    if (from < w.item.m) v[e] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
+                    if (from < w.item.m && c * 8 < a.head_dim) v[e] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
                 }
 #pragma unroll
                 for (int e = 0; e < BATCH; ++e) {
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const int warp_rows = min(32, w.item.m - (m - lane));          // live rows of the warp pair
             if (half * 16 < warp_rows && !w.small()) {
                 constexpr int PER_ROW = HD / 8, ROWS = 32 / PER_ROW, STEPS = 16 / ROWS;
-                const int c = lane % PER_ROW, mine = half * 16 + lane / PER_ROW, q_head = head * HD;
+                const int c = lane % PER_ROW, mine = half * 16 + lane / PER_ROW, q_head = head * a.head_dim;
                 uint4 v[STEPS];
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
@@ -832,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     const int r_from = __shfl_sync(0xFFFFFFFFu, own.x, from), h_from = __shfl_sync(0xFFFFFFFFu, q_head, from);
                     const T *src = reinterpret_cast<const T *>(a.q) + (long long)r_from * a.ldq + h_from + c * 8;
                     v[k] = make_uint4(0, 0, 0, 0);
-                    if (from < warp_rows) v[k] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
+                    if (from < warp_rows && c * 8 < a.head_dim) v[k] = t.wide_q ? __ldg(reinterpret_cast<const uint4 *>(src)) : load_unaligned(src);
                 }
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
@@ -922,14 +926,14 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
             const float inverse = 1.0f / sum;
             const bool strange = bar->strange[g] == i + 1;
             const int c0 = half * (HD / 2);
-            const long long to = (long long)own.x * a.ldo + (long long)head * HD + c0;
+            const long long to = (long long)own.x * a.ldo + (long long)head * a.head_dim + c0;
             // (Rolled, like the rescaling above: this code runs once an item, and fetching it took most of its time.)
             if (w.item.direct && !t.wide_out) {
 #pragma unroll 1
                 for (int c = 0; c < HD / 2; c += 16) {
                     uint32_t o[16];
                     tmem_load16(o_addr + c, o);
-                    if (live) store_anywhere<TYPE>(a, o, inverse, to + c);
+                    if (live) store_anywhere<TYPE>(a, o, inverse, to + c, a.head_dim - c0 - c);
                     __syncwarp();
                 }
             } else {
@@ -938,18 +942,18 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     uint32_t o[32];
                     tmem_load32(o_addr + c, o);
                     tmem_wait_load(o);
-                    if (live) store_output<TYPE, HD>(a, plan, w, o, inverse, own.x, head, record, c0 + c);
+                    if (live) store_output<TYPE>(a, plan, w, o, inverse, own.x, head, record, c0 + c);
                     __syncwarp();
                 }
             }
             if (strange && live) {
-                const int keys = own.y - w.seen_by_all(plan, a.group);
+                const int keys = own.y - w.seen_by_all(plan, a.group), n = min(HD / 2, a.head_dim - c0);
                 if (!w.item.direct)
-                    put_back(bar, g, keys, c0, HD / 2, plan->part_o + ((record - r) * HD + c0 * kTileRows + r * 4), kTileRows * 4);
+                    put_back(bar, g, keys, c0, n, plan->part_o + ((record - r) * a.head_dim + c0 * kTileRows + r * 4), kTileRows * 4);
                 else if (a.out_f32)
-                    put_back(bar, g, keys, c0, HD / 2, reinterpret_cast<float *>(a.out) + to, 4);
+                    put_back(bar, g, keys, c0, n, reinterpret_cast<float *>(a.out) + to, 4);
                 else
-                    put_back(bar, g, keys, c0, HD / 2, reinterpret_cast<T *>(a.out) + to, 4);
+                    put_back(bar, g, keys, c0, n, reinterpret_cast<T *>(a.out) + to, 4);
             }
             if (live && half == 0 && !w.item.direct) plan->part_ml[record] = make_float2(ref, sum);
             // The next item's first O overwrites this one after this group's next p_ready, so these loads are done.
@@ -975,7 +979,7 @@ cudaError_t launch(const TensorArgs &t, const CUtensorMap &map, cudaStream_t str
 
 bool tensor_attention_takes(int type, int head_dim)
 {
-    return (type == SATORI_F16 || type == SATORI_BF16) && (head_dim == 64 || head_dim == 128);
+    return (type == SATORI_F16 || type == SATORI_BF16) && head_dim <= 128;
 }
 
 void tensor_plan_shape(int sm_count, PlanShape &shape)
@@ -1015,16 +1019,16 @@ cudaError_t make_page_map(CUtensorMap *map, void *memory, int type, int head_dim
     const cuuint64_t row = (cuuint64_t)head_dim * size, block = row * page_tokens;
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     CUresult r;
-    if (page_tokens >= kBlockKeys) {       // [block][part][token][columns]: a box is a block of keys, part by part
+    if (page_tokens >= kBlockKeys && head_dim % columns == 0) {        // [block][part][token][columns]: a box is a block of keys, part by part
         const cuuint64_t dims[4] = {columns, (cuuint64_t)page_tokens, (cuuint64_t)head_dim / columns, (cuuint64_t)blocks};
         const cuuint64_t strides[3] = {row, 128, block};
         const cuuint32_t box[4] = {columns, kBlockKeys, (cuuint32_t)head_dim / columns, 1};
         r = reinterpret_cast<EncodeTiled>(f)(map, kind, 4, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    } else {                               // [block][token][dim]: a box is 128 bytes of a page's rows
+    } else {                               // [block][token][dim]: a box is 128 bytes (zeros behind the head) of a page's rows
         const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)page_tokens, (cuuint64_t)blocks}, strides[2] = {row, block};
-        const cuuint32_t box[3] = {columns, (cuuint32_t)page_tokens, 1};
+        const cuuint32_t box[3] = {columns, std::min<cuuint32_t>(page_tokens, kBlockKeys), 1};
         r = reinterpret_cast<EncodeTiled>(f)(map, kind, 3, memory, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1038,8 +1042,8 @@ cudaError_t launch_tensor_attention(const BatchAttn &a, const CUtensorMap &map, 
     t.wide_q = (uintptr_t)a.q % 16 == 0 && a.ldq % 8 == 0;
     t.wide_out = (uintptr_t)a.out % 16 == 0 && a.ldo * (a.out_f32 ? 4 : 2) % 16 == 0;
     if (a.type == SATORI_F16)
-        return a.head_dim == 64 ? launch<SATORI_F16, 64>(t, map, stream) : launch<SATORI_F16, 128>(t, map, stream);
-    return a.head_dim == 64 ? launch<SATORI_BF16, 64>(t, map, stream) : launch<SATORI_BF16, 128>(t, map, stream);
+        return a.head_dim <= 64 ? launch<SATORI_F16, 64>(t, map, stream) : launch<SATORI_F16, 128>(t, map, stream);
+    return a.head_dim <= 64 ? launch<SATORI_BF16, 64>(t, map, stream) : launch<SATORI_BF16, 128>(t, map, stream);
 }
 
 }  // namespace satori

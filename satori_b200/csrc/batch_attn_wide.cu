@@ -1,5 +1,5 @@
-// batch_attn_generic.cu -- attention of a batch over a paged cache on the FP32 units, for the head sizes that
-// neither the tensor-core kernel (16-bit caches, 64 and 128) nor the FP32 one (multiples of 32 up to 128) takes.
+// batch_attn_wide.cu -- attention of a batch over a paged cache with heads of more than 128 columns, on the FP32
+// units.
 //
 // For a query row r and its visible keys t: out_r = sum_t p_rt v_t / sum_t p_rt, p_rt = 2^(s_rt - m_r),
 // s_rt = (q_r . k_t) log2(e) / sqrt(d), m_r the running maximum.  One pass over the keys; the running
@@ -10,7 +10,7 @@
 //  * at most 8 rows (the query heads of one KV head of one request): each warp walks 8 keys at a time on
 //    its own, K and V straight from global memory into registers; HBM bounds it.
 //  * up to 64 rows (a shared prefix, a prompt): 64 x 64 tiles through shared memory, 4 x 4 scores and
-//    4 x HD/16 outputs per thread; the FP32 units bound it.
+//    4 x 16 outputs per thread; the FP32 units bound it.
 #include "batch.cuh"
 #include "common.cuh"
 
@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kTileM = 64, kBlock = 64, kFewRows = 8;
+constexpr int HD = 256;                                // columns; those behind a smaller head's own are zeros
 
 __device__ __forceinline__ float log2_exp(float x) { return exp2f(x); }
 
@@ -46,7 +47,7 @@ __device__ __forceinline__ void unpack16(uint4 v, float *f)
     }
 }
 
-template <int TYPE, int HD>
+template <int TYPE>
 struct Smem {
     float q[kTileM][HD + 4];
     union {
@@ -63,9 +64,9 @@ struct Smem {
 };
 
 // The item's rows: query values scaled by log2(e) / sqrt(d) are not rounded again (FP32), limits, indices.
-template <int TYPE, int HD>
+template <int TYPE>
 __device__ void load_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
-                          Smem<TYPE, HD> &sm, int rows)
+                          Smem<TYPE> &sm, int rows)
 {
     typedef typename Elem<TYPE>::type T;
     const PlanRow *seg_rows = plan_array<PlanRow>(plan, plan->seg_rows) + item.row_off;
@@ -119,15 +120,15 @@ __device__ __forceinline__ void store_out(const BatchAttn &a, int row, int head,
 }
 
 // ---- few rows: one warp, 8 keys at a time
-template <int TYPE, int HD>
+template <int TYPE>
 __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
-                         const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
+                         const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE> &sm)
 {
     typedef typename Elem<TYPE>::type T;
     constexpr int EV = 16 / sizeof(T);                 // elements of a 16-byte chunk
     constexpr int CH = HD / EV / 4;                    // chunks of a K row per lane (4 lanes share a key)
     constexpr int VW = HD / 32;                        // V elements per lane
-    load_rows<TYPE, HD>(a, plan, item, sm, kFewRows);
+    load_rows<TYPE>(a, plan, item, sm, kFewRows);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = lane & 3;
     const int key0 = item.block0 * kBlock, key1 = min(key0 + item.blocks * kBlock, item.keys);
     const int chunks = a.head_dim / EV;
@@ -273,14 +274,14 @@ __device__ void few_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem
 }
 
 // ---- many rows: 64 x 64 tiles
-template <int TYPE, int HD>
+template <int TYPE>
 __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanItem &item,
-                          const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE, HD> &sm)
+                          const KeyRows<typename Elem<TYPE>::type> &rows, Smem<TYPE> &sm)
 {
     typedef typename Elem<TYPE>::type T;
     constexpr int EV = 16 / sizeof(T);
     constexpr int OC = HD / 64;                        // float4 groups of output columns per thread
-    load_rows<TYPE, HD>(a, plan, item, sm, kTileM);
+    load_rows<TYPE>(a, plan, item, sm, kTileM);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int chunks = a.head_dim / EV;
     float m[4], l[4], acc[4][OC * 4];
@@ -410,12 +411,12 @@ __device__ void many_rows(const BatchAttn &a, const DevPlan *plan, const PlanIte
     __syncthreads();
 }
 
-template <int TYPE, int HD>
-__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) generic_attention_kernel(const BatchAttn a)
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads, 1) wide_attention_kernel(const BatchAttn a)
 {
     typedef typename Elem<TYPE>::type T;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    Smem<TYPE, HD> &sm = *reinterpret_cast<Smem<TYPE, HD> *>(smem_raw);
+    Smem<TYPE> &sm = *reinterpret_cast<Smem<TYPE> *>(smem_raw);
     pdl_launch_dependents();
     pdl_wait();
     const DevPlan *plan = a.plan;
@@ -432,52 +433,43 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) generic_attention
         rows.pages = plan_array<int>(plan, plan->pages) + item.page_off;
         rows.head_off = (long long)item.kv_head * a.page_tokens * a.head_dim;
         if (item.m <= kFewRows)
-            few_rows<TYPE, HD>(a, plan, item, rows, sm);
+            few_rows<TYPE>(a, plan, item, rows, sm);
         else
-            many_rows<TYPE, HD>(a, plan, item, rows, sm);
+            many_rows<TYPE>(a, plan, item, rows, sm);
     }
 }
 
-template <int TYPE, int HD>
+template <int TYPE>
 cudaError_t launch(const BatchAttn &a, cudaStream_t stream)
 {
-    cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(&generic_attention_kernel<TYPE, HD>), sizeof(Smem<TYPE, HD>));
+    cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(&wide_attention_kernel<TYPE>), sizeof(Smem<TYPE>));
     if (e != cudaSuccess) return e;
-    return launch_overlapped(generic_attention_kernel<TYPE, HD>, dim3(a.ctas), kThreads, sizeof(Smem<TYPE, HD>), stream, a);
-}
-
-template <int TYPE>
-cudaError_t launch_type(const BatchAttn &a, cudaStream_t stream)
-{
-    if (a.head_dim <= 64) return launch<TYPE, 64>(a, stream);
-    if (a.head_dim <= 128) return launch<TYPE, 128>(a, stream);
-    return launch<TYPE, 256>(a, stream);
+    return launch_overlapped(wide_attention_kernel<TYPE>, dim3(a.ctas), kThreads, sizeof(Smem<TYPE>), stream, a);
 }
 
 }  // namespace
 
-void generic_plan_shape(int type, int head_dim, int sm_count, PlanShape &shape)
+void wide_plan_shape(int sm_count, PlanShape &shape)
 {
     shape.tile_m = kTileM;
     shape.block = kBlock;
-    shape.ctas = sm_count * (head_dim <= 128 ? 2 : 1);
+    shape.ctas = sm_count;
     shape.solo_m = kFewRows;
     // A block of 64 keys costs the small path about half of what the 64-row path needs.
     shape.solo_cost = 2;
     shape.pair_cost = 4;
     shape.item_cost = 2;
     shape.slots_per_item = 1;
-    (void)type;
 }
 
-int generic_record_rows() { return kTileM; }
+int wide_record_rows() { return kTileM; }
 
-cudaError_t launch_generic_attention(const BatchAttn &a, cudaStream_t stream)
+cudaError_t launch_wide_attention(const BatchAttn &a, cudaStream_t stream)
 {
     switch (a.type) {
-    case SATORI_F32: return launch_type<SATORI_F32>(a, stream);
-    case SATORI_F16: return launch_type<SATORI_F16>(a, stream);
-    default: return launch_type<SATORI_BF16>(a, stream);
+    case SATORI_F32: return launch<SATORI_F32>(a, stream);
+    case SATORI_F16: return launch<SATORI_F16>(a, stream);
+    default: return launch<SATORI_BF16>(a, stream);
     }
 }
 

@@ -625,3 +625,19 @@ def test_many_short_segments_behind_long_ones(env, kind, dim, kv_heads, group, n
         if kind != "f32":
             tol = tol + half * size + half * np.abs(exact) + torch.finfo(m.dtype).smallest_normal * half * 2
         assert np.all(np.abs(got[s].reshape(exact.shape) - exact) <= tol), s
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,kv_heads,group", [(16, 2, 3), (40, 1, 8), (80, 2, 1), (104, 2, 5), (120, 1, 12), (136, 2, 4)])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_heads_of_any_size(env, kind, dim, kv_heads, group, page):
+    """Heads whose rows are no whole number of 128 bytes: single tokens, prompts and a shared prefix."""
+    m = Model(env, kind, dim, kv_heads, group, page, layers=2, rope=1e4 if dim % 16 == 0 else 0.0, seed=dim)
+    root = m.new()
+    m.step([root], [300])
+    seqs = m.fork([root] * 3, [300, 290, 70]) + [m.new()]
+    counts = [1, 2, 90, 60]
+    m.check(seqs, counts, m.step(seqs, counts))
+    q = m.step(seqs, [1] * 4)
+    m.check(seqs, [1] * 4, q, out_f32=True)
+    m.check(seqs, [1] * 4, q, strided=True)
