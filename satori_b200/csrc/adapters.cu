@@ -27,6 +27,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <array>
+#include <climits>
 
 using namespace satori;
 namespace cg = cooperative_groups;
@@ -57,6 +59,7 @@ struct AdapterArgs {
     const float *x, *base;
     float *out;
     long long ldx, ldbase, ldo;
+    int splits;                                // clusters that share an item's outputs
     int rows, cols, cols32;                    // output rows, columns, columns rounded up to 32
     int wide_x, wide_out;                      // 16-byte accesses are possible
     unsigned *err;
@@ -71,7 +74,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y)
 
 // (x, y) cut into N packed bf16 parts; each residual is exact in FP32.
 template <int N>
-__device__ __forceinline__ void split(float x, float y, uint32_t *part)
+__device__ __forceinline__ void split_values(float x, float y, uint32_t *part)
 {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -112,7 +115,7 @@ __device__ __forceinline__ void weight_parts(const uint32_t *raw, uint32_t (*par
             else
                 f = make_float2(__uint_as_float(raw[2 * h]), __uint_as_float(raw[2 * h + 1]));
             uint32_t p[Weights<TYPE>::kParts];
-            split<Weights<TYPE>::kParts>(f.x, f.y, p);
+            split_values<Weights<TYPE>::kParts>(f.x, f.y, p);
 #pragma unroll
             for (int i = 0; i < Weights<TYPE>::kParts; ++i) part[i][h] = p[i];
         }
@@ -179,6 +182,25 @@ __device__ __forceinline__ void fragment_place(int rank, int p, int r, int &step
     at = 2 * (p % 8 * 4 + (both ? in / 8 : in / 4)) + p / 8 % 2;
 }
 
+// The sum over the cluster of four values at the same place in every CTA.  (A call: in line its eight loads in flight
+// took registers that the products then spilled.)
+__device__ __noinline__ float4 cluster_sum(float *at, int ctas)
+{
+    cg::cluster_group cluster = cg::this_cluster();
+    float4 v[kMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) v[c] = c < ctas ? *reinterpret_cast<const float4 *>(cluster.map_shared_rank(at, c)) : make_float4(0, 0, 0, 0);
+    float4 sum = v[0];
+#pragma unroll
+    for (int c = 1; c < kMaxCluster; ++c) {
+        sum.x += v[c].x;
+        sum.y += v[c].y;
+        sum.z += v[c].z;
+        sum.w += v[c].w;
+    }
+    return sum;
+}
+
 template <int TYPE, int RM>
 __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113 * 1024 ? 2 : 1) adapter_kernel(const AdapterArgs a)
 {
@@ -202,8 +224,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
     const RowItem *list = reinterpret_cast<const RowItem *>(plan + a.plan->item_off);
     const int *rows = plan + a.plan->rows_off;
 
-    for (int it = blockIdx.x / ctas; it < items; it += gridDim.x / ctas) {
-        const RowItem item = list[it];
+    for (int unit = blockIdx.x / ctas; unit < items * a.splits; unit += gridDim.x / ctas) {
+        const RowItem item = list[unit / a.splits];
+        const int split = unit % a.splits;     // its share of the outputs; t is every share's own
         SlotDesc slot = {};
         if (item.slot >= 0) slot = a.slots[item.slot];
         const int rank = slot.rank16, tiles = (item.rows + 15) / 16;
@@ -262,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     uint32_t p[3];
-                                    split<3>(x[h][4 * s + 2 * e], x[h][4 * s + 2 * e + 1], p);
+                                    split_values<3>(x[h][4 * s + 2 * e], x[h][4 * s + 2 * e + 1], p);
 #pragma unroll
                                     for (int c = 0; c < 3; ++c) xa[c][2 * e + h] = p[c];
                                 }
@@ -285,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
                 }
             }
             __syncthreads();
-            for (int e = tid; e < tiles * 4 * rank; e += kThreads) {
+            for (int e = tid; e < item.rows * (rank / 4); e += kThreads) {
                 const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
                 float4 sum = make_float4(0, 0, 0, 0);
                 for (int w = p / 16; w < kWarps; w += shares) {
@@ -298,37 +321,31 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
                 *reinterpret_cast<float4 *>(&sm.t[p][r]) = sum;
             }
             cluster.sync();
-            // Each CTA adds its share of t over the cluster, scales it, cuts it into bf16 parts and hands them to all.
-            for (int e = cta * kThreads + tid; e < tiles * 4 * rank; e += ctas * kThreads) {
+            // Each CTA adds t over the cluster, scales it and cuts it into bf16 parts.  (Adding a share each and handing
+            // the parts round took longer: 48 remote stores a value, one after the other.)  Rows behind the item's
+            // keep what was there: so do the outputs nobody reads.
+            for (int e = tid; e < item.rows * (rank / 4); e += kThreads) {
                 const int p = e / (rank / 4), r = 4 * (e % (rank / 4));
-                float4 sum = make_float4(0, 0, 0, 0);
-                for (int c = 0; c < ctas; ++c) {
-                    const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sm.t[p][r], c));
-                    sum.x += v.x;
-                    sum.y += v.y;
-                    sum.z += v.z;
-                    sum.w += v.w;
-                }
+                float4 sum = cluster_sum(&sm.t[p][r], ctas);
                 sum.x *= slot.scale;
                 sum.y *= slot.scale;
                 sum.z *= slot.scale;
                 sum.w *= slot.scale;
                 if (TYPE == SATORI_F16) {
-                    for (int c = 0; c < ctas; ++c) *reinterpret_cast<float4 *>(cluster.map_shared_rank(&sm.whole[p][r], c)) = sum;
+                    *reinterpret_cast<float4 *>(&sm.whole[p][r]) = sum;
                     continue;
                 }
                 uint32_t lo[3], hi[3];
-                split<3>(sum.x, sum.y, lo);
-                split<3>(sum.z, sum.w, hi);
+                split_values<3>(sum.x, sum.y, lo);
+                split_values<3>(sum.z, sum.w, hi);
                 int step, at;
                 fragment_place(rank, p, r, step, at);
-                for (int c = 0; c < ctas; ++c)
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) {
-                        uint32_t *to = reinterpret_cast<uint32_t *>(cluster.map_shared_rank(&sm.parts[step][k % Smem::kParts][p / 16][at >> 1], c)) + (at & 1);
-                        to[0] = lo[k];
-                        to[2] = hi[k];
-                    }
+                for (int k = 0; k < 3; ++k) {
+                    uint32_t *to = reinterpret_cast<uint32_t *>(&sm.parts[step][k % Smem::kParts][p / 16][at >> 1]) + (at & 1);
+                    to[0] = lo[k];
+                    to[2] = hi[k];
+                }
             }
             // From here on nobody reads another CTA's t, whose place the ring takes; and the parts are only written
             // again after the next item's first synchronisation, which every CTA of the cluster comes to.
@@ -370,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
         // number of 16s with 4 a lane.
         constexpr int C32 = 1;                 // runs of 32 ranks held at once
         const int run_bytes = 32 * rank * W::kBytes, slots = rank ? min(Smem::kSlots, Smem::kRing / run_bytes) : 1;
-        const int runs = (a.rows + 31) / 32, stride = ctas * kWarps, first = cta * kWarps + warp;
+        const int runs = (a.rows + 31) / 32, stride = a.splits * ctas * kWarps, first = (split * ctas + cta) * kWarps + warp;
         auto fetch = [&](int run, int s) {
             const int bytes = min(32, a.rows - run * 32) * rank * W::kBytes;
             mbar_expect_tx(&sm.full[warp][s], (uint32_t)bytes);
@@ -513,18 +530,59 @@ struct satori_adapter_rows {
 
 namespace {
 
+// How many clusters of each size up to 8 run at once.  The SMs of a GPC hold whole clusters, so it's less than the
+// CTAs' number divided by the cluster's.
+template <typename Kernel>
+std::array<int, kMaxCluster + 1> resident_clusters(Kernel kernel, size_t smem, int sm_count)
+{
+    std::array<int, kMaxCluster + 1> got = {};
+    for (int size = 1; size <= kMaxCluster; ++size) {
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)size;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(sm_count * 8 * size));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&got[size], kernel, &cfg) != cudaSuccess || got[size] < 1) {
+            cudaGetLastError();
+            got[size] = std::max(1, sm_count / size);
+        }
+    }
+    return got;
+}
+
 template <int TYPE, int RM>
-cudaError_t launch_variant(const AdapterArgs &a, int items, int sm_count, cudaStream_t stream)
+cudaError_t launch_variant(AdapterArgs a, int items, int sm_count, cudaStream_t stream)
 {
     auto kernel = adapter_kernel<TYPE, RM>;
     const size_t smem = sizeof(AdapterSmem<TYPE, RM>);
     cudaError_t e = opt_in_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
-    // The largest cluster with which all items are resident at once (two CTAs an SM): few items are spread over
-    // many SMs, many items exchange less, and there is no second wave.
-    int cluster = kMaxCluster;
-    while (cluster > 1 && items * cluster > 2 * sm_count) cluster /= 2;
-    const int clusters = std::max(1, std::min(items, 8 * sm_count / cluster));
+    // All items are resident at once where that can be: a second wave costs as much as the first (2400 rows of one
+    // slot, rank 64, 8960 outputs, in 38 items: 97 us on clusters of 4, 73 on 6).  An item may have several clusters, of which all
+    // compute t and each writes a share of the outputs.  Of the clusters' sizes that fit, the one whose warps have
+    // the fewest runs of 32, of columns for t and (twice the work) of outputs, in turn: one slot's 22 rows, rank 64,
+    // 8960 outputs in FP32 take 13 us, with one cluster an item 28.8.
+    static const std::array<int, kMaxCluster + 1> resident = resident_clusters(kernel, smem, sm_count);
+    const int column_runs = a.cols32 / 32, runs = (a.rows + 31) / 32;
+    auto turns = [](int n, int among) { return (n + among - 1) / among; };
+    int cluster = 1, least = INT_MAX;
+    a.splits = 1;
+    for (int size = kMaxCluster; size >= 1; --size) {
+        if (items > resident[size]) continue;
+        const int most = resident[size] / items, each = turns(runs, size * kWarps * most);
+        const int cost = turns(column_runs, size * kWarps) + 2 * each;
+        if (cost < least) {
+            least = cost;
+            cluster = size;
+            a.splits = turns(runs, size * kWarps * each);
+        }
+    }
+    const int clusters = std::max(1, std::min(items * a.splits, 8 * sm_count / cluster));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * cluster));
     cfg.blockDim = dim3(kThreads);
