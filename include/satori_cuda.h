@@ -239,7 +239,9 @@ SATORI_API int satori_batch_create(satori_pages *p, int q_heads, double rope_bas
  * holds for all layers, until one of its sequences changes otherwise (then the calls below are refused).
  * It is uploaded on the context's stream behind an address that stays the same while the plan fits
  * (satori_batch_info's `reallocations`), so captured append and attention launches may be replayed after
- * the next step when their row buffers are large enough for its rows; a step itself cannot be captured. */
+ * the next step when their row buffers are large enough for its rows; a step itself cannot be captured.  All
+ * calls and replays of a batch run one after another on the context's stream: its layers share the plan and the
+ * space for partial results. */
 SATORI_API int satori_batch_step(satori_batch *b, int n, const int *seqs, const int *counts);
 /* The step's rows, the segments its keys fall into (a run of pages that sequences share is one), its work
  * items, and how often the plan's address has changed. */
@@ -247,14 +249,16 @@ SATORI_API int satori_batch_info(const satori_batch *b, int *rows, int *segments
 /* DenseForward.Step's RopeHalf and cache append (DenseForward.cs:135-141) for every row of the step: k is
  * rotated at its row's position and stored with v in the layer's pages, q (NULL: none) is rotated into q_out
  * [rows][q_heads * head_dim].  Device pointers on the context's stream; inputs are float32 or of the cache's
- * type (in_type), rows ldq / ldk / ldv elements apart (0: packed); q_out has the cache's type.  The rotation
- * is FP64 like RopeHalf's, rounded once. */
+ * type (in_type), rows ldq / ldk / ldv elements apart (0: packed); q_out has the cache's type, and overlaps no
+ * input but may be a packed q of its type itself.  The rotation is FP64 like RopeHalf's, rounded once. */
 SATORI_API int satori_batch_append_device(satori_batch *b, int layer, int in_type, const void *q, long long ldq,
                                           const void *k, long long ldk, const void *v, long long ldv, void *q_out);
 /* TransformerOps.GroupedAttention (TransformerOps.cs:140-179) for every row of the step over its sequence's
  * tokens up to its own position: q [rows][q_heads * head_dim] of the cache's type, rotated and ldq elements
- * apart (0: packed) -> out of the cache's type or float32 (out_type), ldo apart.  Keys that several of the
- * step's sequences share are read once for all their rows.  Scores, sums and accumulators are FP32. */
+ * apart (0: packed) -> out of the cache's type or float32 (out_type), ldo apart, beside q.  Keys that several of the
+ * step's sequences share are read once for all their rows.  Scores, sums and accumulators are FP32; beside 16-bit
+ * pages and heads of up to 128 the softmax weights are rounded to their type before they meet V.  What lies in K
+ * and V of later tokens, infinities and NaN included, does not reach a row. */
 SATORI_API int satori_batch_attention_device(satori_batch *b, int layer, const void *q, long long ldq, void *out,
                                              long long ldo, int out_type);
 SATORI_API int satori_batch_destroy(satori_batch *b);
@@ -280,7 +284,8 @@ SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
 SATORI_API int satori_adapter_rows_destroy(satori_adapter_rows *r);
 /* out[p] = base[p] + scale * B (A x[p]) for the assigned rows: device pointers on the context's stream, x
  * rows of cols floats ldx apart, base and out rows of `rows` floats (0: packed).  out may be base itself and
- * must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits, FP32 sums. */
+ * must not overlap anything else.  FP32 accuracy: weights exact, x to 24 bits, A x to 24 bits (beside fp16 weights
+ * 22), FP32 sums; an infinity in x may come out as NaN in its own row. */
 SATORI_API int satori_adapters_apply_device(satori_adapters *s, const satori_adapter_rows *r, const float *x,
                                             long long ldx, const float *base, long long ldbase, float *out,
                                             long long ldo);

@@ -609,14 +609,6 @@ cudaError_t launch_adapters(const AdapterArgs &a, int rank, int items, int sm_co
     return launch_variant<TYPE, 128>(a, items, sm_count, stream);
 }
 
-bool overlap(const void *a, size_t na, const void *b, size_t nb)
-{
-    const char *x = (const char *)a, *y = (const char *)b;
-    return x < y + nb && y < x + na;
-}
-
-size_t span(long long rows, long long ld, long long width) { return (size_t)((rows - 1) * ld + width) * 4; }
-
 }  // namespace
 
 extern "C" int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int slots, int max_rank, int type,
@@ -804,8 +796,9 @@ extern "C" int satori_adapters_apply_device(satori_adapters *s, const satori_ada
     if (ldx < s->cols || ldbase < s->rows || ldo < s->rows)
         return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
     if (((uintptr_t)x | (uintptr_t)base | (uintptr_t)out) % 4) return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
-    const size_t nx = span(r->rows, ldx, s->cols), nb = span(r->rows, ldbase, s->rows), no = span(r->rows, ldo, s->rows);
-    if (overlap(out, no, x, nx) || (overlap(out, no, base, nb) && !(out == base && ldo == ldbase)))
+    const long long width = s->rows * 4ll;
+    if (rows_overlap(out, ldo * 4, width, x, ldx * 4, s->cols * 4ll, r->rows) ||
+        (rows_overlap(out, ldo * 4, width, base, ldbase * 4, width, r->rows) && !(out == base && ldo == ldbase)))
         return set_error(SATORI_ERR_ARGUMENT, "output must not overlap input (or be base itself)");
     DeviceScope scope(s->ctx->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
@@ -847,7 +840,7 @@ extern "C" int satori_matrix_execute_adapted_device(satori_matrix *m, satori_ada
     if (r->top_slot >= s->slots)
         return set_error(SATORI_ERR_ARGUMENT, "slot %d is assigned; these adapters have %d", r->top_slot, s->slots);
     if (r->rows == 0) return SATORI_OK;
-    if (dx && dy && overlap(dy, span(r->rows, m->rows, m->rows), dx, span(r->rows, m->cols, m->cols)))
+    if (dx && dy && rows_overlap(dy, m->rows * 4ll, m->rows * 4ll, dx, m->cols * 4ll, m->cols * 4ll, r->rows))
         return set_error(SATORI_ERR_ARGUMENT, "output must not overlap input");
     DeviceScope scope(m->ctx->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");

@@ -723,6 +723,10 @@ extern "C" int satori_batch_append_device(satori_batch *b, int layer, int in_typ
     const size_t es = type_size(in_type), os = type_size(p->type);
     if ((uintptr_t)k % es || (uintptr_t)v % es || (uintptr_t)q % es || (uintptr_t)q_out % os)
         return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
+    const long long n = b->plan.head.rows;
+    if (q && ((rows_overlap(q_out, qw * os, qw * os, q, ldq * es, qw * es, n) && !(q_out == q && ldq == qw && in_type == p->type)) ||
+              rows_overlap(q_out, qw * os, qw * os, k, ldk * es, kvw * es, n) || rows_overlap(q_out, qw * os, qw * os, v, ldv * es, kvw * es, n)))
+        return set_error(SATORI_ERR_ARGUMENT, "q_out must not overlap an input (or be the packed q itself)");
     DeviceScope scope(p->ctx->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
     AppendArgs a = {};
@@ -774,6 +778,9 @@ extern "C" int satori_batch_attention_device(satori_batch *b, int layer, const v
     if (ldq < qw || ldo < qw) return set_error(SATORI_ERR_ARGUMENT, "row stride below the row's length");
     if ((uintptr_t)q % type_size(p->type) || (uintptr_t)out % type_size(out_type))
         return set_error(SATORI_ERR_ARGUMENT, "misaligned pointer");
+    const size_t es = type_size(p->type), os = type_size(out_type);
+    if (rows_overlap(out, ldo * os, qw * os, q, ldq * es, qw * es, b->plan.head.rows))
+        return set_error(SATORI_ERR_ARGUMENT, "out must not overlap q");
     DeviceScope scope(p->ctx->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
     const size_t rows = record_rows(b);

@@ -42,6 +42,18 @@ struct BatchAttn {
     unsigned *err;
 };
 
+// Whether two tensors of `rows` rows have a byte in common: rows of wa bytes la apart from a on, of wb bytes lb apart
+// from b on.  Rows of the same distance that lie side by side (slices of wider ones) have none; of other distances
+// anything that is not one before the other counts.
+inline bool rows_overlap(const void *a, long long la, long long wa, const void *b, long long lb, long long wb, long long rows)
+{
+    const long long x = (long long)(uintptr_t)a, y = (long long)(uintptr_t)b;
+    if (x + (rows - 1) * la + wa <= y || y + (rows - 1) * lb + wb <= x) return false;
+    if (la != lb) return true;
+    const long long at = ((y - x) % la + la) % la;
+    return !(at >= wa && at + wb <= la);
+}
+
 // The kernels' share of PlanShape: tile and block sizes, costs and the CTAs a GPU holds at once.
 void wide_plan_shape(int sm_count, PlanShape &shape);
 int wide_record_rows();

@@ -237,3 +237,26 @@ def test_refusals(env):
     aset.dispose()
     with pytest.raises(sat.DisposedError):
         aset.unload(0)
+
+
+def test_rows_that_overlap(env):
+    """x, base and out may be slices of the same wide rows, and out base itself; anything else that overlaps is refused."""
+    sat, torch, ctx = env
+    rows, cols, n = 64, 96, 20
+    aset = sat.AdapterSet(rows, cols, 2, 8, ctx=ctx)
+    weights = _load(torch, aset, "bf16", rows, cols, [8, 5])
+    plan, ids = sat.AdapterRows(ctx), [0, 1] * 10
+    plan.assign(ids)
+    wide = torch.randn((n, cols + 2 * rows), device="cuda")
+    x, base, out = wide.split([cols, rows, rows], 1)
+    kept = wide.clone()
+    aset.apply_device(plan, x, base, out)
+    _check(torch, out, x, base, ids, weights)
+    assert torch.equal(wide[:, :cols + rows], kept[:, :cols + rows])
+    alone = out.clone()
+    aset.apply_device(plan, x, base, base)                    # in place
+    assert torch.equal(base, alone)
+    for b, o in ((base, x[:, :rows]), (base, wide[:, cols - 1:cols - 1 + rows]), (base, wide[:, cols + 1:cols + 1 + rows]),
+                 (base, wide.view(-1)[cols:cols + n * rows].view(n, rows))):
+        with pytest.raises(sat.ArgumentError, match="overlap"):
+            aset.apply_device(plan, x, b, o)

@@ -641,3 +641,37 @@ def test_heads_of_any_size(env, kind, dim, kv_heads, group, page):
     q = m.step(seqs, [1] * 4)
     m.check(seqs, [1] * 4, q, out_f32=True)
     m.check(seqs, [1] * 4, q, strided=True)
+
+
+def test_rows_that_overlap(env):
+    """Slices of the same wide rows are taken, rows that share values refused; a packed q may be rotated in place."""
+    sat, torch, ctx = env
+    m = Model(env, "bf16", 64, 2, 2, 16, layers=1, rope=1e4, seed=33)
+    s = m.new()
+    (q,) = m.step([s], [5])
+    wide = torch.zeros((5, 512), dtype=torch.bfloat16, device="cuda")
+    wide[:, :256] = q
+    m.batch.attention_device(0, wide[:, :256], wide[:, 256:])
+    out = torch.empty_like(q)
+    m.batch.attention_device(0, q, out)
+    assert torch.equal(wide[:, 256:], out) and torch.equal(wide[:, :256], q)
+    flat = torch.zeros(4 * 5 * 256, dtype=torch.bfloat16, device="cuda")
+    cut = lambda at: flat[at:at + 5 * 256].view(5, 256)
+    for a, b in ((q, q), (wide[:, :256], wide[:, 128:384]), (wide[:, 128:384], wide[:, :256]), (cut(0), cut(255)),
+                 (cut(5 * 256 - 1), cut(0)), (cut(8), flat[:5 * 512].view(5, 512)[:, 256:])):
+        with pytest.raises(sat.ArgumentError, match="overlap"):
+            m.batch.attention_device(0, a, b)
+    m.batch.attention_device(0, cut(0), cut(5 * 256))         # neighbours
+    k = m.normal(5, 128).to(torch.bfloat16)
+    raw = m.normal(5, 256).to(torch.bfloat16)
+    m.batch.append_device(0, k, k, raw, out)
+    place = raw.clone()
+    m.batch.append_device(0, k, k, place, place)
+    assert torch.equal(place, out)
+    fused = m.normal(5, 512).to(torch.bfloat16)
+    with pytest.raises(sat.ArgumentError, match="overlap"):
+        m.batch.append_device(0, fused[:, 256:384], fused[:, 384:], fused[:, :256], fused.view(-1)[:5 * 256].view(5, 256))
+    with pytest.raises(sat.ArgumentError, match="overlap"):
+        m.batch.append_device(0, k, k, cut(0), cut(64))
+    with pytest.raises(sat.ArgumentError, match="overlap"):
+        m.batch.append_device(0, cut(0)[:, :128], k, raw, cut(0))
