@@ -988,13 +988,14 @@ void tensor_plan_shape(int sm_count, PlanShape &shape)
     shape.block = kBlockKeys;
     shape.ctas = sm_count;
     shape.solo_m = kTileRows;
-    // About 120 clocks each: a block of a small tile (HBM's share), of a large one, and an item's start and end.  An
-    // item at 60 leaves CTAs with few items behind those with many: 512 requests of 100 tokens behind 2048 then take
-    // 211 us and not 159, 64 of 1000 over 32 KV heads 101 and not 82; a large block at 20 costs 64 requests behind 32k
-    // tokens 73 and not 68 us.
+    // About 120 clocks each: a block of a small tile (HBM's share), of a large one, an item's start and end, and the
+    // shortest item, which is a chain of latencies.  An item at 60 leaves CTAs with few items behind those with many:
+    // 512 requests of 100 tokens behind 2048 then take 211 us and not 157, 64 of 1000 over 32 KV heads 101 and not 82;
+    // a large block at 20 costs 64 requests behind 32k tokens 73 and not 67 us.
     shape.solo_cost = 10;
     shape.pair_cost = 16;
     shape.item_cost = 30;
+    shape.least_cost = 50;
     shape.slots_per_item = 2;
 }
 

@@ -128,8 +128,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                 t.keys = row.position + 1 - seg.start;
             }
             const int blocks = (t.keys + shape.block - 1) / shape.block;
-            const int cost = shape.block_cost(t.m);
-            total += (long long)shape.kv_heads * (blocks * cost + shape.item_cost);
+            total += shape.kv_heads * shape.cost(t.m, blocks);
             plan.tiles.push_back(t);
         }
     }
@@ -170,7 +169,7 @@ void make_plan(const PlanShape &shape, const std::vector<PlanMember> &members, P
                                           h, at, (int)take, 0, 0, 0});
                     ++items;
                     at += (int)take;
-                    room -= take * cost + shape.item_cost;
+                    room -= take == blocks ? shape.cost(tile.m, blocks) : take * cost + shape.item_cost;
                 }
                 // One item holds every key its rows can see: it writes the rows' outputs.  (Tiles that an
                 // item works on in two halves of its blocks leave two records.)

@@ -67,12 +67,18 @@ struct PlanShape {
     int ctas;                                          // CTAs that the items are dealt to
     int solo_m;                                        // tiles of at most this many rows cost solo_cost per block
     int solo_cost, pair_cost, item_cost;               // cost of a block (small / large tile) and of an item
+    int least_cost = 0;                                // of a whole tile's item, however short
     int more_cost = 0;                                 // added to pair_cost in proportion to the rows beyond tile_m / 2
     int slots_per_item;                                // partial records an item writes
     int block_cost(int m) const
     {
         const int half = tile_m / 2;
         return m <= solo_m ? solo_cost : m <= half ? pair_cost : pair_cost + more_cost * (m - half) / half;
+    }
+    long long cost(int m, long long blocks) const      // of a tile as one item
+    {
+        const long long c = blocks * block_cost(m) + item_cost;
+        return c < least_cost ? least_cost : c;
     }
 };
 
