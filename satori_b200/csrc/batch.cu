@@ -597,12 +597,13 @@ cudaError_t satori::launch_combine(const BatchAttn &a, int record_rows, int tile
     // 137 us, with a block for each 172; 512 requests over 8 KV heads 235 and 247, 64 over 32 KV heads 134 and 138);
     // with fewer, their records are better dealt to whole blocks (256 requests over 4 KV heads 83 us, with a warp
     // for each 99; 64 behind 32k tokens 81 and 132).  There as many slices as a row's values leave threads for, and
-    // four when there are too few rows to fill the SMs (one sequence of 4k tokens over 4 KV heads, 66 records a
-    // row: 13 us with one slice, 9 with four).
+    // more while all blocks are resident (4 an SM): one sequence of 4k tokens over 4 KV heads, 66 records a row, takes
+    // 13 us with one slice, 9 with four; the call of 64 requests behind 32k tokens 66.5 us with one, 62.9 with two.
     const int outputs = std::min(a.group, kCombineHeads) * a.head_dim / 4, octets = (a.group + kCombineHeads - 1) / kCombineHeads;
     const long long rows = (long long)merges * octets;
     const bool warps = rows >= 2048;
-    const int slices = warps ? 0 : outputs <= 64 || rows < sm_count ? 4 : outputs <= 128 ? 2 : 1;
+    auto fits = [&](int slices) { return rows * ((outputs * slices + kCombineThreads - 1) / kCombineThreads) <= 4 * sm_count; };
+    const int slices = warps ? 0 : outputs <= 64 || fits(4) ? 4 : outputs <= 128 || fits(2) ? 2 : 1;
     const int quads = warps ? outputs : kCombineThreads / slices;
     const CombineShape c = {record_rows, tile_m, by_column, octets, (outputs + quads - 1) / quads};
     const long long blocks = warps ? (rows + kCombineThreads / 32 - 1) / (kCombineThreads / 32) : rows * c.parts;
