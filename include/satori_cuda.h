@@ -284,8 +284,9 @@ SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
 SATORI_API int satori_adapter_rows_destroy(satori_adapter_rows *r);
 /* out[p] = base[p] + scale * B (A x[p]) for the assigned rows: device pointers on the context's stream, x
  * rows of cols floats ldx apart, base and out rows of `rows` floats (0: packed).  out may be base itself and
- * must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits (A x beside fp16 weights to 22,
- * or to 2^-39 of its row's largest), FP32 sums; an infinity in x may come out as NaN in its own row. */
+ * must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits (beside fp16 weights to 22,
+ * or to 2^-39 of the largest of 32 columns and of the row), FP32 sums; an infinity in x may come out as NaN in its
+ * own row. */
 SATORI_API int satori_adapters_apply_device(satori_adapters *s, const satori_adapter_rows *r, const float *x,
                                             long long ldx, const float *base, long long ldbase, float *out,
                                             long long ldo);

@@ -12,10 +12,10 @@
 // of every sum is fixed by the shapes.
 //
 // Both products run on the tensor cores at FP32 accuracy: x and t are cut into three bf16 parts each (24
-// bits), a weight into as many as it needs to be exact (bf16 1, fp16 2, fp32 3), and the products of parts
-// above 2^-24 of the whole are added in FP32 (3, 5 and 6 MMAs per step).  Beside fp16 weights t, whose rows are
-// at hand, is scaled by a power of two into fp16's range and cut into two fp16 parts (22 bits, or 2^-39 of the row's
-// largest), which meet the weights as they are: 2 MMAs instead of 5 and no conversions.  Bytes bound it: the weights
+// bits), a weight into as many as it needs to be exact (bf16 1, fp32 3), and the products of parts
+// above 2^-24 of the whole are added in FP32 (3 and 6 MMAs per step).  Beside fp16 weights a row of t, or 32 columns
+// of a row of x, is scaled by a power of two into fp16's range and cut into two fp16 parts (22 bits, or 2^-39 of the
+// largest of them), which meet the weights as they are: 2 MMAs and no conversions.  Bytes bound it: the weights
 // of the slots in use, x, base and out.  While outputs are written they move at 5.1 to 5.9 TB/s (4000 rows of 3
 // slots, rank 64, 1536 -> 8960 in bf16, 56 of 98 us; 128 rows of 32 slots, 3584 -> 18944 in fp16, 17 of 40 us); the
 // first product before it is bound by its instructions (the parts of x and of the weights).  B streams through a ring of each warp's own in shared memory, filled by bulk
@@ -94,7 +94,7 @@ struct Weights<SATORI_BF16> {
 };
 template <>
 struct Weights<SATORI_F16> {
-    static constexpr int kParts = 2, kBytes = 2;
+    static constexpr int kParts = 1, kBytes = 2;
 };
 template <>
 struct Weights<SATORI_F32> {
@@ -105,19 +105,14 @@ struct Weights<SATORI_F32> {
 template <int TYPE>
 __device__ __forceinline__ void weight_parts(const uint32_t *raw, uint32_t (*part)[2])
 {
-    if (TYPE == SATORI_BF16) {
+    if (TYPE != SATORI_F32) {
         part[0][0] = raw[0];
         part[0][1] = raw[1];
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float2 f;
-            if (TYPE == SATORI_F16)
-                f = __half22float2(*reinterpret_cast<const __half2 *>(&raw[h]));
-            else
-                f = make_float2(__uint_as_float(raw[2 * h]), __uint_as_float(raw[2 * h + 1]));
             uint32_t p[Weights<TYPE>::kParts];
-            split_values<Weights<TYPE>::kParts>(f.x, f.y, p);
+            split_values<Weights<TYPE>::kParts>(__uint_as_float(raw[2 * h]), __uint_as_float(raw[2 * h + 1]), p);
 #pragma unroll
             for (int i = 0; i < Weights<TYPE>::kParts; ++i) part[i][h] = p[i];
         }
@@ -281,25 +276,65 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
                                 for (int e = 0; e < 8; ++e) x[h][e] = row >= 0 && k + e < a.cols ? __ldg(src + e) : 0.0f;
                             }
                         }
+                        if (TYPE == SATORI_F16) {
+                            // The run's columns of a row, scaled by a power of two, in two fp16 parts.
+                            uint32_t xa[2][2][4];
+                            float back[2];
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            uint32_t xa[3][4];
+                            for (int h = 0; h < 2; ++h) {
+                                float top = fabsf(x[h][0]);
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
+                                for (int e = 1; e < 8; ++e) top = fmaxf(top, fabsf(x[h][e]));
+                                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                                const int up = min(14 - ((int)(__float_as_uint(top) >> 23) - 127), 126);
+                                const float scale = __uint_as_float((uint32_t)(127 + up) << 23);
+                                back[h] = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    uint32_t p[3];
-                                    split_values<3>(x[h][4 * s + 2 * e], x[h][4 * s + 2 * e + 1], p);
+                                for (int s = 0; s < 2; ++s)
 #pragma unroll
-                                    for (int c = 0; c < 3; ++c) xa[c][2 * e + h] = p[c];
-                                }
+                                    for (int e = 0; e < 2; ++e) {
+                                        const float a0 = x[h][4 * s + 2 * e] * scale, a1 = x[h][4 * s + 2 * e + 1] * scale;
+                                        const __half2 hi = __floats2half2_rn(a0, a1);
+                                        const float2 f = __half22float2(hi);
+                                        const __half2 lo = __floats2half2_rn(a0 - f.x, a1 - f.y);
+                                        xa[s][0][2 * e + h] = *reinterpret_cast<const uint32_t *>(&hi);
+                                        xa[s][1][2 * e + h] = *reinterpret_cast<const uint32_t *>(&lo);
+                                    }
+                            }
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
                                 if (j < nt) {
-                                    uint32_t wb[W::kParts][2];
-                                    weight_parts<TYPE>(&raw[j][s * RAW / 2], wb);
-                                    mma_parts<W::kParts>(acc[j], xa, wb);
+                                    float part[4] = {0, 0, 0, 0};
+#pragma unroll
+                                    for (int s = 0; s < 2; ++s) {
+                                        mma_f16(part, xa[s][1], &raw[j][s * RAW / 2]);
+                                        mma_f16(part, xa[s][0], &raw[j][s * RAW / 2]);
+                                    }
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(part[e], back[e / 2], acc[j][e]);
                                 }
+                        } else {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) {
+                                uint32_t xa[3][4];
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        uint32_t p[3];
+                                        split_values<3>(x[h][4 * s + 2 * e], x[h][4 * s + 2 * e + 1], p);
+#pragma unroll
+                                        for (int c = 0; c < 3; ++c) xa[c][2 * e + h] = p[c];
+                                    }
+#pragma unroll
+                                for (int j = 0; j < NT; ++j)
+                                    if (j < nt) {
+                                        uint32_t wb[W::kParts][2];
+                                        weight_parts<TYPE>(&raw[j][s * RAW / 2], wb);
+                                        mma_parts<W::kParts>(acc[j], xa, wb);
+                                    }
+                            }
                         }
                     }
 #pragma unroll

@@ -260,3 +260,26 @@ def test_rows_that_overlap(env):
                  (base, wide.view(-1)[cols:cols + n * rows].view(n, rows))):
         with pytest.raises(sat.ArgumentError, match="overlap"):
             aset.apply_device(plan, x, b, o)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_values_of_every_magnitude(env, kind):
+    """Rows of x from 2^-100 to 2^100 (no product passes FP32's range), zero rows, and columns of very different size:
+    each part that a value is cut into keeps 2^-22 of it, or 2^-39 of the largest beside it."""
+    sat, torch, ctx = env
+    rows, cols, n = 96, 200, 34
+    aset = sat.AdapterSet(rows, cols, 2, 24, dtype=kind, ctx=ctx)
+    weights = _load(torch, aset, kind, rows, cols, [24, 7], 3)
+    plan, ids = sat.AdapterRows(ctx), np.arange(n) % 2
+    plan.assign(ids)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn((n, cols), generator=g, device="cuda")
+    x[:17] *= 2.0 ** torch.linspace(-100, 100, 17, device="cuda").round()[:, None]
+    x[17] = 0
+    x[18:26, ::3] *= 2.0 ** -20
+    x[26:, :64] *= 2.0 ** 12
+    base = torch.zeros((n, rows), device="cuda")
+    out = torch.empty_like(base)
+    aset.apply_device(plan, x, base, out)
+    _check(torch, out, x, base, ids, weights)
+    assert bool((out[17] == 0).all())
