@@ -268,7 +268,11 @@ def _prepare_batch(case, seed):
         if case.get("prefix", 0):
             root = cache.create(1)
             cache.extend(root, [case["prefix"]])
+            # A fork copies the prefix's partial page whole, over the tokens behind it that lie there already.
+            kept = pool[:, s["table"][:, 0]].clone()
             seqs = cache.fork(root * len(counts))
+            torch.cuda.synchronize()
+            pool[:, s["table"][:, 0]] = kept
         else:
             seqs = cache.create(len(counts))
         # Each sequence's pages follow one another: all of its tokens get room, then the step's go again.
