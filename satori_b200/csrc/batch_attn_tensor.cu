@@ -10,7 +10,7 @@
 //  * warp 19 looks through the rows of V that not every row of the tile sees: it clears those behind the last key,
 //    and takes infinities and NaN out of the others, which the rows that do see them get back at the end (a
 //    weight of zero would turn them into NaN).  It also brings the queries of items of at most 24 rows (the usual
-//    step of a request) while the item before is worked on, so that their first scores wait for nothing;
+//    step of a request) while the items before are worked on, so that their first scores wait for nothing;
 //  * warps 0-7 and 8-15 are two softmax groups, each with its own O and two S / P buffers in tensor memory; two
 //    threads share a row, each with half of a block's keys and half of the output's columns.  A large tile
 //    (129..256 rows) gives each group 128 of its rows and every K and V block serves both; a small one gives
@@ -22,8 +22,11 @@
 // result does not depend on it.  P is rounded to the cache's type (half a step, as the operands already are);
 // S, the sums and O are FP32.
 //
-// What bounds it: HBM for up to about 256 rows per block of keys, beyond that the exponentials (16 per clock
-// and SM, 2048 clocks for two tiles' block) and the MMAs (2048 clocks) about equally.
+// What bounds it: HBM for requests of their own (16 of 4096 tokens, 28 heads of 128 over 4: 22 us a CTA, 21 at the rate
+// of HBM, 32 us a call with start and merge).  For large tiles the softmax: a block of 256 rows and 64 keys takes 1750
+// clocks with heads of 128 (64 requests behind 131072 tokens, 137 us) and 2000 with heads of 64, of which the
+// exponentials' unit is busy 770 and the tensor pipe half; four warps a scheduler wait on chains of their own.  An item
+// of one block takes about 6000 clocks, two at a time: 512 requests of one token 96 us.
 #include "batch.cuh"
 #include "common.cuh"
 
