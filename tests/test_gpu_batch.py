@@ -675,3 +675,44 @@ def test_rows_that_overlap(env):
         m.batch.append_device(0, k, k, cut(0), cut(64))
     with pytest.raises(sat.ArgumentError, match="overlap"):
         m.batch.append_device(0, cut(0)[:, :128], k, raw, cut(0))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_graphs_of_one_batch(env, kind):
+    """Each layer captured in a graph of its own: they share the plan and the space for partial results, and may be
+    replayed in any order on one stream, between eager calls too."""
+    sat, torch, ctx = env
+    m = Model(env, kind, 64, 2, 4, 16, pages=128, layers=2, seed=40)
+    root = m.new()
+    m.step([root], [300])
+    seqs = m.fork([root] * 3, [300, 290, 17])
+    m.step(seqs, [1, 40, 130])
+    queries = m.step(seqs, [1] * 3)
+    q = [x.clone() for x in queries]
+    out = [torch.zeros_like(x) for x in q]
+    stream, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        for layer in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                m.batch.attention_device(layer, q[layer], out[layer])
+    finally:
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    for step in range(3):
+        if step:
+            queries = m.step(seqs, [1] * 3)
+            for mine, new in zip(q, queries):
+                mine.copy_(new)
+        eager = [torch.empty_like(x) for x in q]
+        for layer in (0, 1):
+            m.batch.attention_device(layer, q[layer], eager[layer])
+        for order in ((0, 1), (1, 0), (1, 1, 0)):
+            for x in out:
+                x.zero_()
+            for layer in order:
+                graphs[layer].replay()
+                m.batch.attention_device(1 - layer, q[1 - layer], eager[1 - layer])
+            assert all(torch.equal(a, b) for a, b in zip(out, eager))
+        m.check(seqs, [1] * 3, queries)
