@@ -543,6 +543,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
             }
         }
     }
+    pdl_wait();                // also without an item: launches behind this one count on the end of those before
 }
 
 }  // namespace

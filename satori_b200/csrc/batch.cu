@@ -343,6 +343,7 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const Batch
         }
         __syncthreads();
     }
+    pdl_wait();                // also without a row: launches behind this one count on the attention's end
 }
 
 // The same with a warp for a row and up to 8 query heads, for launches with thousands of rows: no barriers, and the
@@ -454,6 +455,7 @@ __global__ void __launch_bounds__(kCombineThreads, ITEMS > 8 ? 2 : 3) combine_ro
             }
         }
     }
+    pdl_wait();                // (see above)
 }
 
 // ------------------------------------------------------------------------------------------- host side

@@ -1,0 +1,130 @@
+"""Batch attention and adapters where one launch, replay or value meets another: strange keys that rows see, partial
+records without a finite score, small weights, many merged rows, moved plans, launches that overlap.
+
+Tolerances are those of test_gpu_batch.py where nothing else is said.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_batch import KINDS, U, Model, env  # noqa: F401  (env: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled(env, kind, dim, kv_heads, group, page, pages, layers, seed):
+    """A model whose pages all hold normal values: nothing has to be appended."""
+    m = Model(env, kind, dim, kv_heads, group, page, pages=pages, layers=layers, seed=seed)
+    m.pool.copy_(m.normal(*m.pool.shape).to(m.dtype))
+    return m
+
+
+def _on_stream(torch, ctx, stream):
+    """Routes the context to a stream for a while."""
+    import contextlib
+
+    @contextlib.contextmanager
+    def scope():
+        torch.cuda.synchronize()
+        ctx.set_stream(stream.cuda_stream)
+        try:
+            yield
+        finally:
+            torch.cuda.synchronize()
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    return scope()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,kv_heads,group", [(128, 4, 7), (136, 2, 4)])
+@pytest.mark.parametrize("behind", ["projection", "adapters", "attention"])
+def test_outputs_without_a_merge_reach_the_launch_behind(env, request, kind, dim, kv_heads, group, behind):  # noqa: F811
+    """Requests of at most 64 tokens: every item writes its outputs itself and the merge has no row.  The next launch
+    may start early; it gets the attention's outputs all the same, eager and in a graph."""
+    sat, torch, ctx = env
+    n, width = 64, kv_heads * group * dim
+    m = _filled(env, kind, dim, kv_heads, group, 16, 5 * n, 1, 11)
+    seqs = m.cache.create(n)
+    m.cache.extend(seqs, [10 + i % 53 for i in range(n)])
+    m.batch.step(seqs, [1] * n)
+    assert m.batch.info()["items"] == n * kv_heads
+    q = m.normal(n, width).to(m.dtype)
+    att = torch.zeros((n, width), dtype=m.dtype if behind == "attention" else torch.float32, device="cuda")
+    if behind == "projection":
+        from satori_b200 import _lib
+        payload = torch.empty(256 * (width // 32) * 34, dtype=torch.uint8, device="cuda")
+        w = m.normal(256 * width) * 0.05
+        _lib.check(_lib.lib().satori_quantize_q_device(ctx.handle, w.data_ptr(), 256, width, sat.Q8_0, payload.data_ptr()))
+        matrix = sat.CudaQuantizedMatrix.from_device(ctx, payload.data_ptr(), payload.numel(), 256, width, sat.Q8_0)
+        request.addfinalizer(matrix.dispose)
+        out = torch.zeros((1, 256), device="cuda")
+        after = lambda: matrix.execute_device(att[n - 1].data_ptr(), out.data_ptr(), 1, _lib.ORDER_BATCH)
+    elif behind == "adapters":
+        aset = sat.AdapterSet(256, width, 2, 16, ctx=ctx)
+        for slot in range(2):
+            aset.load(slot, m.normal(16, width).bfloat16(), m.normal(256, 16).bfloat16())
+        plan = sat.AdapterRows(ctx)
+        plan.assign([i % 3 - 1 for i in range(n)])
+        base, out = m.normal(n, 256), torch.zeros((n, 256), device="cuda")
+        after = lambda: aset.apply_device(plan, att, base, out)
+    else:
+        out = torch.zeros((n, width), dtype=m.dtype, device="cuda")
+        after = lambda: m.batch.attention_device(0, att, out)
+    stream = torch.cuda.Stream()
+    with _on_stream(torch, ctx, stream), torch.cuda.stream(stream):
+        m.batch.attention_device(0, q, att)
+        stream.synchronize()
+        after()
+        stream.synchronize()
+        want = out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            m.batch.attention_device(0, q, att)
+            after()
+        for run in range(40):
+            att.fill_(math.nan)
+            out.fill_(math.nan)
+            stream.synchronize()
+            if run % 2:
+                graph.replay()
+            else:
+                m.batch.attention_device(0, q, att)
+                after()
+            stream.synchronize()
+            assert torch.equal(out, want), run
+
+
+def test_an_application_without_items_waits_for_the_launch_before(env):  # noqa: F811
+    """Replayed after an assignment of no rows between an attention and its reader."""
+    sat, torch, ctx = env
+    n = 64
+    m = _filled(env, "bf16", 128, 4, 7, 16, 5 * n, 1, 12)
+    seqs = m.cache.create(n)
+    m.cache.extend(seqs, [10 + i % 53 for i in range(n)])
+    m.batch.step(seqs, [1] * n)
+    q = m.normal(n, 28 * 128).to(m.dtype)
+    att = torch.zeros((n, 28 * 128), device="cuda")
+    first, second = sat.AdapterRows(ctx), sat.AdapterRows(ctx)
+    first.assign([0] * n)
+    second.assign([0] * n)
+    aset = sat.AdapterSet(96, 28 * 128, 1, 16, ctx=ctx)
+    aset.load(0, m.normal(16, 28 * 128).bfloat16(), m.normal(96, 16).bfloat16())
+    base, unused, out = m.normal(n, 96), torch.zeros((n, 96), device="cuda"), torch.zeros((n, 96), device="cuda")
+    stream = torch.cuda.Stream()
+    with _on_stream(torch, ctx, stream), torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            m.batch.attention_device(0, q, att)
+            aset.apply_device(first, att, base, unused)
+            aset.apply_device(second, att, base, out)
+        graph.replay()
+        stream.synchronize()
+        want = out.clone()
+        first.assign([])
+        for _ in range(20):
+            att.fill_(math.nan)
+            out.fill_(math.nan)
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(out, want)
