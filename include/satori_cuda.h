@@ -94,7 +94,8 @@ SATORI_API void *satori_stream(satori_ctx *ctx);
  * stream), e.g. to capture device-pointer calls into the caller's CUDA graph. */
 SATORI_API int satori_set_stream(satori_ctx *ctx, void *stream);
 /* Waits for the work queued on the context's current stream; reports a device error a kernel recorded
- * (SATORI_ERR_TIMEOUT for an expired bounded wait) like the synchronous calls do. */
+ * (SATORI_ERR_TIMEOUT for an expired bounded wait, SATORI_ERR_ARGUMENT for a replay with an adapter slot that does
+ * not exist) like the synchronous calls do. */
 SATORI_API int satori_synchronize(satori_ctx *ctx);
 
 /* ------------------------------------------------------------------ matrices */
@@ -277,7 +278,9 @@ SATORI_API int satori_adapters_load(satori_adapters *s, int slot, int rank, cons
                                     long long ldb, float scale);
 SATORI_API int satori_adapters_destroy(satori_adapters *s);
 /* Which slot each row of a batch uses (-1: none), for all projections of a step.  Captured applications may
- * be replayed after the next assignment when their row buffers are large enough for its rows. */
+ * be replayed after the next assignment when their row buffers are large enough for its rows; a row whose slot the
+ * applied adapters do not have then gets its base alone, and the next satori_synchronize reports
+ * SATORI_ERR_ARGUMENT. */
 typedef struct satori_adapter_rows satori_adapter_rows;
 SATORI_API int satori_adapter_rows_create(satori_ctx *ctx, satori_adapter_rows **out);
 SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const int *slots);

@@ -61,6 +61,7 @@ struct AdapterArgs {
     const float *x, *base;
     float *out;
     long long ldx, ldbase, ldo;
+    int n_slots;
     int splits;                                // clusters that share an item's outputs
     int rows, cols, cols32;                    // output rows, columns, columns rounded up to 32
     int wide_x, wide_out;                      // 16-byte accesses are possible
@@ -226,7 +227,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
         const RowItem item = list[unit / a.splits];
         const int split = unit % a.splits;     // its share of the outputs; t is every share's own
         SlotDesc slot = {};
-        if (item.slot >= 0) slot = a.slots[item.slot];
+        // (A replay may follow an assignment of slots that these adapters lack: such rows get their base.)
+        if (item.slot >= 0 && item.slot < a.n_slots)
+            slot = a.slots[item.slot];
+        else if (item.slot >= 0 && tid == 0)
+            atomicOr(a.err, kDevErrSlot);
         const int rank = slot.rank16, tiles = (item.rows + 15) / 16;
         pdl_wait();
         __syncthreads();                       // the item before is done with the rows and the ring
@@ -845,6 +850,7 @@ extern "C" int satori_adapters_apply_device(satori_adapters *s, const satori_ada
     AdapterArgs a = {};
     a.plan = reinterpret_cast<const DevRows *>(r->d_plan);
     a.slots = s->d_slots;
+    a.n_slots = s->slots;
     a.x = x;
     a.base = base;
     a.out = out;

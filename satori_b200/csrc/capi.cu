@@ -71,6 +71,10 @@ int check_dev_error(satori_ctx *ctx)
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) return cuda_fail(e, "synchronize");
     if (err & kDevErrTimeout) return set_error(SATORI_ERR_TIMEOUT, "a bounded device wait expired");
+    if (err & kDevErrSlot) {                 // the caller's mistake, not a state of the device: reported once
+        if ((e = clear_dev_error(ctx)) != cudaSuccess) return cuda_fail(e, "synchronize");
+        return set_error(SATORI_ERR_ARGUMENT, "a replayed application met a slot that its adapters do not have");
+    }
     return SATORI_OK;
 }
 

@@ -13,8 +13,9 @@
 namespace satori {
 
 // --------------------------------------------------------------------------- error flags
-// Device-side error word of a context: bit 0 = a bounded wait expired.
-enum : unsigned { kDevErrTimeout = 1u };
+// Device-side error word of a context: bit 0 = a bounded wait expired; bit 1 = a replayed adapter application met a
+// slot that its adapters do not have.
+enum : unsigned { kDevErrTimeout = 1u, kDevErrSlot = 2u };
 
 // Spin budget for mbarrier waits: ~4e9 cycles of polling is seconds, far beyond any copy.
 constexpr long long kWaitBudgetCycles = 4000000000LL;

@@ -128,3 +128,34 @@ def test_an_application_without_items_waits_for_the_launch_before(env):  # noqa:
             graph.replay()
             stream.synchronize()
             assert torch.equal(out, want)
+
+
+def test_a_replay_with_a_slot_that_its_adapters_lack(env):  # noqa: F811
+    """The call itself refuses such a slot; a replay after a later assignment leaves the row's base and reports it."""
+    sat, torch, ctx = env
+    aset = sat.AdapterSet(48, 64, 2, 8, dtype="f32", ctx=ctx)
+    for slot in range(2):
+        aset.load(slot, torch.randn((8, 64), device="cuda"), torch.randn((48, 8), device="cuda"))
+    plan = sat.AdapterRows(ctx)
+    plan.assign([0, 1, 0, -1])
+    x, base = torch.randn((4, 64), device="cuda"), torch.randn((4, 48), device="cuda")
+    out, want = torch.zeros_like(base), torch.zeros_like(base)
+    stream = torch.cuda.Stream()
+    with _on_stream(torch, ctx, stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            aset.apply_device(plan, x, base, out)
+    plan.assign([1, -1, -1, 0])
+    aset.apply_device(plan, x, base, want)
+    ctx.synchronize()
+    plan.assign([1, 2, 1 << 30, 0])
+    with pytest.raises(sat.ArgumentError):
+        aset.apply_device(plan, x, base, want)
+    graph.replay()
+    with pytest.raises(sat.ArgumentError, match="slot"):
+        ctx.synchronize()
+    assert torch.allclose(out, want, rtol=0, atol=1e-3)        # (the items differ, and with them the order of sums)
+    assert torch.equal(out[1:3], base[1:3])
+    plan.assign([1, -1, -1, 0])
+    graph.replay()
+    ctx.synchronize()                                          # reported once
