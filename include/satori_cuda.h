@@ -286,8 +286,8 @@ SATORI_API int satori_adapter_rows_create(satori_ctx *ctx, satori_adapter_rows *
 SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const int *slots);
 SATORI_API int satori_adapter_rows_destroy(satori_adapter_rows *r);
 /* out[p] = base[p] + scale * B (A x[p]) for the assigned rows: device pointers on the context's stream, x
- * rows of cols floats ldx apart, base and out rows of `rows` floats (0: packed).  out may be base itself and
- * must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits (beside fp16 weights to 22,
+ * rows of cols floats ldx apart, base and out rows of `rows` floats (0: packed).  Adapters and rows belong to the
+ * same context.  out may be base itself and must not overlap anything else.  FP32 accuracy: weights exact, x and A x to 24 bits (beside fp16 weights to 22,
  * or to 2^-39 of the largest of 32 columns and of the row), FP32 sums; an infinity in x may come out as NaN in its
  * own row. */
 SATORI_API int satori_adapters_apply_device(satori_adapters *s, const satori_adapter_rows *r, const float *x,

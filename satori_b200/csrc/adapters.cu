@@ -829,7 +829,8 @@ extern "C" int satori_adapters_apply_device(satori_adapters *s, const satori_ada
 {
     if (!s) return set_error(SATORI_ERR_DISPOSED, "adapters are disposed");
     if (!r) return set_error(SATORI_ERR_DISPOSED, "adapter rows are disposed");
-    if (r->ctx->device != s->ctx->device) return set_error(SATORI_ERR_ARGUMENT, "adapters and rows are on different devices");
+    // The assignment was uploaded on its own context's stream: nothing orders it before this context's launch.
+    if (r->ctx != s->ctx) return set_error(SATORI_ERR_ARGUMENT, "adapters and rows belong to different contexts");
     if (r->rows < 0) return set_error(SATORI_ERR_ARGUMENT, "no rows are assigned yet");
     if (r->top_slot >= s->slots)
         return set_error(SATORI_ERR_ARGUMENT, "slot %d is assigned; these adapters have %d", r->top_slot, s->slots);
@@ -882,6 +883,7 @@ extern "C" int satori_matrix_execute_adapted_device(satori_matrix *m, satori_ada
     if (s->rows != m->rows || s->cols != m->cols)
         return set_error(SATORI_ERR_ARGUMENT, "adapters of %d x %d beside a %d x %d matrix", s->rows, s->cols, m->rows, m->cols);
     if (s->ctx != m->ctx) return set_error(SATORI_ERR_ARGUMENT, "adapters and matrix belong to different contexts");
+    if (r->ctx != s->ctx) return set_error(SATORI_ERR_ARGUMENT, "adapters and rows belong to different contexts");
     if (r->rows < 0) return set_error(SATORI_ERR_ARGUMENT, "no rows are assigned yet");
     if (r->top_slot >= s->slots)
         return set_error(SATORI_ERR_ARGUMENT, "slot %d is assigned; these adapters have %d", r->top_slot, s->slots);

@@ -159,3 +159,24 @@ def test_a_replay_with_a_slot_that_its_adapters_lack(env):  # noqa: F811
     plan.assign([1, -1, -1, 0])
     graph.replay()
     ctx.synchronize()                                          # reported once
+
+
+def test_rows_of_another_context_are_refused(env, request):  # noqa: F811
+    sat, torch, ctx = env
+    other = sat.Context(0)
+    try:
+        aset = sat.AdapterSet(16, 32, 1, 4, dtype="f32", ctx=ctx)
+        foreign = sat.AdapterRows(other)
+        foreign.assign([0, -1])
+        x, base = torch.zeros((2, 32), device="cuda"), torch.zeros((2, 16), device="cuda")
+        with pytest.raises(sat.ArgumentError, match="context"):
+            aset.apply_device(foreign, x, base, torch.zeros_like(base))
+        payload = torch.zeros(16 * 34, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        matrix = sat.CudaQuantizedMatrix.from_device(ctx, payload.data_ptr(), payload.numel(), 16, 32, sat.Q8_0)
+        request.addfinalizer(matrix.dispose)
+        with pytest.raises(sat.ArgumentError, match="context"):
+            aset.execute_device(matrix, foreign, x, torch.zeros_like(base))
+        foreign.dispose()
+    finally:
+        other.close()
