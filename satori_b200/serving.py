@@ -422,6 +422,9 @@ class AdapterSet:
             raise _bad(f"{name} is not on device {self.ctx.device}")
         if (w.shape[1] > 1 and w.stride(1) != 1) or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
             w = w.contiguous()
+            if w.is_cuda:                                     # torch's stream makes the copy, the context's reads it
+                import torch
+                torch.cuda.current_stream(w.device).synchronize()
         return w.data_ptr(), (w.stride(0) if w.shape[0] > 1 else w.shape[1]), w
 
     def apply_device(self, rows: AdapterRows, x, base, out) -> None:

@@ -180,3 +180,30 @@ def test_rows_of_another_context_are_refused(env, request):  # noqa: F811
         foreign.dispose()
     finally:
         other.close()
+
+
+def test_transposed_weights_on_a_context_with_its_own_stream(env):  # noqa: F811
+    """load makes a packed copy of a transposed tensor on torch's stream; the context's reads it only then."""
+    sat, torch, _ = env
+    mine = sat.Context(0)
+    try:
+        rows, cols = 64, 96
+        aset = sat.AdapterSet(rows, cols, 1, 16, dtype="f32", ctx=mine)
+        plan = sat.AdapterRows(mine)
+        plan.assign([0] * 5)
+        for seed in range(3):
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            a, b = torch.randn((cols, 16), generator=g, device="cuda"), torch.randn((16, rows), generator=g, device="cuda")
+            x, base = torch.randn((5, cols), generator=g, device="cuda"), torch.zeros((5, rows), device="cuda")
+            out = torch.empty_like(base)
+            torch.cuda.synchronize()
+            torch.cuda._sleep(50_000_000)                      # torch's stream is busy for some 25 ms
+            aset.load(0, a.T, b.T)
+            aset.apply_device(plan, x, base, out)
+            mine.synchronize()
+            exact = (x.double() @ a.double()) @ b.double()
+            assert torch.allclose(out.double(), exact, rtol=0, atol=(96 + 16 + 16) * 2 * U * float((x.abs() @ a.abs() @ b.abs()).max()))
+        plan.dispose()
+        aset.dispose()
+    finally:
+        mine.close()
