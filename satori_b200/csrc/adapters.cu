@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kMaxRank = 128, kMaxCluster = 8, kItemRows = 64;
+constexpr size_t kPlanInts = 1 << 14;          // of a row plan's first block
 
 struct SlotDesc {
     const uint8_t *a, *b;                      // A [rank16][cols32] and B [rows][rank16], zero padded
@@ -50,9 +51,12 @@ struct RowItem {
     int slot, row_off, rows;
 };
 
-// Header of a row plan in device memory; the items and the row list follow.
+// Header of a row plan, at an address that never changes, so that captured applications read the current
+// assignment whatever its size.
 struct DevRows {
-    int items, item_off, rows_off, pad;
+    const RowItem *list;
+    const int *rows;
+    int items, pad[3];
 };
 
 struct AdapterArgs {
@@ -218,10 +222,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(AdapterSmem<TYPE, RM>) <= 113
     uint32_t parity = 0;                       // bit s: this warp's slot s
     // The plan lay there when the launch before this one started: a copy on the stream brought it, and no launch
     // behind a copy starts before it.
-    const int *plan = reinterpret_cast<const int *>(a.plan);
     const int items = a.plan->items;
-    const RowItem *list = reinterpret_cast<const RowItem *>(plan + a.plan->item_off);
-    const int *rows = plan + a.plan->rows_off;
+    const RowItem *list = a.plan->list;
+    const int *rows = a.plan->rows;
 
     for (int unit = blockIdx.x / ctas; unit < items * a.splits; unit += gridDim.x / ctas) {
         const RowItem item = list[unit / a.splits];
@@ -567,9 +570,10 @@ struct satori_adapter_rows {
     satori_ctx *ctx = nullptr;
     int rows = -1, top_slot = -1;              // rows assigned, highest slot used
     int items = 0;
-    int *d_plan = nullptr;
-    size_t plan_ints = 0;
-    std::vector<void *> outgrown;              // kept for graphs captured before the plan moved
+    int *d_plan = nullptr;                     // kPlanInts: the header, and the lists behind it where they fit
+    int *d_lists = nullptr;                    // longer lists
+    size_t list_ints = 0;
+    std::vector<void *> outgrown;              // may still be read by launches that are queued
     Staging staging;
 };
 
@@ -780,31 +784,33 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
             }
             if ((int)items.size() * kMaxCluster >= 2 * ctx->sm_count) break;
         }
-        DevRows head = {};
-        size_t ints = sizeof(DevRows) / 4;
-        head.items = (int)items.size();
-        head.item_off = (int)ints;
-        ints += items.size() * sizeof(RowItem) / 4;
-        head.rows_off = (int)ints;
-        ints += (size_t)n;
-        if (ints > r->plan_ints) {
-            const size_t count = std::max<size_t>(std::max(ints, 2 * r->plan_ints), 1 << 14);
+        const size_t head_ints = sizeof(DevRows) / 4, item_ints = items.size() * sizeof(RowItem) / 4, ints = item_ints + (size_t)n;
+        const bool apart = head_ints + ints > kPlanInts;
+        if (!r->d_plan && (e = cudaMalloc(&r->d_plan, kPlanInts * 4)) != cudaSuccess) return cuda_fail(e, "allocate adapter rows");
+        if (apart && ints > r->list_ints) {
+            const size_t count = std::max(ints, 2 * r->list_ints);
             int *fresh = nullptr;
             r->outgrown.reserve(r->outgrown.size() + 1);
             if ((e = cudaMalloc(&fresh, count * 4)) != cudaSuccess) return cuda_fail(e, "allocate adapter rows");
-            if (r->d_plan) r->outgrown.push_back(r->d_plan);
-            r->d_plan = fresh;
-            r->plan_ints = count;
-            r->rows = -1;                      // nothing there until the upload
+            if (r->d_lists) r->outgrown.push_back(r->d_lists);
+            r->d_lists = fresh;
+            r->list_ints = count;
         }
         void *buffer = nullptr;
-        if ((e = r->staging.take(ints * 4, &buffer)) != cudaSuccess) return cuda_fail(e, "stage adapter rows");
+        if ((e = r->staging.take((head_ints + ints) * 4, &buffer)) != cudaSuccess) return cuda_fail(e, "stage adapter rows");
         int *stage = static_cast<int *>(buffer);
+        int *lists = apart ? r->d_lists : r->d_plan + head_ints;
+        DevRows head = {};
+        head.list = reinterpret_cast<const RowItem *>(lists);
+        head.rows = lists + item_ints;
+        head.items = (int)items.size();
         memcpy(stage, &head, sizeof head);
-        if (n) memcpy(stage + head.item_off, items.data(), items.size() * sizeof(RowItem));
-        if (n) memcpy(stage + head.rows_off, order.data(), (size_t)n * 4);
+        if (n) memcpy(stage + head_ints, items.data(), item_ints * 4);
+        if (n) memcpy(stage + head_ints + item_ints, order.data(), (size_t)n * 4);
         r->rows = -1;
-        if ((e = r->staging.send(r->d_plan, ints * 4, ctx->stream)) != cudaSuccess) return cuda_fail(e, "upload adapter rows");
+        if (apart) e = cudaMemcpyAsync(lists, stage + head_ints, ints * 4, cudaMemcpyHostToDevice, ctx->stream);
+        if (e == cudaSuccess) e = r->staging.send(r->d_plan, (apart ? head_ints : head_ints + ints) * 4, ctx->stream);
+        if (e != cudaSuccess) return cuda_fail(e, "upload adapter rows");
         r->rows = n;
         r->top_slot = top;
         r->items = head.items;
@@ -818,6 +824,7 @@ extern "C" int satori_adapter_rows_destroy(satori_adapter_rows *r)
     DeviceScope scope(r->ctx->device);
     cudaStreamSynchronize(r->ctx->stream);
     cudaFree(r->d_plan);
+    cudaFree(r->d_lists);
     for (void *old : r->outgrown) cudaFree(old);
     r->staging.release();
     delete r;

@@ -20,6 +20,37 @@ def _filled(env, kind, dim, kv_heads, group, page, pages, layers, seed):
     return m
 
 
+def test_a_replay_follows_an_assignment_that_outgrows_its_plan(env):  # noqa: F811
+    sat, torch, ctx = env
+    rows, cols, n = 16, 32, 20000
+    aset = sat.AdapterSet(rows, cols, 2, 4, dtype="f32", ctx=ctx)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for slot in range(2):
+        aset.load(slot, torch.randn((4, cols), generator=g, device="cuda"), torch.randn((rows, 4), generator=g, device="cuda"))
+    plan = sat.AdapterRows(ctx)
+    plan.assign([0, 1, -1])
+    x, base = torch.randn((n, cols), generator=g, device="cuda"), torch.randn((n, rows), generator=g, device="cuda")
+    out = torch.zeros_like(base)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            aset.apply_device(plan, x[:3], base[:3], out[:3])  # (the buffers behind hold 20000 rows)
+    finally:
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    for ids in (np.arange(17000) % 3 - 1, np.arange(5) % 2, np.arange(n) % 2, np.full(9, -1)):
+        plan.assign(ids)
+        out.fill_(7.0)
+        graph.replay()
+        want = torch.full_like(out, 7.0)
+        k = len(ids)
+        aset.apply_device(plan, x[:k], base[:k], want[:k])
+        # (The replay's clusters may be dealt differently from the eager call's: the sums' order is another.)
+        assert torch.allclose(out, want, rtol=0, atol=1e-3) and torch.equal(out[k:], want[k:])
+
+
 def _on_stream(torch, ctx, stream):
     """Routes the context to a stream for a while."""
     import contextlib
