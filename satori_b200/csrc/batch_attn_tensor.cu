@@ -178,17 +178,19 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+// NaN if any of them is.
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float m;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
     return m;
 }
 
 // 2^x on the FP32 units, two at a time, for part of the weights: the special function unit takes 8 clocks for a
 // warp's exponentials and is the scarcer one.  x = n + f with n the nearest integer (left in the low bits of
 // x + 1.5 2^23) and 2^f by a polynomial: the minimax fits on |f| <= 1/2 of degree 3 (relative error 7.5e-5,
-// 1/26 of bf16's half step) and 4 (2.6e-6, for fp16); n goes into the exponent.  x >= -126 is the caller's.
+// 1/26 of bf16's half step) and 4 (2.6e-6, for fp16); n goes into the exponent.  x below -126 counts as -126, and so
+// does a NaN, which the row's other weights and its sum then carry (see the maximum).
 template <int TYPE>
 __device__ __forceinline__ float2 exp2_poly(float2 x)
 {
@@ -876,13 +878,16 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) top[e / 2 & 3] = max3(top[e / 2 & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                    float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
+                    // A score that is NaN or plus infinity makes the row NaN: the maximum is NaN then, which is above
+                    // no bound and below none, and so are the weights that refer to it and their sum from there on.
+                    float high = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
                     // (The barrier also keeps one half's weights from the scores that the other has yet to read.)
-                    if (pair_any(pair_id, high > ref + kLazy || (k == 0 && high > -INFINITY))) {
+                    if (pair_any(pair_id, !(high <= ref + kLazy))) {
                         bar->exchange[g][half][r] = high;
                         pair_sync(pair_id);
-                        high = fmaxf(high, bar->exchange[g][half ^ 1][r]);
-                        const bool raise = high > ref + kLazy || (k == 0 && high > -INFINITY);
+                        high = max3(high, bar->exchange[g][half ^ 1][r], high);
+                        if (high == INFINITY) high = NAN;
+                        const bool raise = !(high <= ref + kLazy);
                         if (k > 0) {
                             // The last block's product may still be adding to O.  The next block's scores follow it.
                             if (k + 1 < blocks)

@@ -20,6 +20,77 @@ def _filled(env, kind, dim, kv_heads, group, page, pages, layers, seed):
     return m
 
 
+def _attend(m, layer, q, rows):
+    out = m.torch.full((rows, m.kv * m.group * m.dim), 7.0, dtype=m.torch.float32, device="cuda")
+    m.batch.attention_device(layer, q, out)
+    return out.double().cpu().numpy().reshape(rows, m.kv, m.group, m.dim)
+
+
+def _tolerance(m, t, exact, size, scores):
+    tol = (2 * (m.dim + 4) * scores[..., None] + 2 * (t + 16)) * U * size
+    return tol if m.kind == "f32" else tol + m.torch.finfo(m.dtype).eps / 2 * size
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,group,n,own", [(128, 8, 40, 1), (64, 8, 40, 1), (64, 1, 1, 200), (136, 8, 9, 1)])
+@pytest.mark.parametrize("special", [math.nan, math.inf, -math.inf])
+def test_a_strange_key_reaches_the_rows_that_see_it(env, kind, dim, group, n, own, special):  # noqa: F811
+    """A key that every row sees, at each of a block's 64 places: a NaN or infinite score makes the row NaN, a score of
+    minus infinity leaves the row without that key."""
+    torch = env[1]
+    m = _filled(env, kind, dim, 8, group, 64, 8 + 2 * n * (-(-own // 64)), 8, 5)
+    root = m.cache.create(1)
+    m.cache.extend(root, [256])
+    seqs = m.cache.fork(root * n)
+    m.batch.step(seqs, [own] * n)
+    table = m.cache.table(seqs[0])
+    for layer in range(8):
+        for h in range(8):
+            token = 64 + 8 * layer + h
+            m.pool[layer, int(table[token // 64]), 0, h, token % 64, 3] = special
+    rows = n * own
+    q = m.normal(rows, 8 * group * dim).to(m.dtype).view(rows, -1, dim)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    qd = q.double().cpu().numpy().reshape(rows, 8, group, dim)
+    some = [s for s in (0, n // 2, n - 1)]
+    tokens = {s: m.read(seqs[s]) for s in some}
+    for layer in range(8):
+        got = _attend(m, layer, q.view(rows, -1), rows)
+        if special != -math.inf:
+            assert np.isnan(got).all(), layer
+            continue
+        assert np.isfinite(got).all(), layer
+        for s in some:
+            for r in (0, own - 1):
+                t = 256 + r + 1
+                k, v = tokens[s][:, layer, :t]
+                for h in range(8):
+                    seen = np.arange(t) != 64 + 8 * layer + h
+                    exact, size, scores = m.formula(qd[s * own + r, h:h + 1], k[seen][:, h:h + 1], v[seen][:, h:h + 1])
+                    err = np.abs(got[s * own + r, h:h + 1] - exact)
+                    assert np.all(err <= _tolerance(m, t, exact, size, scores)), (layer, s, r, h)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 136])
+@pytest.mark.parametrize("special", [math.nan, math.inf])
+def test_a_strange_key_in_a_row_without_partial_records(env, kind, dim, special):  # noqa: F811
+    """Prompts of 200 rows, enough of them that most tiles are one item that writes the outputs itself."""
+    n, own = 48, 200
+    m = _filled(env, kind, dim, 8, 1, 64, 6 * n, 8, 10)
+    seqs = m.cache.create(n)
+    m.cache.extend(seqs, [64] * n)
+    m.batch.step(seqs, [own] * n)
+    first = m.torch.tensor([int(m.cache.table(s)[0]) for s in seqs], device="cuda")
+    for layer in range(8):
+        for h in range(8):
+            m.pool[layer, first, 0, h, 8 * layer + h, 3] = special
+    q = m.normal(n * own, 8, dim).to(m.dtype)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    for layer in range(8):
+        assert np.isnan(_attend(m, layer, q.view(n * own, -1), n * own)).all(), layer
+
+
 def test_a_replay_follows_an_assignment_that_outgrows_its_plan(env):  # noqa: F811
     sat, torch, ctx = env
     rows, cols, n = 16, 32, 20000
