@@ -183,6 +183,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a, int wid
     }
 }
 
+// A record's weight from its (maximum, sum).  A maximum of minus infinity: no key, and nothing was stored (sum 0), or
+// none but scores of NaN (sum NaN), which the row keeps.
+__device__ __forceinline__ float record_weight(float2 ml, float ref)
+{
+    return ml.x == -INFINITY ? ml.y : exp2f(ml.x - ref);
+}
+
 struct CombineShape {
     int record_rows, tile_m, by_column, octets, parts;
 };
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const Batch
                 ref = top;
 #pragma unroll
                 for (int j = 0; j < kCombineChunk / 32; ++j) {
-                    const float w = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - ref);   // no key: nothing was stored
+                    const float w = record_weight(ml[j], ref);
                     if (w != 0) sum = fmaf(w, ml[j].y, sum);
                     weight[mine][j * 32 + lane] = w;
                     base[mine][j * 32 + lane] = at[j];
@@ -398,7 +405,7 @@ __global__ void __launch_bounds__(kCombineThreads, ITEMS > 8 ? 2 : 3) combine_ro
             for (int o = kCombineHeads; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
             top = fmaxf(top, ref);
             const float keep = top == -INFINITY ? 1.0f : exp2f(ref - top);
-            const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);      // no key: nothing was stored
+            const float w = record_weight(ml, top);
             sum *= keep;
             if (w != 0) sum = fmaf(w, ml.y, sum);
             ref = top;

@@ -91,6 +91,28 @@ def test_a_strange_key_in_a_row_without_partial_records(env, kind, dim, special)
         assert np.isnan(_attend(m, layer, q.view(n * own, -1), n * own)).all(), layer
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 136])
+@pytest.mark.parametrize("n", [4, 520])
+def test_a_nan_key_alone_in_its_record(env, kind, dim, n):  # noqa: F811
+    """The only key of a partial record (a request's first own token behind a shared prefix) scores NaN: the merge must
+    not take the record for an empty one."""
+    m = _filled(env, kind, dim, 4, 2, 16, 16 + n, 1, 6)
+    root = m.cache.create(1)
+    m.cache.extend(root, [256])
+    seqs = m.cache.fork(root * n)
+    m.batch.step(seqs, [1] * n)
+    assert m.batch.info()["segments"] == n + 1
+    marked = list(range(0, n, 3))
+    for s in marked:
+        m.pool[0, int(m.cache.table(seqs[s])[16]), 0, s % 4, 0, 1] = math.nan
+    q = m.normal(n, 8 * dim).to(m.dtype)
+    got = _attend(m, 0, q, n)
+    nan = np.zeros((n, 4), bool)
+    nan[marked, [s % 4 for s in marked]] = True
+    assert np.array_equal(np.isnan(got).all((2, 3)), nan) and np.isfinite(got[~nan]).all()
+
+
 def test_a_replay_follows_an_assignment_that_outgrows_its_plan(env):  # noqa: F811
     sat, torch, ctx = env
     rows, cols, n = 16, 32, 20000
