@@ -18,8 +18,8 @@
 //    exponentials of this one.  Eight warps a group, not four: the exponentials are a chain of short steps, and
 //    with two warps per scheduler it was idle two thirds of the time.
 // The maximum that the exponentials refer to is raised only when it is exceeded by more than 2^8, so the
-// accumulator in tensor memory is rescaled a few times per row, not at every block; P stays below 2^8 and the
-// result does not depend on it.  P is rounded to the cache's type (half a step, as the operands already are);
+// accumulator in tensor memory is rescaled a few times per row, not at every block; P stays below 2^8 (beside fp16,
+// whose small weights would lose bits, 2^15: see kLift) and the result does not depend on it.  P is rounded to the cache's type (half a step, as the operands already are);
 // S, the sums and O are FP32.
 //
 // What bounds it: HBM for requests of their own (16 of 4096 tokens, 28 heads of 128 over 4: 22 us a CTA, 21 at the rate
@@ -43,6 +43,10 @@ constexpr int kGroupThreads = 2 * kTileRows, kThreads = 2 * kGroupThreads + 128;
 // 131072 about 6 % less time than with none, and no less with one in two or three.
 constexpr int kEvery = 4;
 constexpr float kLazy = 8.0f;                  // log2 of what a weight may exceed 1 by
+// log2 of a factor of all weights and their sums.  fp16 ends at 2^16 above and keeps its 11 bits down to 2^-14: with the
+// factor weights from 2^-21 of the reference on are rounded by half a step at most, and smaller ones by 2^-32.
+template <int TYPE>
+constexpr float kLift = TYPE == SATORI_F16 ? 7.0f : 0.0f;
 
 template <int HD>
 struct Layout {
@@ -909,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) tensor_attention_kernel(const Ten
                         }
                         if (raise) ref = high;
                     }
-                    const float base = ref == -INFINITY ? 0.0f : ref;
+                    const float base = (ref == -INFINITY ? 0.0f : ref) - kLift<TYPE>;
                     uint32_t p[16];
                     // A masked key's weight is exactly zero, which the polynomial cannot give.
                     sum += masked ? block_weights<TYPE, 0>(s, a.scale_log2, base, p)

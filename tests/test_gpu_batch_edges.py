@@ -113,6 +113,32 @@ def test_a_nan_key_alone_in_its_record(env, kind, dim, n):  # noqa: F811
     assert np.array_equal(np.isnan(got).all((2, 3)), nan) and np.isfinite(got[~nan]).all()
 
 
+def test_small_weights_beside_fp16_pages(env):  # noqa: F811
+    """8192 keys of weight 2^-26 beside one of weight 1: together they are 2^-13 of the row.  A weight is rounded to fp16
+    from 2^7 times itself, so by at most 2^-12 of it or 2^-32 (half a subnormal step of 2^-24, over 2^7)."""
+    torch = env[1]
+    n, kv, dim = 37, 4, 64                                     # 148 tiles: an SM works through most of a row's keys
+    m = Model(env, "f16", dim, kv, 4, 64, pages=n * 129, layers=1)
+    seqs = m.cache.create(n)
+    m.cache.extend(seqs, [8192] * n)
+    m.batch.step(seqs, [1] * n)
+    first_pages = [int(m.cache.table(s)[0]) for s in seqs]
+    assert first_pages == [128 * i for i in range(n)]          # the last page of each lies behind all of these
+    q = torch.zeros((n, kv * 4, dim), dtype=m.dtype, device="cuda")
+    q[..., 0] = 26 * math.log(2) * 8
+    weight = math.exp(-float(q[0, 0, 0]) / 8)
+    exact = 8192 * weight / (1 + 8192 * weight)
+    tol = 8192 * (2.0 ** -12 * weight + 2.0 ** -32) + (2 * 68 * 19 + 2 * 8209) * U * exact
+    for heavy in (0, 5000, 8191):                              # where the heavy key lies
+        m.pool[:, :, 0].zero_()
+        m.pool[:, :, 1].fill_(1.0)
+        pages = torch.tensor(first_pages, device="cuda") + heavy // 64
+        m.pool[0, pages, 0, :, heavy % 64, 0] = 1.0
+        m.pool[0, pages, 1, :, heavy % 64] = 0.0
+        got = _attend(m, 0, q.view(n, -1), n)
+        assert np.all(np.abs(got - exact) <= tol), (heavy, np.abs(got - exact).max(), tol)
+
+
 def test_a_replay_follows_an_assignment_that_outgrows_its_plan(env):  # noqa: F811
     sat, torch, ctx = env
     rows, cols, n = 16, 32, 20000
