@@ -217,7 +217,8 @@ SATORI_API int satori_pages_extend(satori_pages *p, int n, const int *seqs, cons
 SATORI_API int satori_pages_fork(satori_pages *p, int n, const int *parents, const int *positions, int share,
                                  int *children);
 /* Discards the tokens at and after positions[i] (satori_session_rewind for one sequence); a page that the
- * new end cuts is copied first when other sequences share it. */
+ * new end cuts is copied first when other sequences share it (SATORI_ERR_CONTEXT_FULL when the free pages do not
+ * suffice for these copies, unless the call frees more pages than they take). */
 SATORI_API int satori_pages_rewind(satori_pages *p, int n, const int *seqs, const int *positions);
 /* Removes the sequences; pages that no other sequence holds become free. */
 SATORI_API int satori_pages_free(satori_pages *p, int n, const int *seqs);

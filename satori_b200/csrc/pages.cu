@@ -14,6 +14,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <unordered_map>
 
 using namespace satori;
 
@@ -136,6 +137,29 @@ int check_room(satori_pages *p, long long need)
 }
 
 int pages_needed(int tokens, int page_tokens) { return (int)(((long long)tokens + page_tokens - 1) / page_tokens); }
+
+// Whether rewinding the sequences frees more pages than its copies take.
+bool makes_room(const satori_pages *p, int n, const int *seqs, const int *positions)
+{
+    PageTables &tables = const_cast<satori_pages *>(p)->tables;
+    const int pt = tables.page_tokens();
+    std::unordered_map<int, int> fewer;              // page -> references that the call takes away
+    long long gain = 0;
+    for (int i = 0; i < n; ++i) {
+        const PageSequence &s = *tables.find(seqs[i]);
+        for (size_t j = (size_t)pages_needed(positions[i], pt); j < s.pages.size(); ++j)
+            gain += ++fewer[s.pages[j]] == tables.refs(s.pages[j]);
+    }
+    for (int i = 0; i < n; ++i) {
+        if (positions[i] % pt == 0) continue;
+        const int page = tables.find(seqs[i])->pages[positions[i] / pt];
+        int &gone = fewer[page];
+        if (tables.refs(page) - gone == 1) continue;
+        ++gone;                                      // it leaves the page to the others, for a copy
+        --gain;
+    }
+    return gain > 0;
+}
 
 }  // namespace
 
@@ -358,9 +382,10 @@ extern "C" int satori_pages_rewind(satori_pages *p, int n, const int *seqs, cons
             const int whole = positions[i] / pt;
             split += positions[i] % pt && p->tables.refs(s.pages[whole]) > 1;
         }
-        // The pages that this call frees may serve it, but which ones remain shared then is only known
-        // afterwards; asking for them all up front keeps the call all or nothing.
-        if ((rc = check_room(p, split)) || (rc = check_device(p))) return rc;
+        // The pages that this call frees may serve it, and a page may be shared no more when its turn comes: with
+        // too few free pages for the least favourable order, the counts are tried on a copy.
+        if (split > p->tables.free_pages() && !makes_room(p, n, seqs, positions)) return check_room(p, split);
+        if ((rc = check_device(p))) return rc;
         std::vector<int> copies;
         copies.reserve(2 * (size_t)split);
         for (int i = 0; i < n; ++i) {
