@@ -201,6 +201,7 @@ struct CombineShape {
 // then each slice of the threads adds every SLICES-th record, and the slices are added.  Latency bounds it
 // (half a dozen loads one after the other before the first value), so loads go out 8 at a time.
 constexpr int kCombineThreads = 256, kCombineHeads = 8, kCombineChunk = 64, kCombineLinks = 32;
+constexpr int kCombineParts = kCombineHeads * (256 / 4) / (kCombineThreads / 4);       // of an octet's values, at most
 
 template <int TYPE, int SLICES>
 __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const BatchAttn a, const CombineShape c)
@@ -536,8 +537,12 @@ int upload_plan(satori_batch *b)
     head.items = place(p.items, ints);
     head.merges = place(p.merges, ints);
     const size_t rows = record_rows(b);
+    // What the kernels count in 32 bits: records' rows, the merges' units (with a grid's stride behind the last), and
+    // the pairs of the rotation's factors.
+    constexpr long long kUnits = 0x7fffffff - (1 << 20);
+    const long long octets = (b->shape.group + kCombineHeads - 1) / kCombineHeads;
     if (ints > 0x7fffffff || (size_t)p.partials * rows > 0x7fffffff ||
-        (double)p.merges.size() * b->q_heads * b->pages->head_dim > 2e9)
+        (long long)p.merges.size() * octets * kCombineParts > kUnits || (long long)p.head.rows * (b->rotary / 2) > kUnits)
         return set_error(SATORI_ERR_NOT_SUPPORTED, "the step's plan exceeds Int32 limits");
     const size_t record = rows * ((size_t)b->pages->head_dim + 2) * 4;
     const int *old_plan = b->d_plan;

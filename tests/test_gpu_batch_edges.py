@@ -139,6 +139,26 @@ def test_small_weights_beside_fp16_pages(env):  # noqa: F811
         assert np.all(np.abs(got - exact) <= tol), (heavy, np.abs(got - exact).max(), tol)
 
 
+def test_many_merged_rows_of_many_heads(env):  # noqa: F811
+    """16000 rows of 32 KV heads behind a shared prefix: every row and head is merged."""
+    torch = env[1]
+    dim, kv, n, own = 128, 32, 64, 250
+    m = _filled(env, "bf16", dim, kv, 1, 64, 8 + 4 * n, 1, 8)
+    root = m.cache.create(1)
+    m.cache.extend(root, [512])
+    seqs = m.cache.fork(root * n)
+    m.batch.step(seqs, [own] * n)
+    q = m.normal(n * own, kv * dim).to(m.dtype)
+    got = _attend(m, 0, q, n * own)
+    for s in (0, 31, 63):
+        k, v = m.read(seqs[s])[:, 0]
+        for r in (0, 1, 100, 249):
+            t = 512 + r + 1
+            qd = q[s * own + r].double().cpu().numpy().reshape(kv, 1, dim)
+            exact, size, scores = m.formula(qd, k[:t], v[:t])
+            assert np.all(np.abs(got[s * own + r] - exact) <= _tolerance(m, t, exact, size, scores)), (s, r)
+
+
 def test_a_replay_follows_an_assignment_that_outgrows_its_plan(env):  # noqa: F811
     sat, torch, ctx = env
     rows, cols, n = 16, 32, 20000
