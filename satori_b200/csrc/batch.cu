@@ -85,7 +85,8 @@ struct AppendArgs {
     int q_heads, kv_heads, head_dim, rotary, page_tokens;
 };
 
-// Loads and stores of 4 values; `wide`: the rows are aligned for one access.
+// Loads and stores of 4 values; `wide`: the rows are aligned for one access.  (Ordinary loads, not the read-only
+// path: q may be rotated in place.)
 template <int TYPE>
 __device__ __forceinline__ void load4(const typename Elem<TYPE>::type *p, bool wide, float *f)
 {
@@ -97,9 +98,9 @@ __device__ __forceinline__ void load4(const typename Elem<TYPE>::type *p, bool w
     } v;
     if (wide) {
         if (TYPE == SATORI_F32)
-            v.f4 = __ldg(reinterpret_cast<const float4 *>(p));
+            v.f4 = *reinterpret_cast<const float4 *>(p);
         else
-            v.u2 = __ldg(reinterpret_cast<const uint2 *>(p));
+            v.u2 = *reinterpret_cast<const uint2 *>(p);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v.t[i] = p[i];
