@@ -274,7 +274,8 @@ typedef struct satori_adapters satori_adapters;
 SATORI_API int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int slots, int max_rank, int type,
                                       satori_adapters **out);
 /* Copies an adapter into a slot (host or device memory; rows lda / ldb elements apart, 0: packed).  rank 0
- * empties the slot.  Synchronous: queued work that reads the slot runs first. */
+ * empties the slot.  Synchronous: queued work that reads the slot runs first.  Adapters are neither created nor changed
+ * inside a stream capture (SATORI_ERR_NOT_SUPPORTED). */
 SATORI_API int satori_adapters_load(satori_adapters *s, int slot, int rank, const void *a, long long lda, const void *b,
                                     long long ldb, float scale);
 SATORI_API int satori_adapters_destroy(satori_adapters *s);

@@ -579,6 +579,16 @@ struct satori_adapter_rows {
 
 namespace {
 
+// A captured change of the weights or slots would be repeated by every replay.
+int check_not_capturing(const satori_ctx *ctx, const char *what)
+{
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(ctx->stream, &status);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+    if (status != cudaStreamCaptureStatusNone) return set_error(SATORI_ERR_NOT_SUPPORTED, "%s inside a stream capture", what);
+    return SATORI_OK;
+}
+
 // How many clusters of each size up to 8 run at once.  The SMs of a GPC hold whole clusters, so it's less than the
 // CTAs' number divided by the cluster's.
 template <typename Kernel>
@@ -672,6 +682,8 @@ extern "C" int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int s
         if (!type_size(type)) return set_error(SATORI_ERR_ARGUMENT, "unsupported type %d", type);
         DeviceScope scope(ctx->device);
         if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+        int rc = check_not_capturing(ctx, "adapters cannot be created");
+        if (rc) return rc;
         satori_adapters *s = new satori_adapters();
         s->ctx = ctx;
         s->rows = rows;
@@ -684,7 +696,7 @@ extern "C" int satori_adapters_create(satori_ctx *ctx, int rows, int cols, int s
         if (e == cudaSuccess) e = cudaMalloc(&s->d_slots, sizeof(SlotDesc) * (size_t)slots);
         if (e == cudaSuccess) e = cudaMemsetAsync(s->d_slots, 0, sizeof(SlotDesc) * (size_t)slots, ctx->stream);
         if (e != cudaSuccess) {
-            int rc = cuda_fail(e, "allocate adapters");
+            rc = cuda_fail(e, "allocate adapters");
             satori_adapters_destroy(s);
             return rc;
         }
@@ -708,6 +720,8 @@ extern "C" int satori_adapters_load(satori_adapters *s, int slot, int rank, cons
     satori_ctx *ctx = s->ctx;
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
+    int rc = check_not_capturing(ctx, "adapters cannot change");
+    if (rc) return rc;
     const size_t es = type_size(s->type), ka = (size_t)s->cols32() * es;
     const int rank16 = (rank + 15) / 16 * 16;
     uint8_t *da = s->d_weights + (size_t)slot * s->a_bytes();
@@ -764,11 +778,9 @@ extern "C" int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const i
         satori_ctx *ctx = r->ctx;
         DeviceScope scope(ctx->device);
         if (scope.status != cudaSuccess) return cuda_fail(scope.status, "cudaSetDevice");
-        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-        cudaError_t e = cudaStreamIsCapturing(ctx->stream, &status);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-        if (status != cudaStreamCaptureStatusNone)
-            return set_error(SATORI_ERR_NOT_SUPPORTED, "rows cannot be assigned inside a stream capture");
+        int rc = check_not_capturing(ctx, "rows cannot be assigned");
+        if (rc) return rc;
+        cudaError_t e = cudaSuccess;
         std::vector<int> order((size_t)n);
         for (int i = 0; i < n; ++i) order[i] = i;
         std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return slots[x] < slots[y]; });

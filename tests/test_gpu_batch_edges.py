@@ -377,3 +377,30 @@ def test_transposed_weights_on_a_context_with_its_own_stream(env):  # noqa: F811
         aset.dispose()
     finally:
         mine.close()
+
+
+def test_adapters_cannot_change_inside_a_capture(env):  # noqa: F811
+    """The refusals leave the capture as it is."""
+    sat, torch, ctx = env
+    aset = sat.AdapterSet(16, 32, 2, 4, dtype="f32", ctx=ctx)
+    a, b = torch.randn((4, 32), device="cuda"), torch.randn((16, 4), device="cuda")
+    aset.load(0, a, b)
+    plan = sat.AdapterRows(ctx)
+    plan.assign([0, -1, 0])
+    x, base = torch.randn((3, 32), device="cuda"), torch.randn((3, 16), device="cuda")
+    out, want = torch.zeros_like(base), torch.zeros_like(base)
+    aset.apply_device(plan, x, base, want)
+    stream = torch.cuda.Stream()
+    with _on_stream(torch, ctx, stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            aset.apply_device(plan, x, base, out)
+            with pytest.raises(sat.NotSupportedError):
+                aset.load(0, a, b)
+            with pytest.raises(sat.NotSupportedError):
+                aset.unload(0)
+            with pytest.raises(sat.NotSupportedError):
+                sat.AdapterSet(16, 32, 1, 4, ctx=ctx)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
