@@ -29,9 +29,18 @@ def _bad(message: str) -> ArgumentError:
 
 
 def _open(ctx) -> bool:
-    """A handle whose context has been closed cannot be destroyed any more: its memory went with the process's
-    use of the context."""
+    """A handle whose context has been closed cannot be used or destroyed any more: its memory went with the
+    process's use of the context."""
     return ctx is None or bool(ctx._h)
+
+
+def _live(h, ctx, what: str):
+    """The handle, while it and its context are open."""
+    if not h:
+        raise DisposedError(_lib.ERR_DISPOSED, f"{what} disposed")
+    if not _open(ctx):
+        raise DisposedError(_lib.ERR_DISPOSED, "context is disposed")
+    return h
 
 
 def _type(dtype) -> int:
@@ -141,9 +150,7 @@ class PagedCache:
 
     @property
     def handle(self):
-        if not self._h:
-            raise DisposedError(_lib.ERR_DISPOSED, "paged cache is disposed")
-        return self._h
+        return _live(self._h, self.ctx, "paged cache is")
 
     def create(self, n: int = 1) -> list:
         """Ids of n new empty sequences."""
@@ -267,9 +274,7 @@ class DecodeBatch:
 
     @property
     def handle(self):
-        if not self._h:
-            raise DisposedError(_lib.ERR_DISPOSED, "batch is disposed")
-        return self._h
+        return _live(self._h, self.cache.ctx, "batch is")
 
     def step(self, seqs, counts) -> None:
         """Extends each sequence by counts[i] new tokens; the step's rows are these tokens in order."""
@@ -345,9 +350,7 @@ class AdapterRows:
 
     @property
     def handle(self):
-        if not self._h:
-            raise DisposedError(_lib.ERR_DISPOSED, "adapter rows are disposed")
-        return self._h
+        return _live(self._h, self.ctx, "adapter rows are")
 
     def assign(self, slots) -> None:
         s = _Ints(slots, "slots")
@@ -389,9 +392,7 @@ class AdapterSet:
 
     @property
     def handle(self):
-        if not self._h:
-            raise DisposedError(_lib.ERR_DISPOSED, "adapters are disposed")
-        return self._h
+        return _live(self._h, self.ctx, "adapters are")
 
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """A [rank, columns] and B [rows, rank]: CUDA tensors or host arrays / CPU tensors of the set's type;

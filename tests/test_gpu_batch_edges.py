@@ -379,6 +379,22 @@ def test_transposed_weights_on_a_context_with_its_own_stream(env):  # noqa: F811
         mine.close()
 
 
+def test_handles_of_a_closed_context(env):  # noqa: F811
+    sat, torch, _ = env
+    mine = sat.Context(0)
+    cache = sat.PagedCache(1, 4, 16, 1, 64, ctx=mine)
+    batch = sat.DecodeBatch(cache, 1)
+    rows, aset = sat.AdapterRows(mine), sat.AdapterSet(8, 8, 1, 4, ctx=mine)
+    s = cache.create(1)
+    mine.close()
+    for call in (lambda: cache.create(1), lambda: cache.fork(s), lambda: batch.step(s, [1]), lambda: rows.assign([0]),
+                 lambda: aset.unload(0), lambda: cache.info()):
+        with pytest.raises(sat.DisposedError):
+            call()
+    for handle in (batch, cache, rows, aset):
+        handle.dispose()
+
+
 def test_adapters_cannot_change_inside_a_capture(env):  # noqa: F811
     """The refusals leave the capture as it is."""
     sat, torch, ctx = env
