@@ -255,9 +255,11 @@ int run_gemv(satori_ctx *ctx, const uint8_t *d_payload, int rows, int cols, int 
             return e == cudaSuccess ? SATORI_OK : cuda_fail(e, "launch bitplane MatVec");
         }
     }
-    const int per_launch = order == SATORI_ORDER_BATCH ? 8 : 1;
-    for (int p0 = 0; p0 < positions; p0 += per_launch) {
-        const int np = std::min(per_launch, positions - p0);
+    // As many positions a launch as have room in shared memory; a position's sums are its own in any case.
+    int per_launch = order == SATORI_ORDER_BATCH ? std::min(8, positions) : 1;
+    while (per_launch > 1 && !plan_gemv(rows, cols, format, per_launch, ctx->sm_count, ctx->smem_optin).ok) --per_launch;
+    for (int p0 = 0, np = 0; p0 < positions; p0 += np) {
+        np = std::min(per_launch, positions - p0);
         if (order == SATORI_ORDER_BATCH && np == 1) {
             // One decode position: the dedicated kernel when the shape qualifies.
             GemvArgs a = {};

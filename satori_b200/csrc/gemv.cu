@@ -30,6 +30,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxRowsPerCta = 64;
 constexpr int kMaxPositions = 8;
+constexpr size_t kStaticSmem = 128;            // of the kernel, which counts against the launch's limit too
 
 __host__ __device__ constexpr int block_bytes_of(int fmt)
 {
@@ -479,17 +480,22 @@ GemvPlan plan_gemv(int rows, int cols, int format, int positions, int sm_count, 
         if (c >= bpr || (size_t)c * rc * BB >= 12288) break;
     }
     cb = std::max(1, std::min(cb, 64));
-    const int seg_stride = ((cb * BB + 32) + 15) & ~15;
-    const int dstride = cb * positions + 1;
+    // Few rows with several positions would take long chunks, whose block terms (dstride) may not fit: a row's terms
+    // are added block by block either way.
     const size_t xbytes = (size_t)positions * bpr * BE * 4;
-    const size_t dbytes = 2ull * kMaxRowsPerCta * dstride * 4;
-    int stages = 4;
+    int stages, seg_stride, dstride;
     size_t smem = 0;
-    for (; stages >= 2; --stages) {
-        smem = 128 + xbytes + dbytes + 128 + (size_t)stages * rc * seg_stride;
-        if (smem <= smem_limit) break;
+    for (;; cb /= 2) {
+        seg_stride = ((cb * BB + 32) + 15) & ~15;
+        dstride = cb * positions + 1;
+        const size_t dbytes = 2ull * kMaxRowsPerCta * dstride * 4;
+        for (stages = 4; stages >= 2; --stages) {
+            smem = 128 + xbytes + dbytes + 128 + (size_t)stages * rc * seg_stride;
+            if (smem + kStaticSmem <= smem_limit) break;
+        }
+        if (stages >= 2) break;
+        if (cb == 1) return p;
     }
-    if (stages < 2) return p;
     p.grid = grid;
     p.threads = kThreads;
     p.rows_per_cta = rc;

@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 def _filled(env, kind, dim, kv_heads, group, page, pages, layers, seed):
     """A model whose pages all hold normal values: nothing has to be appended."""
     m = Model(env, kind, dim, kv_heads, group, page, pages=pages, layers=layers, seed=seed)
-    m.pool.copy_(m.normal(*m.pool.shape).to(m.dtype))
+    m.pool.normal_(generator=m.torch.Generator(device="cuda").manual_seed(seed))
     return m
 
 
@@ -420,3 +420,29 @@ def test_adapters_cannot_change_inside_a_capture(env):  # noqa: F811
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("fmt", ["Q8_0", "Q4_0"])
+@pytest.mark.parametrize("rows,cols", [(512, 3584), (256, 1536), (1000, 18944), (33, 40000)])
+def test_projections_of_several_rows_fit(env, request, fmt, rows, cols):  # noqa: F811
+    """Narrow and long projections of a batch, whose positions or block sums do not all fit shared memory at once:
+    every row has the bits that it has alone."""
+    sat, torch, ctx = env
+    from satori_b200 import _lib
+    n, f = 11, getattr(sat, fmt)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    w = torch.randn(rows * cols, generator=g, device="cuda") * 0.05
+    payload = torch.empty(rows * (cols // 32) * (34 if f == sat.Q8_0 else 18), dtype=torch.uint8, device="cuda")
+    _lib.check(_lib.lib().satori_quantize_q_device(ctx.handle, w.data_ptr(), rows, cols, f, payload.data_ptr()))
+    matrix = sat.CudaQuantizedMatrix.from_device(ctx, payload.data_ptr(), payload.numel(), rows, cols, f)
+    request.addfinalizer(matrix.dispose)
+    x = torch.randn((n, cols), generator=g, device="cuda")
+    alone, together, adapted = (torch.full((n, rows), math.nan, device="cuda") for _ in range(3))
+    for p in range(n):
+        matrix.execute_device(x[p].data_ptr(), alone[p].data_ptr(), 1)
+    matrix.execute_device(x.data_ptr(), together.data_ptr(), n)
+    assert torch.equal(together, alone)
+    aset, plan = sat.AdapterSet(rows, cols, 1, 4, ctx=ctx), sat.AdapterRows(ctx)
+    plan.assign([-1, 0] * 5 + [-1])                           # an empty slot adds nothing either
+    aset.execute_device(matrix, plan, x, adapted)
+    assert torch.equal(adapted, alone)
