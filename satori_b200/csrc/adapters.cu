@@ -16,10 +16,11 @@
 // above 2^-24 of the whole are added in FP32 (3 and 6 MMAs per step).  Beside fp16 weights a row of t, or 32 columns
 // of a row of x, is scaled by a power of two into fp16's range and cut into two fp16 parts (22 bits, or 2^-39 of the
 // largest of them), which meet the weights as they are: 2 MMAs and no conversions.  Bytes bound it: the weights
-// of the slots in use, x, base and out.  While outputs are written they move at 5.1 to 5.9 TB/s (4000 rows of 3
-// slots, rank 64, 1536 -> 8960 in bf16, 56 of 98 us; 128 rows of 32 slots, 3584 -> 18944 in fp16, 17 of 40 us); the
-// first product before it is bound by its instructions (the parts of x and of the weights).  B streams through a ring of each warp's own in shared memory, filled by bulk
-// copies a run or more ahead: a run's weights are contiguous, and the loads' latency was what the warps waited for.
+// of the slots in use, x, base and out.  While outputs are written they move at 5.1 TB/s for 4000 rows of 3 slots (rank
+// 64, 1536 -> 8960 in bf16, 56 of 97 us) and at 4.2 TB/s for 128 rows of 32 slots (3584 -> 18944 in fp16, 72 MB in 17 of
+// 38 us).  Before that come the first product (the parts of x and of the weights) and the chain of loads, barriers and
+// remote reads around it.  B streams through a ring of each warp's own in shared memory, filled by bulk copies a run or
+// more ahead: a run's weights are contiguous, and the loads' latency was what the warps waited for.
 #include "batch.cuh"
 #include "common.cuh"
 #include "paged_internal.h"

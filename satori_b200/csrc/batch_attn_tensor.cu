@@ -22,8 +22,8 @@
 // whose small weights would lose bits, 2^15: see kLift) and the result does not depend on it.  P is rounded to the cache's type (half a step, as the operands already are);
 // S, the sums and O are FP32.
 //
-// What bounds it: HBM for requests of their own (16 of 4096 tokens, 28 heads of 128 over 4: 22 us a CTA, 21 at the rate
-// of HBM, 32 us a call with start and merge).  For large tiles the softmax: a block of 256 rows and 64 keys takes 1750
+// What bounds it: HBM and latencies for requests of their own (16 of exactly 4096 tokens, 28 heads of 128 over 4: 22 us a
+// CTA, 20.8 at the rate of HBM, 35 us a call with start and merge).  For large tiles the softmax: a block of 256 rows and 64 keys takes 1750
 // clocks with heads of 128 (64 requests behind 131072 tokens, 137 us) and 2000 with heads of 64, of which the
 // exponentials' unit is busy 770 and the tensor pipe half; four warps a scheduler wait on chains of their own.  An item
 // of one block takes about 6000 clocks, two at a time: 512 requests of one token 96 us.

@@ -338,7 +338,8 @@ class DecodeBatch:
 
 
 class AdapterRows:
-    """Which adapter slot each row of a batch uses (-1: none), for all projections of a step."""
+    """Which adapter slot each row of a batch uses (-1: none), for all projections of a step; for adapter sets of the
+    same context."""
 
     def __init__(self, ctx: Context | None = None):
         self._h = _vp()
