@@ -281,8 +281,8 @@ SATORI_API int satori_adapters_load(satori_adapters *s, int slot, int rank, cons
 SATORI_API int satori_adapters_destroy(satori_adapters *s);
 /* Which slot each row of a batch uses (-1: none), for all projections of a step.  Captured applications may
  * be replayed after the next assignment when their row buffers are large enough for its rows; a row whose slot the
- * applied adapters do not have then gets its base alone, and the next satori_synchronize reports
- * SATORI_ERR_ARGUMENT.  Assignments, applications and replays run one after another on the context's stream. */
+ * applied adapters do not have then gets its base alone, and satori_synchronize reports SATORI_ERR_ARGUMENT once (a
+ * synchronous call of the context in between clears the report).  Assignments, applications and replays run one after another on the context's stream. */
 typedef struct satori_adapter_rows satori_adapter_rows;
 SATORI_API int satori_adapter_rows_create(satori_ctx *ctx, satori_adapter_rows **out);
 SATORI_API int satori_adapter_rows_assign(satori_adapter_rows *r, int n, const int *slots);
